@@ -34,6 +34,10 @@ int fail(int code, const char* format, ...) {
     return code;
 }
 
+void clear_error() {
+    t_last_error.clear();
+}
+
 int check_launch(const char* what) {
     const hipError_t status = hipGetLastError();
     if (status != hipSuccess) {
@@ -103,6 +107,8 @@ void rln_zero_parameters_kernel(float* __restrict__ grad_weight, float* __restri
     }
 }
 
+}  // namespace
+
 // Compute units of the current device, looked up once per device (0 when
 // the runtime cannot say; the forward then keeps its device-independent grid).
 int compute_units() {
@@ -125,6 +131,8 @@ int compute_units() {
     });
     return units[device];
 }
+
+namespace {
 
 bool aligned_to(const void* pointer, uintptr_t alignment) {
     return pointer == nullptr || (reinterpret_cast<uintptr_t>(pointer) & (alignment - 1)) == 0;
@@ -182,6 +190,8 @@ int check_common(int64_t rows, int64_t hidden, int branch_dtype) {
     return RLN_OK;
 }
 
+}  // namespace
+
 // A non-default stream must belong to the calling thread's current device:
 // the launch shapes (the forward's CU count) and rln_backward_noalloc's
 // scratch are those of the current device, and the pointers are on it.
@@ -204,6 +214,8 @@ int check_stream(void* stream) {
     }
     return RLN_OK;
 }
+
+namespace {
 
 // The dropout layout `threads` selects: 0 for this library's; 128, 192 or
 // 256 for the reference's stream of a launch with that many threads per row

@@ -1,0 +1,858 @@
+// Kernels of the root-mean-square norm with the residual's addition, its 8-bit
+// output and its 8-bit checkpoint (include/rln.h, the rln_rms_* entry points).
+//
+// Per row of H values (u the new residual stream, rounded to x's type):
+//
+//   u = x + branch                      r = 1 / sqrt(sum(u^2) / H + eps)
+//   normalized = (u * r) * weight
+//   backward: p = gy * weight, c = sum(p * u * r) / H,
+//             g = gu + r * (p - u * r * c),   grad_weight = sum_rows gy * u * r
+//
+// 8-bit outputs take steps of v = u * weight against the largest |v| of each
+// group of columns. Since r is one positive factor of the whole row, it goes
+// into the scale alone: code = round(v * (Q / max|v|)), scale = max|v| / Q * r.
+// The codes therefore depend on no sum (they are the same for every split of a
+// row over lanes), and the maximum and the sum of squares are taken in the same
+// pass over the row. The 8-bit checkpoint of u does the same with u itself.
+//
+// Every pass is bound by memory (under 20 fp32 operations per element against
+// 5-20 bytes), so a row is read once into registers, reduced there, and written
+// from there. A row belongs to `parts` waves; vector j of the row (8 columns of
+// a 16-bit stream, 4 of a 32-bit one: 16 bytes of the stream per lane) sits in
+// slot v of lane l of part p with j = (v * parts + p) * 64 + l. `parts` is a
+// run-time value, so any row length gets a team without idle waves.
+//
+// Any row length, row stride and element alignment is served by the same
+// vector accesses: the hardware takes 128-bit global accesses at element
+// alignment, and only the one vector that crosses the end of a row falls back
+// to element accesses (Tail instances, for lengths no multiple of the vector).
+#ifndef RMS_DEVICE_H
+#define RMS_DEVICE_H
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "rln.h"
+
+namespace rln {
+
+// Defined in rln_api.hip.
+int fail(int code, const char* format, ...);
+int check_launch(const char* what);
+int check_stream(void* stream);
+void clear_error();
+int compute_units();
+
+namespace rms {
+
+using half_t = _Float16;
+using bf16_t = __bf16;
+// Tag of a forward without a branch (the first norm of a stack): u = x, which
+// is not written again.
+struct NoBranch {};
+
+constexpr int kWave = 64;
+constexpr int64_t kMaxHidden = 16384;
+constexpr int kMaxParts = 16;
+constexpr int kCheckpointGroup = 128;
+// The least maximum of a group: keeps Q / max finite where a group is all
+// zeros (or below 2^-100, far under any value a norm is fed).
+constexpr float kLeastMaximum = 0x1p-100f;
+
+// 16 bytes of the stream per lane and slot.
+template <typename X>
+constexpr int kColumns = 16 / static_cast<int>(sizeof(X));
+
+enum class Mode { kNormalize, kCheckpoint, kQuantize };
+
+struct ForwardArgs {
+    const void* x;
+    const void* branch;
+    const void* weight;
+    void* updated;
+    void* normalized;   // or the codes
+    float* rstd;        // may be null
+    int8_t* checkpoint;
+    float* scale;       // of the checkpoint or of the codes
+    int64_t x_stride;
+    int64_t branch_stride;
+    int64_t rows;
+    int hidden;
+    int parts;
+    int weight_dtype;
+    int output_dtype;   // normalized's, or the codes'
+    int group;          // columns under one scale, a multiple of the vector
+    int groups;         // scales per row
+    float eps;
+    float inv_hidden;
+};
+
+struct BackwardArgs {
+    const void* grad_updated;  // may be null
+    const void* grad_normalized;
+    const void* updated;
+    const int8_t* checkpoint;
+    const float* scale;
+    const void* weight;
+    const float* rstd;
+    void* grad_x;
+    void* grad_branch;  // null where it equals grad_x
+    float* partials;    // [blocks][hidden], null without the weight's gradient
+    int64_t updated_stride;
+    int64_t rows;
+    int hidden;
+    int parts;
+    int groups;
+    int weight_dtype;
+    int branch_dtype;
+    float inv_hidden;
+};
+
+// ----------------------------------------------------------------------------
+// Vectors of N elements as raw words, at element alignment.
+
+template <int Words, int Alignment>
+struct Words_;
+#define RMS_WORDS(count, alignment)                                                     \
+    template <>                                                                         \
+    struct Words_<count, alignment> {                                                   \
+        typedef uint32_t plain __attribute__((ext_vector_type(count)));                 \
+        typedef plain type __attribute__((aligned(alignment)));                         \
+    }
+RMS_WORDS(4, 4);
+RMS_WORDS(4, 2);
+RMS_WORDS(2, 4);
+RMS_WORDS(2, 2);
+RMS_WORDS(2, 1);
+#undef RMS_WORDS
+template <>
+struct Words_<1, 1> {
+    typedef uint32_t plain;
+    typedef uint32_t type __attribute__((aligned(1)));
+};
+
+// N elements of T as 32-bit words.
+template <typename T, int N>
+struct Raw {
+    static constexpr int kWords = N * static_cast<int>(sizeof(T)) / 4;
+    uint32_t words[kWords];
+};
+
+// Elements [column, column + N) of a row of `hidden`, zeros past its end. Rows
+// pass once, with the non-temporal hint; the weight (Once = false) stays cached.
+template <bool Tail, typename T, int N, bool Once = true>
+__device__ __forceinline__ Raw<T, N> load(const T* __restrict__ row, int column, int hidden) {
+    Raw<T, N> raw;
+    constexpr int kWords = Raw<T, N>::kWords;
+    constexpr int kChunk = kWords < 4 ? kWords : 4;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+        raw.words[i] = 0;
+    }
+    if (column + N <= hidden) {
+        using W = Words_<kChunk, static_cast<int>(sizeof(T))>;
+#pragma unroll
+        for (int i = 0; i < kWords; i += kChunk) {
+            const typename W::type* from =
+                reinterpret_cast<const typename W::type*>(row + column) + i / kChunk;
+            typename W::plain words;
+            if constexpr (Once) {
+                words = __builtin_nontemporal_load(from);
+            } else {
+                words = *from;
+            }
+            if constexpr (kChunk == 1) {
+                raw.words[i] = words;
+            } else {
+#pragma unroll
+                for (int k = 0; k < kChunk; ++k) {
+                    raw.words[i + k] = words[k];
+                }
+            }
+        }
+    } else if constexpr (Tail) {
+        constexpr int kPerWord = 4 / static_cast<int>(sizeof(T));
+#pragma unroll
+        for (int e = 0; e < N - 1; ++e) {
+            if (column + e < hidden) {
+                uint32_t bits;
+                if constexpr (sizeof(T) == 4) {
+                    bits = reinterpret_cast<const uint32_t*>(row)[column + e];
+                } else if constexpr (sizeof(T) == 2) {
+                    bits = reinterpret_cast<const uint16_t*>(row)[column + e];
+                } else {
+                    bits = reinterpret_cast<const uint8_t*>(row)[column + e];
+                }
+                raw.words[e / kPerWord] |= bits << (e % kPerWord * 8 * static_cast<int>(sizeof(T)));
+            }
+        }
+    }
+    return raw;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void widen(const Raw<T, N>& raw, float (&out)[N]) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        if constexpr (sizeof(T) == 4) {
+            out[e] = __builtin_bit_cast(float, raw.words[e]);
+        } else if constexpr (__is_same(T, bf16_t)) {
+            const uint32_t word = raw.words[e / 2];
+            out[e] = __builtin_bit_cast(float, e % 2 ? word & 0xffff0000u : word << 16);
+        } else if constexpr (__is_same(T, half_t)) {
+            const uint32_t word = raw.words[e / 2];
+            out[e] = static_cast<float>(__builtin_bit_cast(
+                half_t, static_cast<uint16_t>(e % 2 ? word >> 16 : word & 0xffffu)));
+        } else {  // int8_t
+            const uint32_t word = raw.words[e / 4];
+            out[e] = static_cast<float>(static_cast<int8_t>(word >> (e % 4 * 8)));
+        }
+    }
+}
+
+// Each value rounded once to T, to nearest even.
+template <typename T, int N>
+__device__ __forceinline__ Raw<T, N> narrow(const float (&values)[N]) {
+    Raw<T, N> raw;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            raw.words[e] = __builtin_bit_cast(uint32_t, values[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const T low = static_cast<T>(values[e]);
+            const T high = static_cast<T>(values[e + 1]);
+            raw.words[e / 2] = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, low))
+                | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, high)) << 16;
+        }
+    }
+    return raw;
+}
+
+template <bool Tail, typename T, int N>
+__device__ __forceinline__ void store(T* __restrict__ row, int column, int hidden,
+                                      const Raw<T, N>& raw) {
+    constexpr int kWords = Raw<T, N>::kWords;
+    constexpr int kChunk = kWords < 4 ? kWords : 4;
+    if (column + N <= hidden) {
+        using W = Words_<kChunk, static_cast<int>(sizeof(T))>;
+#pragma unroll
+        for (int i = 0; i < kWords; i += kChunk) {
+            typename W::plain words;
+            if constexpr (kChunk == 1) {
+                words = raw.words[i];
+            } else {
+#pragma unroll
+                for (int k = 0; k < kChunk; ++k) {
+                    words[k] = raw.words[i + k];
+                }
+            }
+            reinterpret_cast<typename W::type*>(row + column)[i / kChunk] = words;
+        }
+    } else if constexpr (Tail) {
+        constexpr int kPerWord = 4 / static_cast<int>(sizeof(T));
+#pragma unroll
+        for (int e = 0; e < N - 1; ++e) {
+            if (column + e < hidden) {
+                const uint32_t bits =
+                    raw.words[e / kPerWord] >> (e % kPerWord * 8 * static_cast<int>(sizeof(T)));
+                if constexpr (sizeof(T) == 4) {
+                    reinterpret_cast<uint32_t*>(row)[column + e] = bits;
+                } else if constexpr (sizeof(T) == 2) {
+                    reinterpret_cast<uint16_t*>(row)[column + e] = static_cast<uint16_t>(bits);
+                } else {
+                    reinterpret_cast<uint8_t*>(row)[column + e] = static_cast<uint8_t>(bits);
+                }
+            }
+        }
+    }
+}
+
+// The weight and the outputs choose their type at run time: a wave-uniform
+// branch, where a template parameter would multiply the instances by three.
+template <bool Tail, int N>
+__device__ __forceinline__ void load_weight(const void* weight, int dtype, int column, int hidden,
+                                            float (&out)[N]) {
+    if (dtype == RLN_DTYPE_F32) {
+        widen<float, N>(
+            load<Tail, float, N, false>(static_cast<const float*>(weight), column, hidden), out);
+    } else if (dtype == RLN_DTYPE_F16) {
+        widen<half_t, N>(
+            load<Tail, half_t, N, false>(static_cast<const half_t*>(weight), column, hidden), out);
+    } else {
+        widen<bf16_t, N>(
+            load<Tail, bf16_t, N, false>(static_cast<const bf16_t*>(weight), column, hidden), out);
+    }
+}
+
+template <bool Tail, int N>
+__device__ __forceinline__ void store_as(void* tensor, int dtype, int64_t first, int column,
+                                         int hidden, const float (&values)[N]) {
+    if (dtype == RLN_DTYPE_F32) {
+        store<Tail, float, N>(static_cast<float*>(tensor) + first, column, hidden,
+                              narrow<float, N>(values));
+    } else if (dtype == RLN_DTYPE_F16) {
+        store<Tail, half_t, N>(static_cast<half_t*>(tensor) + first, column, hidden,
+                               narrow<half_t, N>(values));
+    } else {
+        store<Tail, bf16_t, N>(static_cast<bf16_t*>(tensor) + first, column, hidden,
+                               narrow<bf16_t, N>(values));
+    }
+}
+
+// ----------------------------------------------------------------------------
+// 8-bit codes.
+
+// Round to nearest even, clipped to +-127.
+template <int N>
+__device__ __forceinline__ Raw<int8_t, N> narrow_int8(const float (&steps)[N]) {
+    Raw<int8_t, N> raw;
+#pragma unroll
+    for (int w = 0; w < N / 4; ++w) {
+        uint32_t word = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float whole = __builtin_rintf(steps[4 * w + e]);
+            const int code = static_cast<int>(__builtin_fminf(__builtin_fmaxf(whole, -127.0f), 127.0f));
+            word |= (static_cast<uint32_t>(code) & 0xffu) << (8 * e);
+        }
+        raw.words[w] = word;
+    }
+    return raw;
+}
+
+// e4m3 (OCP, the hardware's conversion rounds to nearest even), clipped to +-448.
+template <int N>
+__device__ __forceinline__ Raw<int8_t, N> narrow_e4m3(const float (&steps)[N]) {
+    Raw<int8_t, N> raw;
+    float clipped[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        clipped[e] = __builtin_fminf(__builtin_fmaxf(steps[e], -448.0f), 448.0f);
+    }
+#pragma unroll
+    for (int w = 0; w < N / 4; ++w) {
+        int word = __builtin_amdgcn_cvt_pk_fp8_f32(clipped[4 * w], clipped[4 * w + 1], 0, false);
+        word = __builtin_amdgcn_cvt_pk_fp8_f32(clipped[4 * w + 2], clipped[4 * w + 3], word, true);
+        raw.words[w] = static_cast<uint32_t>(word);
+    }
+    return raw;
+}
+
+template <int N>
+__device__ __forceinline__ void widen_e4m3(const Raw<int8_t, N>& raw, float (&out)[N]) {
+#pragma unroll
+    for (int w = 0; w < N / 4; ++w) {
+        const int word = static_cast<int>(raw.words[w]);
+        out[4 * w] = __builtin_amdgcn_cvt_f32_fp8(word, 0);
+        out[4 * w + 1] = __builtin_amdgcn_cvt_f32_fp8(word, 1);
+        out[4 * w + 2] = __builtin_amdgcn_cvt_f32_fp8(word, 2);
+        out[4 * w + 3] = __builtin_amdgcn_cvt_f32_fp8(word, 3);
+    }
+}
+
+// Bits of |value|: as unsigned integers they order like the magnitudes, with
+// every NaN above infinity, so an integer maximum lets a NaN through (a
+// floating one drops it).
+__device__ __forceinline__ uint32_t magnitude_bits(float value) {
+    return __builtin_bit_cast(uint32_t, value) & 0x7fffffffu;
+}
+
+struct GroupScale {
+    float inverse;  // steps per unit
+    float step;     // units per step
+};
+
+// Q / max and max / Q, each rounded once (correctly rounded divisions). A group
+// that holds an infinity or a NaN gets NaN for its step: its values widen to NaN.
+__device__ __forceinline__ GroupScale group_scale(uint32_t maximum_bits, float top) {
+    const float maximum = __builtin_fmaxf(__builtin_bit_cast(float, maximum_bits), kLeastMaximum);
+    GroupScale scale{top / maximum, maximum / top};
+    if (maximum_bits >= 0x7f800000u) {
+        scale = GroupScale{0.0f, __builtin_bit_cast(float, 0x7fc00000u)};
+    }
+    return scale;
+}
+
+// ----------------------------------------------------------------------------
+// Reductions.
+
+#define RMS_DPP(value, control) \
+    __builtin_amdgcn_update_dpp(0, static_cast<int>(value), (control), 0xF, 0xF, false)
+constexpr int kXor1 = 0xB1;         // quad_perm:[1,0,3,2]
+constexpr int kXor2 = 0x4E;         // quad_perm:[2,3,0,1]
+constexpr int kHalfMirror = 0x141;  // within 8 lanes
+constexpr int kMirror = 0x140;      // within 16 lanes
+
+// Sum over the wave's 64 lanes, the same value in every lane.
+__device__ __forceinline__ float wave_sum(float value) {
+#define RMS_ADD(control) \
+    value += __builtin_bit_cast(float, RMS_DPP(__builtin_bit_cast(uint32_t, value), control))
+    RMS_ADD(kXor1);
+    RMS_ADD(kXor2);
+    RMS_ADD(kHalfMirror);
+    RMS_ADD(kMirror);
+#undef RMS_ADD
+    const int bits = __builtin_bit_cast(int, value);
+    const float low = __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 0))
+        + __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 16));
+    const float high = __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 32))
+        + __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 48));
+    return low + high;
+}
+
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    return a > b ? a : b;
+}
+
+// Maximum over each aligned run of `lanes` lanes (4, 8, 16, 32 or 64).
+__device__ __forceinline__ uint32_t lanes_max(uint32_t value, int lanes) {
+    value = larger(value, RMS_DPP(value, kXor1));
+    value = larger(value, RMS_DPP(value, kXor2));
+    if (lanes > 4) {
+        value = larger(value, RMS_DPP(value, kHalfMirror));
+    }
+    if (lanes > 8) {
+        value = larger(value, RMS_DPP(value, kMirror));
+    }
+    if (lanes > 16) {
+        value = larger(value, __shfl_xor(value, 16));
+    }
+    if (lanes > 32) {
+        value = larger(value, __shfl_xor(value, 32));
+    }
+    return value;
+}
+
+// The wave's index in its block and, from it, its row team and part.
+struct Team {
+    int wave;
+    int index;  // row team in the block
+    int part;
+    int teams;
+};
+
+__device__ __forceinline__ Team team_of(int parts) {
+    Team team;
+    team.wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    team.index = team.wave / parts;
+    team.part = team.wave - team.index * parts;
+    team.teams = static_cast<int>(blockDim.x) / (kWave * parts);
+    return team;
+}
+
+// ----------------------------------------------------------------------------
+// Forward: one row per team and turn. The grid covers the rows up to
+// kForwardMaxBlocks (a launch holds fewer than 2^32 threads); past that the
+// teams walk.
+
+template <typename X, typename B, int V, Mode kMode, bool Tail>
+__global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs a) {
+    constexpr int N = kColumns<X>;
+    constexpr bool kBranch = !__is_same(B, NoBranch);
+    __shared__ float sums[2][kMaxParts];
+    __shared__ uint32_t maxima[2][kMaxParts];
+    const Team team = team_of(a.parts);
+    const int lane = threadIdx.x % kWave;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * team.teams;
+    int turn = 0;
+    // Every team of the block makes the same number of turns (a barrier inside).
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * team.teams; base < a.rows;
+         base += step) {
+        const int64_t row = base + team.index;
+        const bool live = row < a.rows;  // the block's last teams may have no row
+        const int hidden = live ? a.hidden : 0;
+        const int64_t first = row * a.hidden;
+        const X* x = static_cast<const X*>(a.x) + row * a.x_stride;
+        int column[V];
+        float u[V][N];
+        Raw<X, N> raw_x[V];
+        float weight[V][N];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            column[v] = ((v * a.parts + team.part) * kWave + lane) * N;
+            raw_x[v] = load<Tail, X, N>(x, column[v], hidden);
+        }
+        if constexpr (kBranch) {
+            const B* branch = static_cast<const B*>(a.branch) + row * a.branch_stride;
+            Raw<B, N> raw_branch[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                raw_branch[v] = load<Tail, B, N>(branch, column[v], hidden);
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                load_weight<Tail, N>(a.weight, a.weight_dtype, column[v], hidden, weight[v]);
+            }
+            X* updated = static_cast<X*>(a.updated) + first;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float added[N];
+                widen<X, N>(raw_x[v], u[v]);
+                widen<B, N>(raw_branch[v], added);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    u[v][e] += added[e];
+                }
+                // The norm is taken of the rounded stream, which is what the
+                // backward and the next layer read.
+                const Raw<X, N> rounded = narrow<X, N>(u[v]);
+                store<Tail, X, N>(updated, column[v], hidden, rounded);
+                widen<X, N>(rounded, u[v]);
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                load_weight<Tail, N>(a.weight, a.weight_dtype, column[v], hidden, weight[v]);
+                widen<X, N>(raw_x[v], u[v]);
+            }
+        }
+
+        float sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                sum += u[v][e] * u[v][e];
+            }
+        }
+        sum = wave_sum(sum);
+        // The 8-bit steps' values: u itself for the checkpoint, u * weight for codes.
+        uint32_t maximum[V];
+        const bool whole_row = kMode == Mode::kQuantize && a.groups == 1;
+        if constexpr (kMode != Mode::kNormalize) {
+            if constexpr (kMode == Mode::kQuantize) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        u[v][e] *= weight[v][e];
+                    }
+                }
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                maximum[v] = 0;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    maximum[v] = larger(maximum[v], magnitude_bits(u[v][e]));
+                }
+            }
+            if (whole_row) {
+                uint32_t whole = maximum[0];
+#pragma unroll
+                for (int v = 1; v < V; ++v) {
+                    whole = larger(whole, maximum[v]);
+                }
+                whole = lanes_max(whole, kWave);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    maximum[v] = whole;
+                }
+            } else {
+                const int lanes = kMode == Mode::kCheckpoint ? kCheckpointGroup / N : a.group / N;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    maximum[v] = lanes_max(maximum[v], lanes);
+                }
+            }
+        }
+        if (a.parts > 1) {
+            // Two buffers: a team's next turn writes the other one while slower
+            // waves still read this one.
+            sums[turn][team.wave] = sum;
+            if (whole_row) {
+                maxima[turn][team.wave] = maximum[0];
+            }
+            __syncthreads();
+            const int begin = team.index * a.parts;
+            sum = 0.0f;
+            for (int part = 0; part < a.parts; ++part) {
+                sum += sums[turn][begin + part];
+            }
+            if (whole_row) {
+                uint32_t whole = 0;
+                for (int part = 0; part < a.parts; ++part) {
+                    whole = larger(whole, maxima[turn][begin + part]);
+                }
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    maximum[v] = whole;
+                }
+            }
+            turn ^= 1;
+        }
+        const float rstd = 1.0f / __builtin_sqrtf(sum * a.inv_hidden + a.eps);
+        if (kMode != Mode::kQuantize && a.rstd != nullptr && live && team.part == 0 && lane == 0) {
+            a.rstd[row] = rstd;
+        }
+        if constexpr (kMode == Mode::kQuantize) {
+            const bool e4m3 = a.output_dtype == RLN_DTYPE_E4M3;
+            const float top = e4m3 ? 448.0f : 127.0f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const GroupScale scale = group_scale(maximum[v], top);
+                if (column[v] < hidden && column[v] % a.group == 0) {
+                    a.scale[row * a.groups + column[v] / a.group] = scale.step * rstd;
+                }
+                float steps[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    steps[e] = u[v][e] * scale.inverse;
+                }
+                store<Tail, int8_t, N>(static_cast<int8_t*>(a.normalized) + first, column[v],
+                                       hidden,
+                                       e4m3 ? narrow_e4m3<N>(steps) : narrow_int8<N>(steps));
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if constexpr (kMode == Mode::kCheckpoint) {
+                    const GroupScale scale = group_scale(maximum[v], 127.0f);
+                    if (column[v] < hidden && column[v] % kCheckpointGroup == 0) {
+                        a.scale[row * a.groups + column[v] / kCheckpointGroup] = scale.step;
+                    }
+                    float steps[N];
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        steps[e] = u[v][e] * scale.inverse;
+                    }
+                    store<Tail, int8_t, N>(a.checkpoint + first, column[v], hidden,
+                                           narrow_int8<N>(steps));
+                }
+                float normalized[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    normalized[e] = u[v][e] * rstd * weight[v][e];
+                }
+                store_as<Tail, N>(a.normalized, a.output_dtype, first, column[v], hidden,
+                                  normalized);
+            }
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------
+// Backward: a block's teams walk the rows block by block; each lane keeps its
+// columns' share of the weight's gradient in registers, the block adds its
+// teams' shares through LDS and writes them to its row of the partials, which
+// reduce_kernel adds in a fixed order (no atomics: the same bits on every run).
+
+template <typename X, typename Y, int V, bool Checkpoint, bool Tail>
+__global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArgs a) {
+    constexpr int N = kColumns<X>;
+    extern __shared__ float shares[];  // [teams - 1][hidden], the weight's gradient
+    __shared__ float sums[2][kMaxParts];
+    const Team team = team_of(a.parts);
+    const int lane = threadIdx.x % kWave;
+    int column[V];
+    float weight[V][N];
+    float grad_weight[V][N];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        column[v] = ((v * a.parts + team.part) * kWave + lane) * N;
+        load_weight<Tail, N>(a.weight, a.weight_dtype, column[v], a.hidden, weight[v]);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            grad_weight[v][e] = 0.0f;
+        }
+    }
+    const int64_t step = static_cast<int64_t>(gridDim.x) * team.teams;
+    int turn = 0;
+    // Every team of the block makes the same number of turns (barriers inside).
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * team.teams; base < a.rows;
+         base += step) {
+        const int64_t row = base + team.index;
+        const bool live = row < a.rows;
+        const int hidden = live ? a.hidden : 0;
+        const int64_t first = row * a.hidden;
+        Raw<Y, N> raw_y[V];
+        Raw<X, N> raw_u[V];
+        Raw<int8_t, N> raw_kept[V];
+        float kept_step[V];
+        Raw<X, N> raw_grad[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            raw_y[v] = load<Tail, Y, N>(static_cast<const Y*>(a.grad_normalized) + first,
+                                        column[v], hidden);
+            if constexpr (Checkpoint) {
+                raw_kept[v] = load<Tail, int8_t, N>(a.checkpoint + first, column[v], hidden);
+                kept_step[v] = column[v] < hidden
+                    ? a.scale[row * a.groups + column[v] / kCheckpointGroup] : 0.0f;
+            } else {
+                raw_u[v] = load<Tail, X, N>(
+                    static_cast<const X*>(a.updated) + row * a.updated_stride, column[v], hidden);
+            }
+        }
+        if (a.grad_updated != nullptr) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                raw_grad[v] = load<Tail, X, N>(static_cast<const X*>(a.grad_updated) + first,
+                                               column[v], hidden);
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+#pragma unroll
+                for (int i = 0; i < Raw<X, N>::kWords; ++i) {
+                    raw_grad[v].words[i] = 0;
+                }
+            }
+        }
+        const float rstd = live ? a.rstd[row] : 0.0f;
+        float unit[V][N];
+        float product[V][N];
+        float sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float upstream[N];
+            widen<Y, N>(raw_y[v], upstream);
+            if constexpr (Checkpoint) {
+                widen<int8_t, N>(raw_kept[v], unit[v]);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    unit[v][e] = unit[v][e] * kept_step[v];
+                }
+            } else {
+                widen<X, N>(raw_u[v], unit[v]);
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                unit[v][e] *= rstd;
+                product[v][e] = upstream[e] * weight[v][e];
+                sum += product[v][e] * unit[v][e];
+                grad_weight[v][e] += upstream[e] * unit[v][e];
+            }
+        }
+        sum = wave_sum(sum);
+        if (a.parts > 1) {
+            // Two buffers: a team's next turn writes the other one while
+            // slower waves still read this one.
+            sums[turn][team.wave] = sum;
+            __syncthreads();
+            const int begin = team.index * a.parts;
+            sum = 0.0f;
+            for (int part = 0; part < a.parts; ++part) {
+                sum += sums[turn][begin + part];
+            }
+            turn ^= 1;
+        }
+        const float shared = sum * a.inv_hidden;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float gradient[N];
+            widen<X, N>(raw_grad[v], gradient);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                gradient[e] += rstd * (product[v][e] - unit[v][e] * shared);
+            }
+            store<Tail, X, N>(static_cast<X*>(a.grad_x) + first, column[v], hidden,
+                              narrow<X, N>(gradient));
+            if (a.grad_branch != nullptr) {
+                store_as<Tail, N>(a.grad_branch, a.branch_dtype, first, column[v], hidden,
+                                  gradient);
+            }
+        }
+    }
+    if (a.partials == nullptr) {
+        return;
+    }
+    // Teams 1, 2, ... leave their shares; team 0 adds them in that order.
+    if (team.index > 0) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if (column[v] + e < a.hidden) {
+                    shares[(team.index - 1) * a.hidden + column[v] + e] = grad_weight[v][e];
+                }
+            }
+        }
+    }
+    if (team.teams > 1) {
+        __syncthreads();
+    }
+    if (team.index == 0) {
+        float* partial = a.partials + static_cast<int64_t>(blockIdx.x) * a.hidden;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            for (int other = 0; other < team.teams - 1; ++other) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    if (column[v] + e < a.hidden) {
+                        grad_weight[v][e] += shares[other * a.hidden + column[v] + e];
+                    }
+                }
+            }
+            store<Tail, float, N>(partial, column[v], a.hidden, narrow<float, N>(grad_weight[v]));
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------
+// Launch shapes (host).
+
+struct Shape {
+    int slots;  // V
+    int parts;
+    int threads;
+};
+
+// Teams of `parts` waves so that `slots` vectors per lane hold a row.
+inline Shape shape_of(int64_t hidden, int columns, int slots, int least_waves) {
+    const int64_t wave_vectors = (hidden + columns * kWave - 1) / (columns * kWave);
+    while (slots * kMaxParts < wave_vectors) {
+        slots *= 2;
+    }
+    Shape shape;
+    shape.slots = slots;
+    shape.parts = static_cast<int>((wave_vectors + slots - 1) / slots);
+    const int teams = shape.parts >= least_waves ? 1 : least_waves / shape.parts;
+    shape.threads = teams * shape.parts * kWave;
+    return shape;
+}
+
+inline int columns_of(int dtype) {
+    return dtype == RLN_DTYPE_F32 ? 4 : 8;
+}
+
+inline Shape forward_shape(int64_t rows, int64_t hidden, int x_dtype) {
+    static_cast<void>(rows);
+    return shape_of(hidden, columns_of(x_dtype), 1, 4);
+}
+
+inline Shape backward_shape(int64_t hidden, int x_dtype) {
+    return shape_of(hidden, columns_of(x_dtype), 1, 4);
+}
+
+inline int teams_of(const Shape& shape) {
+    return shape.threads / (kWave * shape.parts);
+}
+
+constexpr int64_t kForwardMaxBlocks = 1 << 21;
+constexpr int64_t kBackwardMaxBlocks = 1024;
+
+inline int64_t forward_blocks(int64_t rows, const Shape& shape) {
+    const int64_t blocks = (rows + teams_of(shape) - 1) / teams_of(shape);
+    return blocks < kForwardMaxBlocks ? blocks : kForwardMaxBlocks;
+}
+
+inline int64_t backward_blocks(int64_t rows, const Shape& shape) {
+    const int64_t blocks = (rows + teams_of(shape) - 1) / teams_of(shape);
+    return blocks < kBackwardMaxBlocks ? blocks : kBackwardMaxBlocks;
+}
+
+// Defined in rms_kernels.hip, one translation unit per stream type and pass.
+template <typename X>
+int launch_forward(const ForwardArgs& a, const Shape& shape, int branch_dtype, Mode mode,
+                   hipStream_t stream);
+template <typename X>
+int launch_backward(const BackwardArgs& a, const Shape& shape, int grad_dtype,
+                    hipStream_t stream);
+
+}  // namespace rms
+}  // namespace rln
+
+#endif  // RMS_DEVICE_H

@@ -21,6 +21,8 @@ LIBRARY_PATH = Path(__file__).resolve().parent / "librln_gfx950.so"
 RLN_DTYPE_F32 = 0
 RLN_DTYPE_F16 = 1
 RLN_DTYPE_BF16 = 2
+RLN_DTYPE_INT8 = 3
+RLN_DTYPE_E4M3 = 4
 
 RLN_OK = 0
 RLN_ERR_INVALID = 1
@@ -72,6 +74,27 @@ SIGNATURES = {
     "rln_mask_words": (_I64, [_I64, _I64]),
     "rln_hidden_supported": (ctypes.c_int, [_I64]),
     "rln_supported_hidden_sizes": (ctypes.c_int, [ctypes.POINTER(_I64), ctypes.c_int]),
+    "rln_rms_forward": (
+        ctypes.c_int,
+        [_P, ctypes.c_int, _I64, _P, ctypes.c_int, _I64, _P, ctypes.c_int, _P, _P, ctypes.c_int,
+         _P, _P, _P, _I64, _I64, ctypes.c_double, _P],
+    ),
+    "rln_rms_backward": (
+        ctypes.c_int,
+        [_P, _P, ctypes.c_int, _P, _I64, _P, _P, ctypes.c_int, _P, ctypes.c_int, _P, _P, _P,
+         ctypes.c_int, _P, _I64, _I64, _P, ctypes.c_size_t, _P],
+    ),
+    "rln_rms_backward_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, ctypes.c_int]),
+    "rln_rms_quantize": (
+        ctypes.c_int,
+        [_P, ctypes.c_int, _I64, _P, ctypes.c_int, _I64, _P, ctypes.c_int, _P, _P, ctypes.c_int,
+         _P, _I64, _I64, _I64, ctypes.c_double, _P],
+    ),
+    "rln_dequantize": (
+        ctypes.c_int,
+        [_P, ctypes.c_int, _P, _I64, _P, ctypes.c_int, _I64, _I64, _P],
+    ),
+    "rln_rms_hidden_supported": (ctypes.c_int, [_I64]),
     "rln_last_error": (ctypes.c_char_p, []),
     "rln_target_arch": (ctypes.c_char_p, []),
     "rln_version": (ctypes.c_char_p, []),
@@ -178,3 +201,65 @@ def philox_increment(hidden: int, threads: int = 0) -> int:
 
 def mask_words(rows: int, hidden: int) -> int:
     return int(library().rln_mask_words(rows, hidden))
+
+
+def rms_forward(
+    x, x_dtype, weight, weight_dtype, normalized, normalized_dtype, rows, hidden, eps,
+    branch=None, branch_dtype=RLN_DTYPE_F32, updated=None, rstd=None, checkpoint=None,
+    checkpoint_scale=None, x_stride=None, branch_stride=None, stream=None,
+):
+    """Call ``rln_rms_forward`` with integer device addresses (dense rows where
+    no stride is given); raises RlnError."""
+    _check(
+        library().rln_rms_forward(
+            x, x_dtype, hidden if x_stride is None else x_stride, branch, branch_dtype,
+            hidden if branch_stride is None else branch_stride, weight, weight_dtype, updated,
+            normalized, normalized_dtype, rstd, checkpoint, checkpoint_scale, rows, hidden, eps,
+            stream,
+        )
+    )
+
+
+def rms_backward(
+    grad_updated, grad_normalized, grad_normalized_dtype, x_dtype, weight, weight_dtype, rstd,
+    grad_x, rows, hidden, updated=None, updated_stride=None, checkpoint=None,
+    checkpoint_scale=None, grad_branch=None, branch_dtype=RLN_DTYPE_F32, grad_weight=None,
+    workspace=None, workspace_bytes=0, stream=None,
+):
+    """Call ``rln_rms_backward`` with integer device addresses; raises RlnError."""
+    _check(
+        library().rln_rms_backward(
+            grad_updated, grad_normalized, grad_normalized_dtype, updated,
+            hidden if updated_stride is None else updated_stride, checkpoint, checkpoint_scale,
+            x_dtype, weight, weight_dtype, rstd, grad_x, grad_branch, branch_dtype, grad_weight,
+            rows, hidden, workspace, workspace_bytes, stream,
+        )
+    )
+
+
+def rms_backward_workspace_bytes(rows: int, hidden: int, x_dtype: int) -> int:
+    return int(library().rln_rms_backward_workspace_bytes(rows, hidden, x_dtype))
+
+
+def rms_quantize(
+    x, x_dtype, weight, weight_dtype, quantized, quantized_dtype, scale, group, rows, hidden, eps,
+    branch=None, branch_dtype=RLN_DTYPE_F32, updated=None, x_stride=None, branch_stride=None,
+    stream=None,
+):
+    """Call ``rln_rms_quantize`` with integer device addresses; raises RlnError."""
+    _check(
+        library().rln_rms_quantize(
+            x, x_dtype, hidden if x_stride is None else x_stride, branch, branch_dtype,
+            hidden if branch_stride is None else branch_stride, weight, weight_dtype, updated,
+            quantized, quantized_dtype, scale, group, rows, hidden, eps, stream,
+        )
+    )
+
+
+def dequantize(quantized, quantized_dtype, scale, group, values, values_dtype, rows, hidden,
+               stream=None):
+    """Call ``rln_dequantize`` with integer device addresses; raises RlnError."""
+    _check(
+        library().rln_dequantize(quantized, quantized_dtype, scale, group, values, values_dtype,
+                                 rows, hidden, stream)
+    )

@@ -27,6 +27,9 @@ fused op instead of breaking around it (the reference does not support
   With ``compute_parameters`` false (the backward pass needs neither weight
   nor bias gradient: frozen parameters, or gradients taken for the inputs
   only) the weight/bias sums are skipped and those two outputs are empty.
+* ``gfx1010_kernels::rms_forward`` / ``rms_backward`` / ``rms_quantized`` /
+  ``dequantize`` do the same for the root-mean-square norm
+  (``_C.residual_rms_norm_*``). They draw nothing, so equal calls may be merged.
 """
 
 from __future__ import annotations
@@ -173,4 +176,168 @@ def residual_layer_norm_op(x, branch, weight, bias, dropout_p, eps, training,
     return updated, normalized
 
 
-__all__ = ["rln_backward", "rln_forward", "residual_layer_norm_op"]
+@torch.library.custom_op(f"{_NAMESPACE}::rms_forward", mutates_args=(), device_types="cuda")
+def rms_forward(
+    x: Tensor,
+    branch: Optional[Tensor],
+    weight: Tensor,
+    eps: float,
+    normalized_dtype: Optional[torch.dtype] = None,
+    checkpoint: bool = False,
+) -> tuple[Tensor, Tensor, Tensor]:
+    return _native().residual_rms_norm_forward(x, branch, weight, float(eps), normalized_dtype,
+                                               checkpoint)
+
+
+def _rms_state_bytes(rows, hidden, checkpoint):
+    """Bytes of the state tensor (rstd; with the checkpoint its scales and
+    codes), as rms_torch.cpp lays it out."""
+    if not checkpoint:
+        return 4 * rows
+    groups = (hidden + 127) // 128
+    return (4 * rows + 255) // 256 * 256 + (4 * rows * groups + 255) // 256 * 256 + rows * hidden
+
+
+@rms_forward.register_fake
+def _rms_forward_fake(x, branch, weight, eps, normalized_dtype=None, checkpoint=False):
+    hidden = x.shape[-1]
+    rows = x.numel() // hidden
+    return (
+        x.new_empty((0,)) if branch is None else x.new_empty(x.shape),
+        x.new_empty(x.shape, dtype=normalized_dtype or x.dtype),
+        x.new_empty((_rms_state_bytes(rows, hidden, checkpoint),), dtype=torch.uint8),
+    )
+
+
+@torch.library.custom_op(f"{_NAMESPACE}::rms_backward", mutates_args=(), device_types="cuda")
+def rms_backward(
+    grad_updated: Optional[Tensor],
+    grad_normalized: Tensor,
+    updated: Optional[Tensor],
+    state: Tensor,
+    weight: Tensor,
+    x_dtype: torch.dtype,
+    branch_dtype: Optional[torch.dtype],
+    checkpoint: bool,
+    weight_gradient: bool,
+) -> tuple[Tensor, Tensor, Tensor]:
+    grad_x, grad_branch, grad_weight = _native().residual_rms_norm_backward(
+        grad_updated, grad_normalized, updated, state, weight, x_dtype, branch_dtype, checkpoint,
+        weight_gradient)
+    empty = grad_x.new_empty((0,))
+    return (grad_x, empty if grad_branch is None else grad_branch,
+            empty.clone() if grad_weight is None else grad_weight)
+
+
+@rms_backward.register_fake
+def _rms_backward_fake(grad_updated, grad_normalized, updated, state, weight, x_dtype,
+                       branch_dtype, checkpoint, weight_gradient):
+    own_branch = branch_dtype is not None and branch_dtype != x_dtype
+    return (
+        grad_normalized.new_empty(grad_normalized.shape, dtype=x_dtype),
+        grad_normalized.new_empty(grad_normalized.shape, dtype=branch_dtype) if own_branch
+        else grad_normalized.new_empty((0,), dtype=x_dtype),
+        weight.new_empty(weight.shape) if weight_gradient
+        else grad_normalized.new_empty((0,), dtype=x_dtype),
+    )
+
+
+def _rms_setup_context(ctx, inputs, output):
+    x, branch, weight, _, _, checkpoint = inputs
+    updated, _, state = output
+    kept = None if checkpoint else x if branch is None else updated
+    ctx.save_for_backward(kept, weight, state)
+    ctx.x_dtype = x.dtype
+    ctx.branch_dtype = None if branch is None else branch.dtype
+    ctx.checkpoint = checkpoint
+    ctx.mark_non_differentiable(*([updated, state] if branch is None else [state]))
+    ctx.set_materialize_grads(False)
+
+
+def _rms_backward_formula(ctx, grad_updated, grad_normalized, _grad_state):
+    grads = [None] * 6
+    if grad_normalized is None:
+        if grad_updated is not None:
+            grads[0] = grad_updated
+            grads[1] = grad_updated.to(ctx.branch_dtype)
+        return tuple(grads)
+    kept, weight, state = ctx.saved_tensors
+    grad_x, grad_branch, grad_weight = rms_backward(
+        grad_updated if ctx.branch_dtype is not None else None, grad_normalized, kept, state,
+        weight, ctx.x_dtype, ctx.branch_dtype, ctx.checkpoint, ctx.needs_input_grad[2])
+    grads[0] = grad_x
+    if ctx.branch_dtype is not None:
+        grads[1] = grad_x if ctx.branch_dtype == ctx.x_dtype else grad_branch
+    if ctx.needs_input_grad[2]:
+        grads[2] = grad_weight
+    return tuple(grads)
+
+
+rms_forward.register_autograd(_rms_backward_formula, setup_context=_rms_setup_context)
+
+
+def residual_rms_norm_op(x, branch, weight, eps, normalized_dtype=None, checkpoint=False):
+    """``(updated, normalized)`` through the registered custom op."""
+    updated, normalized, _ = rms_forward(x, branch, weight, float(eps), normalized_dtype,
+                                         checkpoint)
+    return (x if branch is None else updated), normalized
+
+
+@torch.library.custom_op(f"{_NAMESPACE}::rms_quantized", mutates_args=(), device_types="cuda")
+def rms_quantized(
+    x: Tensor,
+    branch: Optional[Tensor],
+    weight: Tensor,
+    eps: float,
+    dtype: torch.dtype,
+    group: int,
+) -> tuple[Tensor, Tensor, Tensor]:
+    updated, quantized, scale = _native().residual_rms_norm_quantized(
+        x, branch, weight, float(eps), dtype, group)
+    return (x.new_empty((0,)) if branch is None else updated), quantized, scale
+
+
+@rms_quantized.register_fake
+def _rms_quantized_fake(x, branch, weight, eps, dtype, group):
+    groups = 1 if group == 0 else (x.shape[-1] + group - 1) // group
+    return (
+        x.new_empty((0,)) if branch is None else x.new_empty(x.shape),
+        x.new_empty(x.shape, dtype=dtype),
+        x.new_empty((*x.shape[:-1], groups), dtype=torch.float32),
+    )
+
+
+def residual_rms_norm_quantized_op(x, branch, weight, eps, dtype, group_size):
+    """``(updated, quantized, scale)`` through the registered custom op."""
+    updated, quantized, scale = rms_quantized(x, branch, weight, float(eps), dtype,
+                                              group_size or 0)
+    return (x if branch is None else updated), quantized, scale
+
+
+@torch.library.custom_op(f"{_NAMESPACE}::dequantize", mutates_args=(), device_types="cuda")
+def dequantize(quantized: Tensor, scale: Tensor, group: int, dtype: torch.dtype) -> Tensor:
+    return _native().dequantize(quantized, scale, group, dtype)
+
+
+@dequantize.register_fake
+def _dequantize_fake(quantized, scale, group, dtype):
+    return quantized.new_empty(quantized.shape, dtype=dtype)
+
+
+def dequantize_op(quantized, scale, group_size, dtype):
+    """The widened values through the registered custom op."""
+    return dequantize(quantized, scale, group_size or 0, dtype)
+
+
+__all__ = [
+    "dequantize",
+    "dequantize_op",
+    "residual_layer_norm_op",
+    "residual_rms_norm_op",
+    "residual_rms_norm_quantized_op",
+    "rln_backward",
+    "rln_forward",
+    "rms_backward",
+    "rms_forward",
+    "rms_quantized",
+]

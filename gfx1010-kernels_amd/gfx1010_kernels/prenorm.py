@@ -13,9 +13,11 @@ This module is that recipe as code:
 * :func:`prenorm_forward` runs a stack of pre-norm blocks
   (``h = ln_1(x); x = x + drop(attn(h)); h = ln_2(x); x = x + drop(mlp(h))``
   per block, then the final norm) with every residual add fused into the
-  LayerNorm after it: a block's ``ln_2`` after its attention, the next
+  norm after it: a block's ``ln_2`` after its attention, the next
   block's ``ln_1`` after its MLP, and the final norm after the last MLP. Only
   the first ``ln_1`` (no residual add before it) runs as a plain LayerNorm.
+
+Both take ``nn.RMSNorm`` modules as well, through ``residual_rms_norm``.
 
 Neither function owns parameters: they read the caller's modules, so a model
 that switches its ``forward`` to them keeps its ``state_dict`` unchanged.
@@ -30,6 +32,7 @@ from torch import nn
 from torch.nn import functional as F
 
 from .normalization import residual_layer_norm
+from .rms_norm import residual_rms_norm
 
 # How a block exposes a sublayer or norm: an attribute name, or a function of
 # the block (and, for sublayers, the normalized input).
@@ -37,25 +40,49 @@ Accessor = Union[str, Callable]
 
 
 def _check_norm(norm: nn.Module, hidden: int) -> None:
-    if not isinstance(norm, nn.LayerNorm):
-        raise TypeError(f"expected torch.nn.LayerNorm, got {type(norm).__name__}")
+    if not isinstance(norm, (nn.LayerNorm, nn.RMSNorm)):
+        raise TypeError(
+            f"expected torch.nn.LayerNorm or torch.nn.RMSNorm, got {type(norm).__name__}")
+    kind = "LayerNorm" if isinstance(norm, nn.LayerNorm) else "RMSNorm"
     if tuple(norm.normalized_shape) != (hidden,):
         raise ValueError(
-            f"LayerNorm normalizes {tuple(norm.normalized_shape)}, the residual stream has "
+            f"{kind} normalizes {tuple(norm.normalized_shape)}, the residual stream has "
             f"hidden size {hidden}")
-    if norm.weight is None or norm.bias is None:
-        raise ValueError("LayerNorm needs elementwise affine weight and bias")
+    if norm.weight is None or (kind == "LayerNorm" and norm.bias is None):
+        raise ValueError(f"{kind} needs elementwise affine weight"
+                         + (" and bias" if kind == "LayerNorm" else ""))
 
 
-def residual_norm(x, branch, norm: nn.LayerNorm, dropout_p: float = 0.0, training: bool = True,
-                  *, implementation: str = "auto", normalized_dtype=None):
+def _rms_norm(x, branch, norm: nn.RMSNorm, dropout_p, training, implementation, normalized_dtype,
+              checkpoint_dtype):
+    if branch is not None and training and dropout_p != 0.0:
+        branch = F.dropout(branch, dropout_p, True)
+    eps = torch.finfo(x.dtype).eps if norm.eps is None else norm.eps
+    return residual_rms_norm(x, branch, norm.weight, eps, implementation=implementation,
+                             normalized_dtype=normalized_dtype, checkpoint_dtype=checkpoint_dtype)
+
+
+def _refuse_checkpoint(checkpoint_dtype) -> None:
+    if checkpoint_dtype is not None:
+        raise ValueError("checkpoint_dtype needs torch.nn.RMSNorm modules")
+
+
+def residual_norm(x, branch, norm: Union[nn.LayerNorm, nn.RMSNorm], dropout_p: float = 0.0,
+                  training: bool = True, *, implementation: str = "auto", normalized_dtype=None,
+                  checkpoint_dtype=None):
     """``x + dropout(branch)`` followed by ``norm``, as one fused operation.
 
-    Returns ``(updated, normalized)`` like ``residual_layer_norm``; ``norm``
-    supplies weight, bias and eps and keeps its parameters (and their
-    ``state_dict`` keys) in the caller's model.
+    Returns ``(updated, normalized)`` like ``residual_layer_norm``, or like
+    ``residual_rms_norm`` for an ``nn.RMSNorm`` (whose dropout, if any, is a
+    separate ``F.dropout``); ``norm`` supplies weight, bias and eps and keeps its
+    parameters (and their ``state_dict`` keys) in the caller's model.
+    ``checkpoint_dtype`` is ``residual_rms_norm``'s.
     """
     _check_norm(norm, x.shape[-1])
+    if isinstance(norm, nn.RMSNorm):
+        return _rms_norm(x, branch, norm, dropout_p, training, implementation, normalized_dtype,
+                         checkpoint_dtype)
+    _refuse_checkpoint(checkpoint_dtype)
     return residual_layer_norm(
         x, branch, norm.weight, norm.bias, dropout_p=dropout_p, eps=norm.eps,
         training=training, implementation=implementation, normalized_dtype=normalized_dtype)
@@ -74,7 +101,7 @@ def _sublayer(block: nn.Module, accessor: Accessor, hidden_states):
 def prenorm_forward(
     x: torch.Tensor,
     blocks: Sequence[nn.Module],
-    final_norm: nn.LayerNorm,
+    final_norm: Union[nn.LayerNorm, nn.RMSNorm],
     *,
     dropout_p: float = 0.0,
     training: bool = True,
@@ -84,6 +111,7 @@ def prenorm_forward(
     ln2: Accessor = "ln_2",
     implementation: str = "auto",
     normalized_dtype=None,
+    checkpoint_dtype=None,
 ):
     """Run pre-norm blocks with fused residual LayerNorms; returns ``(x, out)``.
 
@@ -96,16 +124,27 @@ def prenorm_forward(
     names or functions ``f(block)``). ``normalized_dtype`` (fp16 / bf16)
     rounds every normalized output, including ``out``, for half-precision
     sublayers; the residual stream stays fp32.
+
+    The norms may be ``nn.RMSNorm`` modules instead. The residual stream is then
+    of ``x``'s own type, fp32, fp16 or bf16, which is also the normalized
+    outputs' without ``normalized_dtype``, and ``checkpoint_dtype=torch.int8``
+    keeps each norm's input for the backward in 8 bits
+    (``residual_rms_norm``), so that no norm keeps the stream itself alive.
     """
     if len(blocks) == 0:
         raise ValueError("prenorm_forward needs at least one block")
     hidden = x.shape[-1]
     first = _module(blocks[0], ln1)
     _check_norm(first, hidden)
-    normalized = F.layer_norm(x, (hidden,), first.weight, first.bias, first.eps)
-    if normalized_dtype is not None:
-        normalized = normalized.to(normalized_dtype)
-    options = dict(implementation=implementation, normalized_dtype=normalized_dtype)
+    options = dict(implementation=implementation, normalized_dtype=normalized_dtype,
+                   checkpoint_dtype=checkpoint_dtype)
+    if isinstance(first, nn.RMSNorm):
+        x, normalized = _rms_norm(x, None, first, 0.0, training, **options)
+    else:
+        _refuse_checkpoint(checkpoint_dtype)
+        normalized = F.layer_norm(x, (hidden,), first.weight, first.bias, first.eps)
+        if normalized_dtype is not None:
+            normalized = normalized.to(normalized_dtype)
     for index, block in enumerate(blocks):
         x, normalized = residual_norm(x, _sublayer(block, attention, normalized),
                                       _module(block, ln2), dropout_p, training, **options)

@@ -48,7 +48,10 @@ extern "C" {
 enum rln_dtype {
     RLN_DTYPE_F32 = 0,
     RLN_DTYPE_F16 = 1,
-    RLN_DTYPE_BF16 = 2
+    RLN_DTYPE_BF16 = 2,
+    /* 8-bit codes, of rln_rms_quantize and rln_dequantize only: */
+    RLN_DTYPE_INT8 = 3, /* -127 .. 127 */
+    RLN_DTYPE_E4M3 = 4  /* OCP float8 e4m3 (finite and NaN), +-448 */
 };
 
 enum rln_status {
@@ -255,6 +258,151 @@ int rln_hidden_supported(int64_t hidden);
  * how many exist (the reference's NATIVE_HIDDEN_SIZES,
  * gfx1010_kernels/normalization.py:12). */
 int rln_supported_hidden_sizes(int64_t* out, int capacity);
+
+/*
+ * Root-mean-square norm with the residual's addition. It has no counterpart in
+ * the reference, whose only norm is LayerNorm. Per row of `hidden` elements:
+ *
+ *   updated    = x + branch                       (added in fp32, rounded to x's type)
+ *   rstd       = 1 / sqrt(sum(updated^2) / hidden + eps)
+ *   normalized = updated * rstd * weight          (fp32, rounded to normalized's type)
+ *
+ * x, branch, weight and normalized each use fp32, fp16 or bf16; updated has x's
+ * type. x and branch are rows of consecutive elements, `x_stride` and
+ * `branch_stride` elements apart (any value, 0 for one row read by all);
+ * updated and normalized are dense. Every address is aligned to its elements; more
+ * is not asked. Any hidden from 1 to 16384 (rln_rms_hidden_supported).
+ * branch and updated are both NULL for a norm without an addition (updated = x).
+ * rstd: fp32 [rows] for the backward, or NULL.
+ * checkpoint, checkpoint_scale: both NULL, or the 8-bit checkpoint of updated
+ * for rln_rms_backward: int8 [rows, hidden] and fp32 [rows, ceil(hidden / 128)].
+ * With m = max(|updated|, 2^-100) over a group of 128 columns (the last one
+ * shorter), code = round(updated * (127 / m)) to nearest even and scale = m / 127,
+ * each operation rounded once to fp32. A group that holds an infinity or a NaN
+ * has NaN for its scale.
+ */
+int rln_rms_forward(
+    const void* x,
+    int x_dtype,
+    int64_t x_stride,
+    const void* branch,
+    int branch_dtype,
+    int64_t branch_stride,
+    const void* weight,
+    int weight_dtype,
+    void* updated,
+    void* normalized,
+    int normalized_dtype,
+    float* rstd,
+    int8_t* checkpoint,
+    float* checkpoint_scale,
+    int64_t rows,
+    int64_t hidden,
+    double eps,
+    void* stream);
+
+/*
+ * Backward of rln_rms_forward (no counterpart in the reference). Per row, with
+ * u = updated, or checkpoint * checkpoint_scale where the checkpoint is given:
+ *
+ *   p = grad_normalized * weight
+ *   g = grad_updated + rstd * (p - u * rstd * sum(p * u * rstd) / hidden)
+ *   grad_x = g in x's type, grad_branch = g in the branch's type
+ *   grad_weight = sum over the rows of grad_normalized * u * rstd, in the
+ *                 weight's type, added in fp32 in a fixed order (bitwise
+ *                 reproducible; the library's rln_backward offers both)
+ *
+ * grad_updated (x's type) may be NULL, meaning zero. Gradients are dense;
+ * updated is rows `updated_stride` elements apart. grad_branch may be NULL
+ * (no addition, or a branch of x's type, whose gradient is grad_x itself), and
+ * so may grad_weight. workspace: device scratch of
+ * rln_rms_backward_workspace_bytes(rows, hidden, x_dtype) bytes, aligned to 4
+ * (unused, may be NULL, without grad_weight); nothing in it needs clearing, and
+ * calls that overlap need one each.
+ */
+int rln_rms_backward(
+    const void* grad_updated,
+    const void* grad_normalized,
+    int grad_normalized_dtype,
+    const void* updated,
+    int64_t updated_stride,
+    const int8_t* checkpoint,
+    const float* checkpoint_scale,
+    int x_dtype,
+    const void* weight,
+    int weight_dtype,
+    const float* rstd,
+    void* grad_x,
+    void* grad_branch,
+    int branch_dtype,
+    void* grad_weight,
+    int64_t rows,
+    int64_t hidden,
+    void* workspace,
+    size_t workspace_bytes,
+    void* stream);
+
+/* Workspace bytes rln_rms_backward needs for grad_weight: the per-block sums
+ * of its fixed-order reduction (no counterpart in the reference). */
+size_t rln_rms_backward_workspace_bytes(
+    int64_t rows,
+    int64_t hidden,
+    int x_dtype);
+
+/*
+ * rln_rms_forward with its output in 8 bits (no counterpart in the reference),
+ * for a consumer that multiplies 8-bit activations. quantized: [rows, hidden] in
+ * RLN_DTYPE_INT8 or RLN_DTYPE_E4M3; scale: fp32 [rows, groups], where `group` is the
+ * number of columns under one scale, 32, 64, 128 or 256 (the last group of a
+ * row may be shorter), or 0 for one scale per row. With v = updated * weight in
+ * fp32, m = max(|v|, 2^-100) over the group and Q = 127 or 448:
+ *
+ *   code  = v * (Q / m), rounded to nearest even
+ *   scale = (m / Q) * rstd;    normalized ~ code * scale
+ *
+ * each operation rounded once to fp32: rstd, a factor of the whole row, is in
+ * the scale alone, so the codes do not depend on the order of any sum. A group
+ * that holds an infinity or a NaN has NaN for its scale.
+ */
+int rln_rms_quantize(
+    const void* x,
+    int x_dtype,
+    int64_t x_stride,
+    const void* branch,
+    int branch_dtype,
+    int64_t branch_stride,
+    const void* weight,
+    int weight_dtype,
+    void* updated,
+    void* quantized,
+    int quantized_dtype,
+    float* scale,
+    int64_t group,
+    int64_t rows,
+    int64_t hidden,
+    double eps,
+    void* stream);
+
+/*
+ * values = code * scale of the code's group, rounded to the values' type (fp32,
+ * fp16 or bf16): what rln_rms_quantize wrote, for a consumer that does not read 8
+ * bits (no counterpart in the reference). All tensors are dense; `group` as in
+ * rln_rms_quantize, 1 <= hidden < 2^31 - 4096.
+ */
+int rln_dequantize(
+    const void* quantized,
+    int quantized_dtype,
+    const float* scale,
+    int64_t group,
+    void* values,
+    int values_dtype,
+    int64_t rows,
+    int64_t hidden,
+    void* stream);
+
+/* 1 if the rln_rms_* entry points serve rows of `hidden` values, 1 to 16384,
+ * else 0 (no counterpart in the reference). */
+int rln_rms_hidden_supported(int64_t hidden);
 
 /* Thread-local message for the last failed call on this thread (the text of
  * the reference's TORCH_CHECK messages, csrc/residual_layer_norm_kernel.hip:26-166). */
