@@ -112,7 +112,7 @@ int forward_args(const void* x, int x_dtype, int64_t x_stride, const void* branc
 }
 
 int launch(ForwardArgs& a, int x_dtype, int branch_dtype, Mode mode, void* stream) {
-    const Shape shape = forward_shape(a.rows, a.hidden, x_dtype);
+    const Shape shape = forward_shape(a.hidden, x_dtype);
     a.parts = shape.parts;
     const hipStream_t queue = static_cast<hipStream_t>(stream);
     switch (x_dtype) {
@@ -295,7 +295,7 @@ size_t rln_rms_backward_workspace_bytes(int64_t rows, int64_t hidden, int x_dtyp
     if (rows <= 0 || !rln_rms_hidden_supported(hidden) || !float_dtype(x_dtype)) {
         return 0;
     }
-    return static_cast<size_t>(backward_blocks(rows, backward_shape(hidden, x_dtype)))
+    return static_cast<size_t>(backward_blocks(rows, backward_shape(rows, hidden, x_dtype)))
         * static_cast<size_t>(hidden) * sizeof(float);
 }
 
@@ -343,7 +343,7 @@ int rln_rms_backward(
         || (status = check_alignment("workspace", workspace, RLN_DTYPE_F32)) != RLN_OK) {
         return status;
     }
-    const Shape shape = backward_shape(hidden, x_dtype);
+    const Shape shape = backward_shape(rows, hidden, x_dtype);
     const size_t needed = grad_weight != nullptr
         ? rln_rms_backward_workspace_bytes(rows, hidden, x_dtype) : 0;
     if (needed > 0 && (workspace == nullptr || workspace_bytes < needed)) {

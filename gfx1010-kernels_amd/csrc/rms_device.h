@@ -792,7 +792,23 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 }
 
 // ----------------------------------------------------------------------------
-// Launch shapes (host).
+// Launch shapes (host). Measured on MI355X, graphs of launches over buffers that
+// pass the caches, TB/s of algorithmic bytes (a large copy reaches 5.4):
+//
+//  * 16 bytes of the stream per lane and slot. A 16-bit stream takes one slot
+//    while a row fits 8 waves of them ([16384, 4096] bf16: forward 6.0 against
+//    5.7 with two slots, backward 5.9 against 5.6), a 32-bit one two, whose
+//    half as many waves then read as much of a 16-bit branch ([32768, 2048]
+//    int8 in groups: 5.9 against 5.6).
+//  * The forward doubles the slots until a row fits 8 waves: blocks of 16 waves
+//    leave a CU idle while they wait for each other ([8192, 8192] fp32 with the
+//    checkpoint: 5.6 with four slots and 8 waves, 5.2 with two and 16). Rows over
+//    8192 columns take 16 waves.
+//  * The backward's grid is what the chip holds at 16 waves per CU, in blocks of 8
+//    waves: fewer leave the memory idle ([16384, 4096] bf16: 101 us at 8 per CU,
+//    91 at 16), more only add partial sums of the weight's gradient (108). Short
+//    launches, less than two rows per team, keep one slot, so that more
+//    teams share the rows ([1024, 384]: 7.4 against 8.9 us).
 
 struct Shape {
     int slots;  // V
@@ -800,48 +816,65 @@ struct Shape {
     int threads;
 };
 
-// Teams of `parts` waves so that `slots` vectors per lane hold a row.
-inline Shape shape_of(int64_t hidden, int columns, int slots, int least_waves) {
-    const int64_t wave_vectors = (hidden + columns * kWave - 1) / (columns * kWave);
-    while (slots * kMaxParts < wave_vectors) {
-        slots *= 2;
-    }
-    Shape shape;
-    shape.slots = slots;
-    shape.parts = static_cast<int>((wave_vectors + slots - 1) / slots);
-    const int teams = shape.parts >= least_waves ? 1 : least_waves / shape.parts;
-    shape.threads = teams * shape.parts * kWave;
-    return shape;
-}
-
 inline int columns_of(int dtype) {
     return dtype == RLN_DTYPE_F32 ? 4 : 8;
 }
 
-inline Shape forward_shape(int64_t rows, int64_t hidden, int x_dtype) {
-    static_cast<void>(rows);
-    return shape_of(hidden, columns_of(x_dtype), 1, 4);
+// Waves that one slot per lane needs for a row.
+inline int64_t wave_vectors(int64_t hidden, int x_dtype) {
+    const int columns = columns_of(x_dtype) * kWave;
+    return (hidden + columns - 1) / columns;
 }
 
-inline Shape backward_shape(int64_t hidden, int x_dtype) {
-    return shape_of(hidden, columns_of(x_dtype), 1, 4);
+// Teams of the fewest waves that hold a row at `slots` vectors per lane, at
+// least `least_waves` in a block.
+inline Shape shape_of(int64_t vectors, int slots, int least_waves) {
+    Shape shape;
+    shape.slots = slots;
+    shape.parts = static_cast<int>((vectors + slots - 1) / slots);
+    const int teams = shape.parts >= least_waves ? 1 : least_waves / shape.parts;
+    shape.threads = teams * shape.parts * kWave;
+    return shape;
 }
 
 inline int teams_of(const Shape& shape) {
     return shape.threads / (kWave * shape.parts);
 }
 
+inline Shape forward_shape(int64_t hidden, int x_dtype) {
+    const int64_t vectors = wave_vectors(hidden, x_dtype);
+    const int most = x_dtype == RLN_DTYPE_F32 ? 4 : 2;
+    int slots = x_dtype == RLN_DTYPE_F32 && vectors > 1 ? 2 : 1;
+    while (slots < most && slots * 8 < vectors) {
+        slots *= 2;
+    }
+    return shape_of(vectors, slots, 4);
+}
+
 constexpr int64_t kForwardMaxBlocks = 1 << 21;
-constexpr int64_t kBackwardMaxBlocks = 1024;
 
 inline int64_t forward_blocks(int64_t rows, const Shape& shape) {
     const int64_t blocks = (rows + teams_of(shape) - 1) / teams_of(shape);
     return blocks < kForwardMaxBlocks ? blocks : kForwardMaxBlocks;
 }
 
+// 256 CUs of 16 waves.
+constexpr int64_t kBackwardWaves = 4096;
+
+inline Shape backward_shape(int64_t rows, int64_t hidden, int x_dtype) {
+    const int64_t vectors = wave_vectors(hidden, x_dtype);
+    int slots = x_dtype == RLN_DTYPE_F32 && vectors > 1 && rows >= 2 * kBackwardWaves / vectors
+        ? 2 : 1;
+    while (slots * kMaxParts < vectors) {
+        slots *= 2;
+    }
+    return shape_of(vectors, slots, 8);
+}
+
 inline int64_t backward_blocks(int64_t rows, const Shape& shape) {
     const int64_t blocks = (rows + teams_of(shape) - 1) / teams_of(shape);
-    return blocks < kBackwardMaxBlocks ? blocks : kBackwardMaxBlocks;
+    const int64_t most = kBackwardWaves * kWave / shape.threads;
+    return blocks < most ? blocks : most;
 }
 
 // Defined in rms_kernels.hip, one translation unit per stream type and pass.

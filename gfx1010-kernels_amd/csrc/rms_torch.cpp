@@ -9,6 +9,7 @@
 //   residual_rms_norm_backward(...)       (grad_x, grad_branch, grad_weight)
 //   residual_rms_norm_quantized(...)      (updated, quantized, scale)
 //   dequantize(quantized, scale, group, dtype)
+//   ..._if_supported(...)                 either of the two, or None
 //
 // The reference has no such operator. This file owns what the C ABI leaves to
 // the caller: tensor allocation, row strides, the device guard and the current
@@ -346,6 +347,13 @@ class ResidualRmsNormFunction : public torch::autograd::Function<ResidualRmsNorm
     }
 };
 
+// Whether a call on these inputs has a gradient to record.
+bool recorded(const at::Tensor& x, const at::Tensor& branch, const at::Tensor& weight) {
+    return at::GradMode::is_enabled()
+        && (x.requires_grad() || (branch.defined() && branch.requires_grad())
+            || weight.requires_grad());
+}
+
 // (updated, normalized); x itself is `updated` without a branch.
 std::tuple<at::Tensor, at::Tensor> residual_rms_norm(
     const at::Tensor& x,
@@ -355,10 +363,7 @@ std::tuple<at::Tensor, at::Tensor> residual_rms_norm(
     std::optional<at::ScalarType> normalized_dtype,
     bool checkpoint) {
     const at::Tensor branch = branch_in.value_or(at::Tensor());
-    const bool recorded = at::GradMode::is_enabled()
-        && (x.requires_grad() || (branch.defined() && branch.requires_grad())
-            || weight.requires_grad());
-    if (!recorded) {
+    if (!recorded(x, branch, weight)) {
         // Nothing to record: no state is kept, and no checkpoint written.
         auto [updated, normalized] =
             forward_impl(x, branch, weight, eps, normalized_dtype, false, nullptr, nullptr);
@@ -494,6 +499,23 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> residual_rms_norm_quantized(
     return {updated, quantized, scale};
 }
 
+// The same for inputs the native path serves and calls that lose no gradient,
+// else None: the auto path's common case in one call.
+std::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor>>
+residual_rms_norm_quantized_if_supported(
+    const at::Tensor& x,
+    const std::optional<at::Tensor>& branch_in,
+    const at::Tensor& weight,
+    double eps,
+    at::ScalarType dtype,
+    int64_t group) {
+    const at::Tensor branch = branch_in.value_or(at::Tensor());
+    if (!rms_inputs_supported(x, branch, weight, eps) || recorded(x, branch, weight)) {
+        return std::nullopt;
+    }
+    return residual_rms_norm_quantized(x, branch_in, weight, eps, dtype, group);
+}
+
 at::Tensor dequantize(const at::Tensor& quantized, const at::Tensor& scale, int64_t group,
                       at::ScalarType dtype) {
     TORCH_CHECK(quantized.is_cuda(), "quantized must be a HIP tensor");
@@ -520,6 +542,20 @@ at::Tensor dequantize(const at::Tensor& quantized, const at::Tensor& scale, int6
     return values;
 }
 
+// The same, or None where the checks above would raise.
+std::optional<at::Tensor> dequantize_if_supported(const at::Tensor& quantized,
+                                                  const at::Tensor& scale, int64_t group,
+                                                  at::ScalarType dtype) {
+    if (!quantized.is_cuda() || scale.device() != quantized.device() || quantized.dim() < 1
+        || !code_type(quantized.scalar_type()) || scale.scalar_type() != at::kFloat
+        || quantized.size(-1) < 1
+        || scale.sizes() != at::IntArrayRef(scale_sizes(quantized.sizes(), group))
+        || (at::GradMode::is_enabled() && scale.requires_grad())) {
+        return std::nullopt;
+    }
+    return dequantize(quantized, scale, group, dtype);
+}
+
 }  // namespace
 
 void bind_rms(pybind11::module_& module) {
@@ -533,5 +569,8 @@ void bind_rms(pybind11::module_& module) {
     module.def("residual_rms_norm_forward", &residual_rms_norm_forward);
     module.def("residual_rms_norm_backward", &residual_rms_norm_backward);
     module.def("residual_rms_norm_quantized", &residual_rms_norm_quantized);
+    module.def("residual_rms_norm_quantized_if_supported",
+               &residual_rms_norm_quantized_if_supported);
     module.def("dequantize", &dequantize);
+    module.def("dequantize_if_supported", &dequantize_if_supported);
 }

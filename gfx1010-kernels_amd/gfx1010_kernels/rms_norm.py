@@ -282,6 +282,13 @@ def residual_rms_norm_quantized(
     For serving: it records no gradient, and raises where one would be lost
     (grad mode on and an input that requires grad).
     """
+    if (implementation == "auto" and x.is_cuda and dtype in QUANTIZED_DTYPES
+            and group_size in GROUP_SIZES and x.get_device() in _READY_DEVICES
+            and not torch.compiler.is_compiling()):
+        result = _extension()[0].residual_rms_norm_quantized_if_supported(
+            x, branch, weight, float(eps), dtype, group_size or 0)
+        if result is not None:
+            return result
     _check_implementation(implementation)
     if dtype not in QUANTIZED_DTYPES:
         raise ValueError("dtype must be torch.int8 or torch.float8_e4m3fn")
@@ -318,6 +325,12 @@ def dequantize(quantized, scale, *, group_size=None, dtype=torch.bfloat16,
     """``quantized * scale`` in ``dtype`` (fp32, fp16 or bf16), for a consumer of
     :func:`residual_rms_norm_quantized`'s output that does not read 8 bits.
     ``group_size`` is the one the values were made with. Records no gradient."""
+    if (implementation == "auto" and quantized.is_cuda and dtype in STREAM_DTYPES
+            and group_size in GROUP_SIZES and quantized.get_device() in _READY_DEVICES
+            and not torch.compiler.is_compiling()):
+        result = _extension()[0].dequantize_if_supported(quantized, scale, group_size or 0, dtype)
+        if result is not None:
+            return result
     _check_implementation(implementation)
     _check_group_size(group_size)
     if dtype not in STREAM_DTYPES:
