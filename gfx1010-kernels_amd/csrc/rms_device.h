@@ -841,6 +841,12 @@ inline int teams_of(const Shape& shape) {
     return shape.threads / (kWave * shape.parts);
 }
 
+// Blocks that give every row a team (no overflow for any row count).
+inline int64_t blocks_of(int64_t rows, const Shape& shape) {
+    const int teams = teams_of(shape);
+    return rows / teams + (rows % teams != 0);
+}
+
 inline Shape forward_shape(int64_t hidden, int x_dtype) {
     const int64_t vectors = wave_vectors(hidden, x_dtype);
     const int most = x_dtype == RLN_DTYPE_F32 ? 4 : 2;
@@ -854,7 +860,7 @@ inline Shape forward_shape(int64_t hidden, int x_dtype) {
 constexpr int64_t kForwardMaxBlocks = 1 << 21;
 
 inline int64_t forward_blocks(int64_t rows, const Shape& shape) {
-    const int64_t blocks = (rows + teams_of(shape) - 1) / teams_of(shape);
+    const int64_t blocks = blocks_of(rows, shape);
     return blocks < kForwardMaxBlocks ? blocks : kForwardMaxBlocks;
 }
 
@@ -872,7 +878,7 @@ inline Shape backward_shape(int64_t rows, int64_t hidden, int x_dtype) {
 }
 
 inline int64_t backward_blocks(int64_t rows, const Shape& shape) {
-    const int64_t blocks = (rows + teams_of(shape) - 1) / teams_of(shape);
+    const int64_t blocks = blocks_of(rows, shape);
     const int64_t most = kBackwardWaves * kWave / shape.threads;
     return blocks < most ? blocks : most;
 }

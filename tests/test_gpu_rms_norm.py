@@ -7,9 +7,11 @@ lane, a short last vector, groups of 32 to 256 columns that end inside a vector.
 """
 
 import itertools
+import threading
 
 import pytest
 import torch
+import torch.utils.checkpoint
 from torch import nn
 
 import rms_reference as reference
@@ -454,6 +456,88 @@ def test_checkpoint_is_what_it_is_documented_to_be():
     assert kept[torch.int8] <= x.nbytes // 2 * (1 + 4 / 128) + 4096 * 4 + 4096
 
 
+def test_gradients_of_two_leaves_are_no_alias():
+    """One tensor is handed to x and to a branch of its type; what accumulates
+    in their .grad must not be shared."""
+    for checkpoint in (None, torch.int8):
+        x, branch, weight = (t.cuda().requires_grad_() for t in make((9, 128), BF16, BF16, BF16))
+        for turn in range(2):
+            updated, normalized = residual_rms_norm(x, branch, weight,
+                                                    checkpoint_dtype=checkpoint)
+            (updated.float().sum() + normalized.float().square().sum()).backward()
+            assert reference.same_bits(x.grad, branch.grad)
+            assert x.grad.data_ptr() != branch.grad.data_ptr()
+        before = branch.grad.clone()
+        x.grad.zero_()
+        assert reference.same_bits(branch.grad, before)
+    # The same tensor as both inputs: its gradient counts twice.
+    (twice,) = torch.autograd.grad(residual_rms_norm(x, x, weight)[0].float().sum(), x)
+    assert (twice == 2).all()
+
+
+@pytest.mark.parametrize("checkpoint", [None, torch.int8])
+@pytest.mark.parametrize("added", [True, False])
+def test_the_graph_is_kept_and_released_as_any(checkpoint, added):
+    x, branch, weight = (t.cuda().requires_grad_() for t in make((9, 200), F32, BF16, F32))
+    leaves = [x, branch, weight] if added else [x, weight]
+
+    def forward():
+        return residual_rms_norm(x, branch if added else None, weight,
+                                 checkpoint_dtype=checkpoint)[1].square().sum()
+
+    loss = forward()
+    first = torch.autograd.grad(loss, leaves, retain_graph=True)
+    again = torch.autograd.grad(loss, leaves)
+    assert all(reference.same_bits(a, b) for a, b in zip(first, again))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(loss, leaves)
+    # Saved tensors go through hooks, and a recomputed segment saves the same.
+    with torch.autograd.graph.save_on_cpu():
+        loss = forward()
+    assert all(reference.same_bits(a, b)
+               for a, b in zip(first, torch.autograd.grad(loss, leaves)))
+    loss = torch.utils.checkpoint.checkpoint(forward, use_reentrant=False)
+    assert all(reference.same_bits(a, b)
+               for a, b in zip(first, torch.autograd.grad(loss, leaves)))
+
+
+def test_two_threads_at_once():
+    """Forward, backward and 8-bit calls from two host threads, each on its
+    stream, equal the same calls alone."""
+    cases = [tuple(t.cuda() for t in make((257, hidden), BF16, BF16, BF16, hidden))
+             for hidden in (1000, 2048)]
+
+    def work(x, branch, weight):
+        leaves = [t.clone().requires_grad_() for t in (x, branch, weight)]
+        outputs = residual_rms_norm(*leaves, EPS, checkpoint_dtype=torch.int8)
+        grads = torch.autograd.grad(outputs, leaves, [x, branch])
+        with torch.no_grad():
+            codes = residual_rms_norm_quantized(x, branch, weight, EPS, group_size=64)
+            return [*outputs, *grads, *codes, dequantize(*codes[1:], group_size=64)]
+
+    expected = [work(*case) for case in cases]
+    torch.cuda.synchronize()
+    failures = []
+
+    def run(case, answer):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    found = work(*case)
+            stream.synchronize()
+            assert all(reference.same_bits(a, b) for a, b in zip(found, answer))
+        except BaseException as error:  # reported by the main thread
+            failures.append(error)
+
+    threads = [threading.Thread(target=run, args=pair) for pair in zip(cases, expected)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join(timeout=60)
+    assert not failures, failures
+
+
 def test_second_order_gradients_are_refused():
     x = torch.randn(4, 64, device="cuda", requires_grad=True)
     weight = torch.ones(64, device="cuda", requires_grad=True)
@@ -672,6 +756,39 @@ def test_rows_past_two_to_the_31_elements():
                         "last row")
         assert not grads[0][:-1].any()
         del grads
+
+
+def test_more_rows_than_one_grid():
+    """A launch has at most 2^21 blocks; teams walk over the rows past that, and
+    so do the widening's."""
+    rows, hidden = (1 << 23) + 5, 4
+    generator = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, hidden, device="cuda", generator=generator)
+    weight = torch.randn(hidden, device="cuda", generator=generator)
+    u = x + x
+    normalized = residual_rms_norm(x, x, weight, EPS, implementation="gfx950")[1]
+    value = reference.normalized(u, weight, EPS)
+    assert ((normalized.double() - value).abs() <= 33 * reference.U * value.abs()).all()
+    updated, codes, scale = residual_rms_norm_quantized(x, x, weight, EPS, dtype=torch.int8,
+                                                        implementation="gfx950")
+    assert torch.equal(updated, u)
+    values = dequantize(codes, scale, dtype=F32)
+    assert ((values - value).abs() <= 0.51 * scale).all()
+    del value, values, normalized
+    leaf, scale_leaf = x.clone().requires_grad_(), weight.clone().requires_grad_()
+    ones = torch.ones_like(x)
+    grads = torch.autograd.grad(residual_rms_norm(leaf, None, scale_leaf, EPS)[1],
+                                [leaf, scale_leaf], ones)
+    # 4096 teams of rows/4096 = 2049 rows each, then 4 teams and 512 blocks.
+    g, gw, size, terms = reference.gradients(x, x, weight, EPS, None, ones)
+    assert ((grads[0].double() - g).abs() <= 128 * reference.U * size + reference.U * g.abs()).all()
+    assert ((grads[1].double() - gw).abs() <= (32 + 2049 + 516) * reference.U * terms).all()
+    del grads, g, size, ones
+    rows = (1 << 29) + 1000
+    codes = torch.randint(-127, 128, (rows, 1), device="cuda", dtype=torch.int8)
+    scale = torch.rand(rows, 1, device="cuda")
+    values = dequantize(codes, scale, dtype=F32, implementation="gfx950")
+    assert torch.equal(values, codes.float().mul_(scale))
 
 
 # Together, as they are used.
