@@ -49,9 +49,20 @@ int check_stride(const char* name, int64_t stride, int64_t rows) {
     return RLN_OK;
 }
 
+int64_t size_of(int dtype) {
+    return dtype == RLN_DTYPE_F32 ? 4 : code_dtype(dtype) ? 1 : 2;
+}
+
+// Whether rows `stride` elements apart from `pointer` on start on whole vectors
+// of `columns` elements (16 bytes of a longer one): what Aligned instances ask.
+bool whole_vectors(const void* pointer, int dtype, int64_t stride, int columns) {
+    const int64_t bytes = columns * size_of(dtype) < 16 ? columns * size_of(dtype) : 16;
+    return static_cast<int64_t>(reinterpret_cast<uintptr_t>(pointer) % bytes) == 0
+        && stride * size_of(dtype) % bytes == 0;
+}
+
 int check_alignment(const char* name, const void* pointer, int dtype) {
-    const uintptr_t size = dtype == RLN_DTYPE_F32 ? 4 : 2;
-    if (reinterpret_cast<uintptr_t>(pointer) % size != 0) {
+    if (reinterpret_cast<uintptr_t>(pointer) % size_of(dtype) != 0) {
         return fail(RLN_ERR_INVALID, "%s is not aligned to its elements", name);
     }
     return RLN_OK;
@@ -114,6 +125,13 @@ int forward_args(const void* x, int x_dtype, int64_t x_stride, const void* branc
 int launch(ForwardArgs& a, int x_dtype, int branch_dtype, Mode mode, void* stream) {
     const Shape shape = forward_shape(a.hidden, x_dtype);
     a.parts = shape.parts;
+    const int columns = columns_of(x_dtype);
+    a.aligned = a.hidden % columns == 0 && whole_vectors(a.x, x_dtype, a.x_stride, columns)
+        && whole_vectors(a.branch, branch_dtype, a.branch_stride, columns)
+        && whole_vectors(a.weight, a.weight_dtype, 0, columns)
+        && whole_vectors(a.updated, x_dtype, 0, columns)
+        && whole_vectors(a.normalized, a.output_dtype, 0, columns)
+        && whole_vectors(a.checkpoint, RLN_DTYPE_INT8, 0, columns);
     const hipStream_t queue = static_cast<hipStream_t>(stream);
     switch (x_dtype) {
         case RLN_DTYPE_F32:
@@ -185,7 +203,7 @@ struct DequantizeArgs {
 
 constexpr int kDequantizeThreads = 256;
 
-template <bool Tail>
+template <bool Aligned>
 __global__ __launch_bounds__(kDequantizeThreads) void dequantize_kernel(DequantizeArgs a) {
     constexpr int N = 8;
     const int64_t step = static_cast<int64_t>(gridDim.x) * kDequantizeThreads;
@@ -196,10 +214,17 @@ __global__ __launch_bounds__(kDequantizeThreads) void dequantize_kernel(Dequanti
         const uint32_t rows_on = from / static_cast<uint32_t>(a.row_vectors);
         const int column = static_cast<int>(from - rows_on * a.row_vectors) * N;
         const int64_t row = begin_row + rows_on;
-        const int hidden = begin + threadIdx.x < a.vectors ? a.hidden : 0;
-        const int64_t first = row * a.hidden;
-        const Raw<int8_t, N> raw = load<Tail, int8_t, N>(a.codes + first, column, hidden);
-        const float scale = column < hidden ? a.scale[row * a.groups + column / a.group] : 0.0f;
+        const bool live = begin + threadIdx.x < a.vectors;
+        const float scale = live ? a.scale[row * a.groups + column / a.group] : 0.0f;
+        // Whole vectors lie one after another over the rows, so the block's are
+        // one run that starts at a uniform address; short ones go row by row.
+        const int64_t left = a.vectors - begin;
+        const int64_t first = Aligned ? begin * N : row * a.hidden;
+        const int place = Aligned ? static_cast<int>(threadIdx.x) * N : column;
+        const int extent = Aligned
+            ? static_cast<int>(left < kDequantizeThreads ? left : kDequantizeThreads) * N
+            : live ? a.hidden : 0;
+        const Raw<int8_t, N> raw = load<Aligned, int8_t, N>(a.codes + first, place, extent);
         float values[N];
         if (a.code_dtype == RLN_DTYPE_E4M3) {
             widen_e4m3<N>(raw, values);
@@ -210,7 +235,7 @@ __global__ __launch_bounds__(kDequantizeThreads) void dequantize_kernel(Dequanti
         for (int e = 0; e < N; ++e) {
             values[e] *= scale;
         }
-        store_as<Tail, N>(a.values, a.value_dtype, first, column, hidden, values);
+        store_as<Aligned, kBackwardStores, N>(a.values, a.value_dtype, first, place, extent, values);
     }
 }
 
@@ -372,6 +397,15 @@ int rln_rms_backward(
     a.weight_dtype = weight_dtype;
     a.branch_dtype = branch_dtype;
     a.inv_hidden = 1.0f / static_cast<float>(hidden);
+    const int columns = columns_of(x_dtype);
+    a.aligned = hidden % columns == 0 && whole_vectors(grad_updated, x_dtype, 0, columns)
+        && whole_vectors(grad_normalized, grad_normalized_dtype, 0, columns)
+        && whole_vectors(updated, x_dtype, updated_stride, columns)
+        && whole_vectors(checkpoint, RLN_DTYPE_INT8, 0, columns)
+        && whole_vectors(weight, weight_dtype, 0, columns)
+        && whole_vectors(grad_x, x_dtype, 0, columns)
+        && whole_vectors(grad_branch, branch_dtype, 0, columns)
+        && whole_vectors(a.partials, RLN_DTYPE_F32, 0, columns);
     const hipStream_t queue = static_cast<hipStream_t>(stream);
     switch (x_dtype) {
         case RLN_DTYPE_F32:
@@ -441,12 +475,13 @@ int rln_dequantize(
     int64_t blocks = (a.vectors + kDequantizeThreads - 1) / kDequantizeThreads;
     blocks = blocks < kForwardMaxBlocks ? blocks : kForwardMaxBlocks;
     const hipStream_t queue = static_cast<hipStream_t>(stream);
-    if (hidden % 8 == 0) {
-        dequantize_kernel<false><<<dim3(static_cast<unsigned>(blocks)), kDequantizeThreads, 0,
-                                   queue>>>(a);
-    } else {
+    if (hidden % 8 == 0 && whole_vectors(quantized, quantized_dtype, 0, 8)
+        && whole_vectors(values, values_dtype, 0, 8)) {
         dequantize_kernel<true><<<dim3(static_cast<unsigned>(blocks)), kDequantizeThreads, 0,
                                   queue>>>(a);
+    } else {
+        dequantize_kernel<false><<<dim3(static_cast<unsigned>(blocks)), kDequantizeThreads, 0,
+                                   queue>>>(a);
     }
     return check_launch("rms dequantize_kernel");
 }

@@ -17,12 +17,12 @@ int launch(Kernel kernel, const Args& a, int64_t blocks, int threads, size_t lds
 
 #if RMS_PASS == 1
 template <typename X, typename B, int V, Mode kMode>
-int forward_tail(const ForwardArgs& a, const Shape& shape, hipStream_t stream) {
+int forward_access(const ForwardArgs& a, const Shape& shape, hipStream_t stream) {
     const int64_t blocks = forward_blocks(a.rows, shape);
-    return a.hidden % kColumns<X> == 0
-        ? launch(forward_kernel<X, B, V, kMode, false>, a, blocks, shape.threads, 0, stream,
+    return a.aligned
+        ? launch(forward_kernel<X, B, V, kMode, true>, a, blocks, shape.threads, 0, stream,
                  "rms forward_kernel")
-        : launch(forward_kernel<X, B, V, kMode, true>, a, blocks, shape.threads, 0, stream,
+        : launch(forward_kernel<X, B, V, kMode, false>, a, blocks, shape.threads, 0, stream,
                  "rms forward_kernel");
 }
 
@@ -30,12 +30,12 @@ template <typename X, typename B, Mode kMode>
 int forward_slots(const ForwardArgs& a, const Shape& shape, hipStream_t stream) {
     switch (shape.slots) {
         case 1:
-            return forward_tail<X, B, 1, kMode>(a, shape, stream);
+            return forward_access<X, B, 1, kMode>(a, shape, stream);
         case 2:
-            return forward_tail<X, B, 2, kMode>(a, shape, stream);
+            return forward_access<X, B, 2, kMode>(a, shape, stream);
         default:
             if constexpr (kColumns<X> == 4) {
-                return forward_tail<X, B, 4, kMode>(a, shape, stream);
+                return forward_access<X, B, 4, kMode>(a, shape, stream);
             }
             return fail(RLN_ERR_UNSUPPORTED, "rms forward: %d slots", shape.slots);
     }
@@ -58,14 +58,14 @@ int forward_branch(const ForwardArgs& a, const Shape& shape, int branch_dtype,
 }
 #else
 template <typename X, typename Y, int V, bool Checkpoint>
-int backward_tail(const BackwardArgs& a, const Shape& shape, hipStream_t stream) {
+int backward_access(const BackwardArgs& a, const Shape& shape, hipStream_t stream) {
     const int64_t blocks = backward_blocks(a.rows, shape);
     const size_t lds = a.partials == nullptr
         ? 0 : static_cast<size_t>(teams_of(shape) - 1) * a.hidden * sizeof(float);
-    return a.hidden % kColumns<X> == 0
-        ? launch(backward_kernel<X, Y, V, Checkpoint, false>, a, blocks, shape.threads, lds,
+    return a.aligned
+        ? launch(backward_kernel<X, Y, V, Checkpoint, true>, a, blocks, shape.threads, lds,
                  stream, "rms backward_kernel")
-        : launch(backward_kernel<X, Y, V, Checkpoint, true>, a, blocks, shape.threads, lds,
+        : launch(backward_kernel<X, Y, V, Checkpoint, false>, a, blocks, shape.threads, lds,
                  stream, "rms backward_kernel");
 }
 
@@ -73,12 +73,12 @@ template <typename X, typename Y, bool Checkpoint>
 int backward_slots(const BackwardArgs& a, const Shape& shape, hipStream_t stream) {
     switch (shape.slots) {
         case 1:
-            return backward_tail<X, Y, 1, Checkpoint>(a, shape, stream);
+            return backward_access<X, Y, 1, Checkpoint>(a, shape, stream);
         case 2:
-            return backward_tail<X, Y, 2, Checkpoint>(a, shape, stream);
+            return backward_access<X, Y, 2, Checkpoint>(a, shape, stream);
         default:
             if constexpr (kColumns<X> == 4) {
-                return backward_tail<X, Y, 4, Checkpoint>(a, shape, stream);
+                return backward_access<X, Y, 4, Checkpoint>(a, shape, stream);
             }
             return fail(RLN_ERR_UNSUPPORTED, "rms backward: %d slots", shape.slots);
     }

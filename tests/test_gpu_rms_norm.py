@@ -538,6 +538,23 @@ def test_two_threads_at_once():
     assert not failures, failures
 
 
+def test_transforms_and_fake_tensors_are_refused():
+    """A functorch transform and a FakeTensorMode around real tensors ask for
+    what the kernels cannot give; the call raises and the next one is served."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    x, branch, weight = (t.cuda() for t in make((3, 64), F32, F32, F32))
+    expected = residual_rms_norm(x, branch, weight)
+    with pytest.raises(Exception):
+        torch.func.grad(lambda t: residual_rms_norm(t, branch, weight)[1].sum())(x)
+    with pytest.raises(Exception):
+        torch.func.vmap(lambda t: residual_rms_norm(t, None, weight)[1])(x)
+    with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(Exception):
+        residual_rms_norm(x, branch, weight)
+    for a, b in zip(residual_rms_norm(x, branch, weight), expected):
+        assert reference.same_bits(a, b)
+
+
 def test_second_order_gradients_are_refused():
     x = torch.randn(4, 64, device="cuda", requires_grad=True)
     weight = torch.ones(64, device="cuda", requires_grad=True)
