@@ -53,12 +53,11 @@ int64_t size_of(int dtype) {
     return dtype == RLN_DTYPE_F32 ? 4 : code_dtype(dtype) ? 1 : 2;
 }
 
-// Whether rows `stride` elements apart from `pointer` on start on whole vectors
-// of `columns` elements (16 bytes of a longer one): what Aligned instances ask.
-bool whole_vectors(const void* pointer, int dtype, int64_t stride, int columns) {
-    const int64_t bytes = columns * size_of(dtype) < 16 ? columns * size_of(dtype) : 16;
-    return static_cast<int64_t>(reinterpret_cast<uintptr_t>(pointer) % bytes) == 0
-        && stride * size_of(dtype) % bytes == 0;
+// Whether rows of `hidden` elements, `stride` elements apart from `pointer` on,
+// start and end on whole 32-bit words: what Access::kWords asks.
+bool whole_words(const void* pointer, int dtype, int64_t stride, int64_t hidden) {
+    return reinterpret_cast<uintptr_t>(pointer) % 4 == 0 && stride * size_of(dtype) % 4 == 0
+        && hidden * size_of(dtype) % 4 == 0;
 }
 
 int check_alignment(const char* name, const void* pointer, int dtype) {
@@ -125,13 +124,14 @@ int forward_args(const void* x, int x_dtype, int64_t x_stride, const void* branc
 int launch(ForwardArgs& a, int x_dtype, int branch_dtype, Mode mode, void* stream) {
     const Shape shape = forward_shape(a.hidden, x_dtype);
     a.parts = shape.parts;
-    const int columns = columns_of(x_dtype);
-    a.aligned = a.hidden % columns == 0 && whole_vectors(a.x, x_dtype, a.x_stride, columns)
-        && whole_vectors(a.branch, branch_dtype, a.branch_stride, columns)
-        && whole_vectors(a.weight, a.weight_dtype, 0, columns)
-        && whole_vectors(a.updated, x_dtype, 0, columns)
-        && whole_vectors(a.normalized, a.output_dtype, 0, columns)
-        && whole_vectors(a.checkpoint, RLN_DTYPE_INT8, 0, columns);
+    const int64_t hidden = a.hidden;
+    a.words = whole_words(a.x, x_dtype, a.x_stride, hidden)
+        && (a.branch == nullptr || whole_words(a.branch, branch_dtype, a.branch_stride, hidden))
+        && whole_words(a.weight, a.weight_dtype, 0, hidden)
+        && whole_words(a.updated, x_dtype, hidden, hidden)
+        && whole_words(a.normalized, a.output_dtype, hidden, hidden)
+        && (a.checkpoint == nullptr
+            || whole_words(a.checkpoint, RLN_DTYPE_INT8, hidden, hidden));
     const hipStream_t queue = static_cast<hipStream_t>(stream);
     switch (x_dtype) {
         case RLN_DTYPE_F32:
@@ -203,9 +203,10 @@ struct DequantizeArgs {
 
 constexpr int kDequantizeThreads = 256;
 
-template <bool Aligned>
+template <Access kAccess>
 __global__ __launch_bounds__(kDequantizeThreads) void dequantize_kernel(DequantizeArgs a) {
     constexpr int N = 8;
+    constexpr bool kRun = kAccess == Access::kWords;
     const int64_t step = static_cast<int64_t>(gridDim.x) * kDequantizeThreads;
     for (int64_t begin = static_cast<int64_t>(blockIdx.x) * kDequantizeThreads;
          begin < a.vectors; begin += step) {
@@ -219,12 +220,12 @@ __global__ __launch_bounds__(kDequantizeThreads) void dequantize_kernel(Dequanti
         // Whole vectors lie one after another over the rows, so the block's are
         // one run that starts at a uniform address; short ones go row by row.
         const int64_t left = a.vectors - begin;
-        const int64_t first = Aligned ? begin * N : row * a.hidden;
-        const int place = Aligned ? static_cast<int>(threadIdx.x) * N : column;
-        const int extent = Aligned
+        const int64_t first = kRun ? begin * N : row * a.hidden;
+        const int place = kRun ? static_cast<int>(threadIdx.x) * N : column;
+        const int extent = kRun
             ? static_cast<int>(left < kDequantizeThreads ? left : kDequantizeThreads) * N
             : live ? a.hidden : 0;
-        const Raw<int8_t, N> raw = load<Aligned, int8_t, N>(a.codes + first, place, extent);
+        const Raw<int8_t, N> raw = load<kAccess, int8_t, N>(a.codes + first, place, extent);
         float values[N];
         if (a.code_dtype == RLN_DTYPE_E4M3) {
             widen_e4m3<N>(raw, values);
@@ -235,7 +236,7 @@ __global__ __launch_bounds__(kDequantizeThreads) void dequantize_kernel(Dequanti
         for (int e = 0; e < N; ++e) {
             values[e] *= scale;
         }
-        store_as<Aligned, kBackwardStores, N>(a.values, a.value_dtype, first, place, extent, values);
+        store_as<kAccess, kBackwardStores, N>(a.values, a.value_dtype, first, place, extent, values);
     }
 }
 
@@ -320,7 +321,7 @@ size_t rln_rms_backward_workspace_bytes(int64_t rows, int64_t hidden, int x_dtyp
     if (rows <= 0 || !rln_rms_hidden_supported(hidden) || !float_dtype(x_dtype)) {
         return 0;
     }
-    return static_cast<size_t>(backward_blocks(rows, backward_shape(rows, hidden, x_dtype)))
+    return static_cast<size_t>(backward_blocks(rows, backward_shape(hidden, x_dtype)))
         * static_cast<size_t>(hidden) * sizeof(float);
 }
 
@@ -368,7 +369,7 @@ int rln_rms_backward(
         || (status = check_alignment("workspace", workspace, RLN_DTYPE_F32)) != RLN_OK) {
         return status;
     }
-    const Shape shape = backward_shape(rows, hidden, x_dtype);
+    const Shape shape = backward_shape(hidden, x_dtype);
     const size_t needed = grad_weight != nullptr
         ? rln_rms_backward_workspace_bytes(rows, hidden, x_dtype) : 0;
     if (needed > 0 && (workspace == nullptr || workspace_bytes < needed)) {
@@ -397,15 +398,13 @@ int rln_rms_backward(
     a.weight_dtype = weight_dtype;
     a.branch_dtype = branch_dtype;
     a.inv_hidden = 1.0f / static_cast<float>(hidden);
-    const int columns = columns_of(x_dtype);
-    a.aligned = hidden % columns == 0 && whole_vectors(grad_updated, x_dtype, 0, columns)
-        && whole_vectors(grad_normalized, grad_normalized_dtype, 0, columns)
-        && whole_vectors(updated, x_dtype, updated_stride, columns)
-        && whole_vectors(checkpoint, RLN_DTYPE_INT8, 0, columns)
-        && whole_vectors(weight, weight_dtype, 0, columns)
-        && whole_vectors(grad_x, x_dtype, 0, columns)
-        && whole_vectors(grad_branch, branch_dtype, 0, columns)
-        && whole_vectors(a.partials, RLN_DTYPE_F32, 0, columns);
+    a.words = whole_words(grad_updated, x_dtype, hidden, hidden)
+        && whole_words(grad_normalized, grad_normalized_dtype, hidden, hidden)
+        && (updated == nullptr || whole_words(updated, x_dtype, updated_stride, hidden))
+        && (checkpoint == nullptr || whole_words(checkpoint, RLN_DTYPE_INT8, hidden, hidden))
+        && whole_words(weight, weight_dtype, 0, hidden)
+        && whole_words(grad_x, x_dtype, hidden, hidden)
+        && (grad_branch == nullptr || whole_words(grad_branch, branch_dtype, hidden, hidden));
     const hipStream_t queue = static_cast<hipStream_t>(stream);
     switch (x_dtype) {
         case RLN_DTYPE_F32:
@@ -475,12 +474,12 @@ int rln_dequantize(
     int64_t blocks = (a.vectors + kDequantizeThreads - 1) / kDequantizeThreads;
     blocks = blocks < kForwardMaxBlocks ? blocks : kForwardMaxBlocks;
     const hipStream_t queue = static_cast<hipStream_t>(stream);
-    if (hidden % 8 == 0 && whole_vectors(quantized, quantized_dtype, 0, 8)
-        && whole_vectors(values, values_dtype, 0, 8)) {
-        dequantize_kernel<true><<<dim3(static_cast<unsigned>(blocks)), kDequantizeThreads, 0,
+    if (hidden % 8 == 0 && whole_words(quantized, quantized_dtype, 0, 8)
+        && whole_words(values, values_dtype, 0, 8)) {
+        dequantize_kernel<Access::kWords><<<dim3(static_cast<unsigned>(blocks)), kDequantizeThreads, 0,
                                   queue>>>(a);
     } else {
-        dequantize_kernel<false><<<dim3(static_cast<unsigned>(blocks)), kDequantizeThreads, 0,
+        dequantize_kernel<Access::kLanes><<<dim3(static_cast<unsigned>(blocks)), kDequantizeThreads, 0,
                                    queue>>>(a);
     }
     return check_launch("rms dequantize_kernel");

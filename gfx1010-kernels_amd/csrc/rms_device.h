@@ -22,12 +22,14 @@
 // slot v of lane l of part p with j = (v * parts + p) * 64 + l. `parts` is a
 // run-time value, so any row length gets a team without idle waves.
 //
-// Two ways of access. Aligned instances (rows of whole, aligned vectors) go
-// through one buffer descriptor per row and tensor: lanes past the end of the row
-// are dropped by the hardware's range check, without a branch, and stores carry a
-// cache policy. Every other row length, stride and element alignment takes global
-// accesses, which the hardware serves in 128 bits at element alignment; only the
-// one vector that crosses the end of a row falls back to element accesses.
+// A row is read and written in vectors, through one buffer descriptor per row and
+// tensor where its rows start and end on whole 32-bit words (Access::kWords; 32-bit
+// elements always do): words past the end of the row are dropped by the
+// hardware's range check, without a branch, and stores carry a cache policy.
+// 16- and 8-bit rows of other lengths, strides and alignments (Access::kElements)
+// take global accesses, which the hardware serves in 128 bits at element
+// alignment; the one vector that crosses the end of a row is read shifted and
+// stored by elements.
 #ifndef RMS_DEVICE_H
 #define RMS_DEVICE_H
 
@@ -65,6 +67,14 @@ constexpr float kLeastMaximum = 0x1p-100f;
 template <typename X>
 constexpr int kColumns = 16 / static_cast<int>(sizeof(X));
 
+// How rows are accessed (see above); kLanes: as kElements, and each lane has a
+// row of its own, where the others ask for one row per wave.
+enum class Access { kWords, kElements, kLanes };
+
+template <Access kAccess, typename T>
+constexpr bool kBuffer =
+    kAccess == Access::kWords || (kAccess == Access::kElements && sizeof(T) == 4);
+
 enum class Mode { kNormalize, kCheckpoint, kQuantize };
 
 struct ForwardArgs {
@@ -81,7 +91,7 @@ struct ForwardArgs {
     int64_t rows;
     int hidden;
     int parts;
-    int aligned;        // every row is whole vectors, aligned to them
+    int words;          // Access::kWords serves every tensor
     int weight_dtype;
     int output_dtype;   // normalized's, or the codes'
     int group;          // columns under one scale, a multiple of the vector
@@ -105,7 +115,7 @@ struct BackwardArgs {
     int64_t rows;
     int hidden;
     int parts;
-    int aligned;
+    int words;
     int groups;
     int weight_dtype;
     int branch_dtype;
@@ -154,8 +164,9 @@ constexpr int kOnce = 2;
 constexpr int kForwardStores = 2;
 constexpr int kBackwardStores = 17;
 
-// A descriptor over `count` elements at a wave-uniform address (count 0: nothing
-// is read or written through it, wherever it points).
+// A descriptor over `count` elements at a wave-uniform address, whole words
+// (count 0: nothing is read or written through it, wherever it points). Accesses
+// of several words are range-checked word by word.
 template <typename T>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const T* row, int count) {
     const uint64_t bits = reinterpret_cast<uint64_t>(row);
@@ -168,12 +179,12 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const T* row, int c
 
 // Elements [column, column + N) of a row of `hidden` (both wave-uniform but for
 // the column), zeros past its end.
-template <bool Aligned, typename T, int N, int Policy = kOnce>
+template <Access kAccess, typename T, int N, int Policy = kOnce>
 __device__ __forceinline__ Raw<T, N> load(const T* __restrict__ row, int column, int hidden) {
     Raw<T, N> raw;
     constexpr int kWords = Raw<T, N>::kWords;
     constexpr int kChunk = kWords < 4 ? kWords : 4;
-    if constexpr (Aligned) {
+    if constexpr (kBuffer<kAccess, T>) {
         const auto buffer = row_buffer(row, hidden);
 #pragma unroll
         for (int i = 0; i < kWords; i += kChunk) {
@@ -194,16 +205,19 @@ __device__ __forceinline__ Raw<T, N> load(const T* __restrict__ row, int column,
         }
         return raw;
     }
+    // Vectors of up to 16 bytes; one that crosses the row's end is read from the
+    // row's last whole vector and shifted down, so that no lane branches around
+    // memory (by elements, each load waited for the one before: [8192, 4095] bf16
+    // backward 121 us, 85 so).
+    constexpr int kElements = 4 * kChunk / static_cast<int>(sizeof(T));
+    using W = Words_<kChunk, static_cast<int>(sizeof(T))>;
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-        raw.words[i] = 0;
-    }
-    if (column + N <= hidden) {
-        using W = Words_<kChunk, static_cast<int>(sizeof(T))>;
-#pragma unroll
-        for (int i = 0; i < kWords; i += kChunk) {
-            const typename W::type* from =
-                reinterpret_cast<const typename W::type*>(row + column) + i / kChunk;
+    for (int i = 0; i < kWords; i += kChunk) {
+        const int begin = column + i / kChunk * kElements;
+        unsigned __int128 bits = 0;
+        if (hidden >= kElements) {
+            const int start = begin < hidden - kElements ? begin : hidden - kElements;
+            const typename W::type* from = reinterpret_cast<const typename W::type*>(row + start);
             typename W::plain words;
             if constexpr (Policy == kOnce) {
                 words = __builtin_nontemporal_load(from);
@@ -211,29 +225,37 @@ __device__ __forceinline__ Raw<T, N> load(const T* __restrict__ row, int column,
                 words = *from;
             }
             if constexpr (kChunk == 1) {
-                raw.words[i] = words;
+                bits = words;
             } else {
 #pragma unroll
-                for (int k = 0; k < kChunk; ++k) {
-                    raw.words[i + k] = words[k];
+                for (int k = kChunk - 1; k >= 0; --k) {
+                    bits = bits << 32 | words[k];
+                }
+            }
+            if (begin != start) {
+                const int shift = (begin - start) * 8 * static_cast<int>(sizeof(T));
+                bits = begin < hidden ? bits >> shift : 0;
+            }
+        } else {  // rows shorter than a vector, and no row at all
+#pragma unroll
+            for (int e = 0; e < kElements - 1; ++e) {
+                if (begin + e < hidden) {
+                    uint32_t element;
+                    if constexpr (sizeof(T) == 4) {
+                        element = reinterpret_cast<const uint32_t*>(row)[begin + e];
+                    } else if constexpr (sizeof(T) == 2) {
+                        element = reinterpret_cast<const uint16_t*>(row)[begin + e];
+                    } else {
+                        element = reinterpret_cast<const uint8_t*>(row)[begin + e];
+                    }
+                    bits |= static_cast<unsigned __int128>(element)
+                        << (e * 8 * static_cast<int>(sizeof(T)));
                 }
             }
         }
-    } else {
-        constexpr int kPerWord = 4 / static_cast<int>(sizeof(T));
 #pragma unroll
-        for (int e = 0; e < N - 1; ++e) {
-            if (column + e < hidden) {
-                uint32_t bits;
-                if constexpr (sizeof(T) == 4) {
-                    bits = reinterpret_cast<const uint32_t*>(row)[column + e];
-                } else if constexpr (sizeof(T) == 2) {
-                    bits = reinterpret_cast<const uint16_t*>(row)[column + e];
-                } else {
-                    bits = reinterpret_cast<const uint8_t*>(row)[column + e];
-                }
-                raw.words[e / kPerWord] |= bits << (e % kPerWord * 8 * static_cast<int>(sizeof(T)));
-            }
+        for (int k = 0; k < kChunk; ++k) {
+            raw.words[i + k] = static_cast<uint32_t>(bits >> (32 * k));
         }
     }
     return raw;
@@ -280,12 +302,12 @@ __device__ __forceinline__ Raw<T, N> narrow(const float (&values)[N]) {
     return raw;
 }
 
-template <bool Aligned, int Policy, typename T, int N>
+template <Access kAccess, int Policy, typename T, int N>
 __device__ __forceinline__ void store(T* __restrict__ row, int column, int hidden,
                                       const Raw<T, N>& raw) {
     constexpr int kWords = Raw<T, N>::kWords;
     constexpr int kChunk = kWords < 4 ? kWords : 4;
-    if constexpr (Aligned) {
+    if constexpr (kBuffer<kAccess, T>) {
         const auto buffer = row_buffer(row, hidden);
 #pragma unroll
         for (int i = 0; i < kWords; i += kChunk) {
@@ -338,32 +360,32 @@ __device__ __forceinline__ void store(T* __restrict__ row, int column, int hidde
 
 // The weight and the outputs choose their type at run time: a wave-uniform
 // branch, where a template parameter would multiply the instances by three.
-template <bool Aligned, int N>
+template <Access kAccess, int N>
 __device__ __forceinline__ void load_weight(const void* weight, int dtype, int column, int hidden,
                                             float (&out)[N]) {
     if (dtype == RLN_DTYPE_F32) {
         widen<float, N>(
-            load<Aligned, float, N, kCached>(static_cast<const float*>(weight), column, hidden), out);
+            load<kAccess, float, N, kCached>(static_cast<const float*>(weight), column, hidden), out);
     } else if (dtype == RLN_DTYPE_F16) {
         widen<half_t, N>(
-            load<Aligned, half_t, N, kCached>(static_cast<const half_t*>(weight), column, hidden), out);
+            load<kAccess, half_t, N, kCached>(static_cast<const half_t*>(weight), column, hidden), out);
     } else {
         widen<bf16_t, N>(
-            load<Aligned, bf16_t, N, kCached>(static_cast<const bf16_t*>(weight), column, hidden), out);
+            load<kAccess, bf16_t, N, kCached>(static_cast<const bf16_t*>(weight), column, hidden), out);
     }
 }
 
-template <bool Aligned, int Policy, int N>
+template <Access kAccess, int Policy, int N>
 __device__ __forceinline__ void store_as(void* tensor, int dtype, int64_t first, int column,
                                          int hidden, const float (&values)[N]) {
     if (dtype == RLN_DTYPE_F32) {
-        store<Aligned, Policy, float, N>(static_cast<float*>(tensor) + first, column, hidden,
+        store<kAccess, Policy, float, N>(static_cast<float*>(tensor) + first, column, hidden,
                               narrow<float, N>(values));
     } else if (dtype == RLN_DTYPE_F16) {
-        store<Aligned, Policy, half_t, N>(static_cast<half_t*>(tensor) + first, column, hidden,
+        store<kAccess, Policy, half_t, N>(static_cast<half_t*>(tensor) + first, column, hidden,
                                narrow<half_t, N>(values));
     } else {
-        store<Aligned, Policy, bf16_t, N>(static_cast<bf16_t*>(tensor) + first, column, hidden,
+        store<kAccess, Policy, bf16_t, N>(static_cast<bf16_t*>(tensor) + first, column, hidden,
                                narrow<bf16_t, N>(values));
     }
 }
@@ -514,7 +536,7 @@ __device__ __forceinline__ Team team_of(int parts) {
 // kForwardMaxBlocks (a launch holds fewer than 2^32 threads); past that the
 // teams walk.
 
-template <typename X, typename B, int V, Mode kMode, bool Aligned>
+template <typename X, typename B, int V, Mode kMode, Access kAccess>
 __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs a) {
     constexpr int N = kColumns<X>;
     constexpr bool kBranch = !__is_same(B, NoBranch);
@@ -539,18 +561,18 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             column[v] = ((v * a.parts + team.part) * kWave + lane) * N;
-            raw_x[v] = load<Aligned, X, N>(x, column[v], hidden);
+            raw_x[v] = load<kAccess, X, N>(x, column[v], hidden);
         }
         if constexpr (kBranch) {
             const B* branch = static_cast<const B*>(a.branch) + row * a.branch_stride;
             Raw<B, N> raw_branch[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                raw_branch[v] = load<Aligned, B, N>(branch, column[v], hidden);
+                raw_branch[v] = load<kAccess, B, N>(branch, column[v], hidden);
             }
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                load_weight<Aligned, N>(a.weight, a.weight_dtype, column[v], hidden, weight[v]);
+                load_weight<kAccess, N>(a.weight, a.weight_dtype, column[v], hidden, weight[v]);
             }
             X* updated = static_cast<X*>(a.updated) + first;
 #pragma unroll
@@ -565,13 +587,13 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
                 // The norm is taken of the rounded stream, which is what the
                 // backward and the next layer read.
                 const Raw<X, N> rounded = narrow<X, N>(u[v]);
-                store<Aligned, kForwardStores, X, N>(updated, column[v], hidden, rounded);
+                store<kAccess, kForwardStores, X, N>(updated, column[v], hidden, rounded);
                 widen<X, N>(rounded, u[v]);
             }
         } else {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                load_weight<Aligned, N>(a.weight, a.weight_dtype, column[v], hidden, weight[v]);
+                load_weight<kAccess, N>(a.weight, a.weight_dtype, column[v], hidden, weight[v]);
                 widen<X, N>(raw_x[v], u[v]);
             }
         }
@@ -668,7 +690,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
                 for (int e = 0; e < N; ++e) {
                     steps[e] = u[v][e] * scale.inverse;
                 }
-                store<Aligned, kForwardStores, int8_t, N>(static_cast<int8_t*>(a.normalized) + first, column[v],
+                store<kAccess, kForwardStores, int8_t, N>(static_cast<int8_t*>(a.normalized) + first, column[v],
                                        hidden,
                                        e4m3 ? narrow_e4m3<N>(steps) : narrow_int8<N>(steps));
             }
@@ -685,7 +707,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
                     for (int e = 0; e < N; ++e) {
                         steps[e] = u[v][e] * scale.inverse;
                     }
-                    store<Aligned, kForwardStores, int8_t, N>(a.checkpoint + first, column[v], hidden,
+                    store<kAccess, kForwardStores, int8_t, N>(a.checkpoint + first, column[v], hidden,
                                            narrow_int8<N>(steps));
                 }
                 float normalized[N];
@@ -693,7 +715,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
                 for (int e = 0; e < N; ++e) {
                     normalized[e] = u[v][e] * rstd * weight[v][e];
                 }
-                store_as<Aligned, kForwardStores, N>(a.normalized, a.output_dtype, first, column[v], hidden,
+                store_as<kAccess, kForwardStores, N>(a.normalized, a.output_dtype, first, column[v], hidden,
                                   normalized);
             }
         }
@@ -706,7 +728,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
 // teams' shares through LDS and writes them to its row of the partials, which
 // reduce_kernel adds in a fixed order (no atomics: the same bits on every run).
 
-template <typename X, typename Y, int V, bool Checkpoint, bool Aligned>
+template <typename X, typename Y, int V, bool Checkpoint, Access kAccess>
 __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArgs a) {
     constexpr int N = kColumns<X>;
     extern __shared__ float shares[];  // [teams - 1][hidden], the weight's gradient
@@ -719,7 +741,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         column[v] = ((v * a.parts + team.part) * kWave + lane) * N;
-        load_weight<Aligned, N>(a.weight, a.weight_dtype, column[v], a.hidden, weight[v]);
+        load_weight<kAccess, N>(a.weight, a.weight_dtype, column[v], a.hidden, weight[v]);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             grad_weight[v][e] = 0.0f;
@@ -741,21 +763,21 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
         Raw<X, N> raw_grad[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            raw_y[v] = load<Aligned, Y, N>(static_cast<const Y*>(a.grad_normalized) + first,
+            raw_y[v] = load<kAccess, Y, N>(static_cast<const Y*>(a.grad_normalized) + first,
                                         column[v], hidden);
             if constexpr (Checkpoint) {
-                raw_kept[v] = load<Aligned, int8_t, N>(a.checkpoint + first, column[v], hidden);
+                raw_kept[v] = load<kAccess, int8_t, N>(a.checkpoint + first, column[v], hidden);
                 kept_step[v] = column[v] < hidden
                     ? a.scale[row * a.groups + column[v] / kCheckpointGroup] : 0.0f;
             } else {
-                raw_u[v] = load<Aligned, X, N>(
+                raw_u[v] = load<kAccess, X, N>(
                     static_cast<const X*>(a.updated) + row * a.updated_stride, column[v], hidden);
             }
         }
         if (a.grad_updated != nullptr) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                raw_grad[v] = load<Aligned, X, N>(static_cast<const X*>(a.grad_updated) + first,
+                raw_grad[v] = load<kAccess, X, N>(static_cast<const X*>(a.grad_updated) + first,
                                                column[v], hidden);
             }
         } else {
@@ -814,10 +836,10 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
             for (int e = 0; e < N; ++e) {
                 gradient[e] += rstd * (product[v][e] - unit[v][e] * shared);
             }
-            store<Aligned, kBackwardStores, X, N>(static_cast<X*>(a.grad_x) + first, column[v], hidden,
+            store<kAccess, kBackwardStores, X, N>(static_cast<X*>(a.grad_x) + first, column[v], hidden,
                               narrow<X, N>(gradient));
             if (a.grad_branch != nullptr) {
-                store_as<Aligned, kBackwardStores, N>(a.grad_branch, a.branch_dtype, first, column[v], hidden,
+                store_as<kAccess, kBackwardStores, N>(a.grad_branch, a.branch_dtype, first, column[v], hidden,
                                   gradient);
             }
         }
@@ -852,7 +874,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
                     }
                 }
             }
-            store<Aligned, kBackwardStores, float, N>(partial, column[v], a.hidden, narrow<float, N>(grad_weight[v]));
+            store<kAccess, kBackwardStores, float, N>(partial, column[v], a.hidden, narrow<float, N>(grad_weight[v]));
         }
     }
 }
@@ -861,20 +883,22 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 // Launch shapes (host). Measured on MI355X, graphs of launches over buffers that
 // pass the caches, TB/s of algorithmic bytes (a large copy reaches 5.4):
 //
-//  * 16 bytes of the stream per lane and slot. A 16-bit stream takes one slot
-//    while a row fits 8 waves of them ([16384, 4096] bf16: forward 6.0 against
-//    5.7 with two slots, backward 5.9 against 5.6), a 32-bit one two, whose
-//    half as many waves then read as much of a 16-bit branch ([32768, 2048]
-//    int8 in groups: 5.9 against 5.6).
-//  * The forward doubles the slots until a row fits 8 waves: blocks of 16 waves
-//    leave a CU idle while they wait for each other ([8192, 8192] fp32 with the
-//    checkpoint: 5.6 with four slots and 8 waves, 5.2 with two and 16). Rows over
-//    8192 columns take 16 waves.
-//  * The backward's grid is what the chip holds at 16 waves per CU, in blocks of 8
-//    waves: fewer leave the memory idle ([16384, 4096] bf16: 101 us at 8 per CU,
-//    91 at 16), more only add partial sums of the weight's gradient (108). Short
-//    launches, less than two rows per team, keep one slot, so that more
-//    teams share the rows ([1024, 384]: 7.4 against 8.9 us).
+//  * 16 bytes of the stream per lane and slot. The forward takes one slot of a
+//    16-bit stream ([16384, 4096] bf16: 6.2 against 5.9 with two) and two of a
+//    32-bit one, whose half as many waves then store whole words of codes
+//    ([32768, 1024] e4m3 in fp32: 6.2 against 5.4 with one; without codes 6.2
+//    against 5.9), and doubles them until a row fits 8 waves: in blocks of 16
+//    waves a CU idles while they wait for each other ([8192, 8192] fp32 with the
+//    checkpoint: 5.6 with four slots and 8 waves, 5.2 with two and 16).
+//  * The backward holds the weight and its gradient's sums in registers besides
+//    and takes one slot up to 8 waves a row ([32768, 1024] fp32: 5.7 against 5.4
+//    with two). Longer 32-bit rows take two up to 16 waves ([8192, 8192]: 5.5
+//    against 5.2 with four and 8 waves).
+//  * Its grid is two blocks of about 8 waves for each CU, or one of more: the same
+//    number everywhere, since blocks walk the rows at one pace ([6553, 5120] bf16:
+//    52 us with two blocks of 5 waves per CU, 61 with three), and no more, since
+//    each adds a row of partial sums ([16384, 4096] bf16: 90 us at 16 waves per CU,
+//    104 at 8, 104 at 32).
 
 struct Shape {
     int slots;  // V
@@ -892,14 +916,14 @@ inline int64_t wave_vectors(int64_t hidden, int x_dtype) {
     return (hidden + columns - 1) / columns;
 }
 
-// Teams of the fewest waves that hold a row at `slots` vectors per lane, at
-// least `least_waves` in a block.
-inline Shape shape_of(int64_t vectors, int slots, int least_waves) {
+// Waves per row at `slots` vectors per lane, and teams that make blocks of about
+// `waves` waves (nearest; at least one team).
+inline Shape shape_of(int64_t vectors, int slots, int waves) {
     Shape shape;
     shape.slots = slots;
     shape.parts = static_cast<int>((vectors + slots - 1) / slots);
-    const int teams = shape.parts >= least_waves ? 1 : least_waves / shape.parts;
-    shape.threads = teams * shape.parts * kWave;
+    const int teams = (waves + shape.parts / 2) / shape.parts;
+    shape.threads = (teams > 1 ? teams : 1) * shape.parts * kWave;
     return shape;
 }
 
@@ -930,22 +954,17 @@ inline int64_t forward_blocks(int64_t rows, const Shape& shape) {
     return blocks < kForwardMaxBlocks ? blocks : kForwardMaxBlocks;
 }
 
-// 256 CUs of 16 waves.
-constexpr int64_t kBackwardWaves = 4096;
-
-inline Shape backward_shape(int64_t rows, int64_t hidden, int x_dtype) {
+inline Shape backward_shape(int64_t hidden, int x_dtype) {
     const int64_t vectors = wave_vectors(hidden, x_dtype);
-    int slots = x_dtype == RLN_DTYPE_F32 && vectors > 1 && rows >= 2 * kBackwardWaves / vectors
-        ? 2 : 1;
-    while (slots * kMaxParts < vectors) {
-        slots *= 2;
-    }
+    const int slots = vectors <= 8 ? 1 : vectors <= 2 * kMaxParts ? 2 : 4;
     return shape_of(vectors, slots, 8);
 }
 
+constexpr int64_t kComputeUnits = 256;
+
 inline int64_t backward_blocks(int64_t rows, const Shape& shape) {
     const int64_t blocks = blocks_of(rows, shape);
-    const int64_t most = kBackwardWaves * kWave / shape.threads;
+    const int64_t most = shape.threads <= 10 * kWave ? 2 * kComputeUnits : kComputeUnits;
     return blocks < most ? blocks : most;
 }
 

@@ -28,9 +28,9 @@ pytestmark = pytest.mark.gpu
 EPS = 1e-6
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 CODE = {F32: 0, F16: 1, BF16: 2, torch.int8: 3, torch.float8_e4m3fn: 4}
-LENGTHS = [1, 2, 3, 4, 5, 7, 8, 9, 31, 64, 100, 127, 128, 129, 200, 255, 256, 257, 384, 511, 512,
-           513, 768, 1000, 1001, 1023, 1024, 1025, 1600, 2047, 2048, 2049, 2880, 4095, 4096, 4097,
-           5120, 6000, 8191, 8192, 8193, 11008, 12289, 16383, 16384]
+LENGTHS = [1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 31, 64, 100, 127, 128, 129, 200, 254, 255, 256, 257,
+           384, 510, 511, 512, 513, 514, 516, 768, 1000, 1001, 1023, 1024, 1025, 1030, 1280, 1600, 2046, 2047, 2048, 2049, 2880, 4094, 4095, 4096, 4097, 4100,
+           5120, 6000, 8191, 8192, 8193, 8194, 11008, 12289, 16383, 16384]
 TYPES = list(itertools.product([F32, F16, BF16], repeat=2))
 
 
@@ -109,9 +109,10 @@ def variants(tensor):
     wide = torch.zeros(rows, 2 * hidden + 3, dtype=tensor.dtype, device="cuda")
     wide[:, 3:3 + hidden] = tensor
     yield "one part of wider rows", wide[:, 3:3 + hidden]
-    flat = torch.zeros(rows * hidden + 1, dtype=tensor.dtype, device="cuda")
-    flat[1:] = tensor.flatten()
-    yield "one element off alignment", flat[1:].view(rows, hidden)
+    for off in (1, 2):
+        flat = torch.zeros(rows * hidden + off, dtype=tensor.dtype, device="cuda")
+        flat[off:] = tensor.flatten()
+        yield f"{off} elements off alignment", flat[off:].view(rows, hidden)
     yield "transposed", tensor.t().contiguous().t()
     spaced = torch.zeros(rows, hidden, 2, dtype=tensor.dtype, device="cuda")
     spaced[..., 1] = tensor
@@ -120,7 +121,7 @@ def variants(tensor):
         (rows, hidden), (hidden, 1)).flip(0)
 
 
-@pytest.mark.parametrize("hidden", [96, 515, 1600])
+@pytest.mark.parametrize("hidden", [96, 514, 515, 1600])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_strides_offsets_and_orders(hidden, dtype):
     x, branch, weight = make((6, hidden), dtype, dtype, dtype, 2)
@@ -589,7 +590,7 @@ def guarded(count, dtype):
     return inner, check
 
 
-@pytest.mark.parametrize("hidden", [1, 63, 130, 520, 2055, 4096, 16383])
+@pytest.mark.parametrize("hidden", [1, 2, 4, 6, 63, 130, 514, 516, 520, 2055, 4096, 16382, 16383])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_nothing_is_written_outside_the_outputs(hidden, dtype):
     rows, stream = 5, torch.cuda.current_stream().cuda_stream
