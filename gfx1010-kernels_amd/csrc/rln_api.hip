@@ -107,8 +107,6 @@ void rln_zero_parameters_kernel(float* __restrict__ grad_weight, float* __restri
     }
 }
 
-}  // namespace
-
 // Compute units of the current device, looked up once per device (0 when
 // the runtime cannot say; the forward then keeps its device-independent grid).
 int compute_units() {
@@ -131,8 +129,6 @@ int compute_units() {
     });
     return units[device];
 }
-
-namespace {
 
 bool aligned_to(const void* pointer, uintptr_t alignment) {
     return pointer == nullptr || (reinterpret_cast<uintptr_t>(pointer) & (alignment - 1)) == 0;

@@ -122,7 +122,7 @@ int forward_args(const void* x, int x_dtype, int64_t x_stride, const void* branc
 }
 
 int launch(ForwardArgs& a, int x_dtype, int branch_dtype, Mode mode, void* stream) {
-    const Shape shape = forward_shape(a.hidden, x_dtype);
+    const Shape shape = forward_shape(a.rows, a.hidden, x_dtype);
     a.parts = shape.parts;
     const int64_t hidden = a.hidden;
     a.words = whole_words(a.x, x_dtype, a.x_stride, hidden)

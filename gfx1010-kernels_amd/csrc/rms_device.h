@@ -45,7 +45,6 @@ int fail(int code, const char* format, ...);
 int check_launch(const char* what);
 int check_stream(void* stream);
 void clear_error();
-int compute_units();
 
 namespace rms {
 
@@ -126,10 +125,10 @@ struct BackwardArgs {
 // Vectors of N elements as raw words, at element alignment.
 
 template <int Words, int Alignment>
-struct Words_;
+struct WordVector;
 #define RMS_WORDS(count, alignment)                                                     \
     template <>                                                                         \
-    struct Words_<count, alignment> {                                                   \
+    struct WordVector<count, alignment> {                                                   \
         typedef uint32_t plain __attribute__((ext_vector_type(count)));                 \
         typedef plain type __attribute__((aligned(alignment)));                         \
     }
@@ -140,7 +139,7 @@ RMS_WORDS(2, 2);
 RMS_WORDS(2, 1);
 #undef RMS_WORDS
 template <>
-struct Words_<1, 1> {
+struct WordVector<1, 1> {
     typedef uint32_t plain;
     typedef uint32_t type __attribute__((aligned(1)));
 };
@@ -210,7 +209,7 @@ __device__ __forceinline__ Raw<T, N> load(const T* __restrict__ row, int column,
     // memory (by elements, each load waited for the one before: [8192, 4095] bf16
     // backward 121 us, 85 so).
     constexpr int kElements = 4 * kChunk / static_cast<int>(sizeof(T));
-    using W = Words_<kChunk, static_cast<int>(sizeof(T))>;
+    using W = WordVector<kChunk, static_cast<int>(sizeof(T))>;
 #pragma unroll
     for (int i = 0; i < kWords; i += kChunk) {
         const int begin = column + i / kChunk * kElements;
@@ -313,18 +312,18 @@ __device__ __forceinline__ void store(T* __restrict__ row, int column, int hidde
         for (int i = 0; i < kWords; i += kChunk) {
             const int offset = column * static_cast<int>(sizeof(T)) + 4 * i;
             if constexpr (kChunk == 4) {
-                const typename Words_<4, 4>::plain words = {raw.words[i], raw.words[i + 1],
+                const typename WordVector<4, 4>::plain words = {raw.words[i], raw.words[i + 1],
                                                             raw.words[i + 2], raw.words[i + 3]};
                 __builtin_amdgcn_raw_buffer_store_b128(words, buffer, offset, 0, Policy);
             } else if constexpr (kChunk == 2) {
-                const typename Words_<2, 4>::plain words = {raw.words[i], raw.words[i + 1]};
+                const typename WordVector<2, 4>::plain words = {raw.words[i], raw.words[i + 1]};
                 __builtin_amdgcn_raw_buffer_store_b64(words, buffer, offset, 0, Policy);
             } else {
                 __builtin_amdgcn_raw_buffer_store_b32(raw.words[i], buffer, offset, 0, Policy);
             }
         }
     } else if (column + N <= hidden) {
-        using W = Words_<kChunk, static_cast<int>(sizeof(T))>;
+        using W = WordVector<kChunk, static_cast<int>(sizeof(T))>;
 #pragma unroll
         for (int i = 0; i < kWords; i += kChunk) {
             typename W::plain words;
@@ -900,6 +899,13 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 //    each adds a row of partial sums ([16384, 4096] bf16: 90 us at 16 waves per CU,
 //    104 at 8, 104 at 32).
 
+//  * Decode-sized forwards, at most a row for each CU, wait for one row's chain of
+//    steps: one slot up to 12 waves ([64, 5120] bf16 e4m3: 4.1 against 4.4 us,
+//    [256, 2048] fp32 3.5 against 3.8), longer rows as above ([8, 4096] fp32:
+//    3.1 with two slots, 3.5 with one and 16 waves).
+
+constexpr int64_t kComputeUnits = 256;
+
 struct Shape {
     int slots;  // V
     int parts;
@@ -937,8 +943,11 @@ inline int64_t blocks_of(int64_t rows, const Shape& shape) {
     return rows / teams + (rows % teams != 0);
 }
 
-inline Shape forward_shape(int64_t hidden, int x_dtype) {
+inline Shape forward_shape(int64_t rows, int64_t hidden, int x_dtype) {
     const int64_t vectors = wave_vectors(hidden, x_dtype);
+    if (rows <= kComputeUnits && vectors <= 12) {
+        return shape_of(vectors, 1, 4);
+    }
     const int most = x_dtype == RLN_DTYPE_F32 ? 4 : 2;
     int slots = x_dtype == RLN_DTYPE_F32 && vectors > 1 ? 2 : 1;
     while (slots < most && slots * 8 < vectors) {
@@ -959,8 +968,6 @@ inline Shape backward_shape(int64_t hidden, int x_dtype) {
     const int slots = vectors <= 8 ? 1 : vectors <= 2 * kMaxParts ? 2 : 4;
     return shape_of(vectors, slots, 8);
 }
-
-constexpr int64_t kComputeUnits = 256;
 
 inline int64_t backward_blocks(int64_t rows, const Shape& shape) {
     const int64_t blocks = blocks_of(rows, shape);
