@@ -25,6 +25,15 @@ int64_t groups_of(int64_t hidden, int64_t group) {
     return group == 0 ? 1 : (hidden + group - 1) / group;
 }
 
+// log2 of a group's columns (valid ones are powers of two).
+int group_shift(int64_t group) {
+    int shift = 0;
+    while (int64_t{1} << shift < group) {
+        ++shift;
+    }
+    return shift;
+}
+
 int check_size(int64_t rows, int64_t hidden) {
     if (rows <= 0) {
         return fail(RLN_ERR_INVALID, "empty tensors are unsupported");
@@ -195,7 +204,7 @@ struct DequantizeArgs {
     int64_t vectors;      // rows * row_vectors
     int row_vectors;      // vectors per row
     int hidden;
-    int group;
+    int group_shift;
     int groups;
     int code_dtype;
     int value_dtype;
@@ -216,7 +225,7 @@ __global__ __launch_bounds__(kDequantizeThreads) void dequantize_kernel(Dequanti
         const int column = static_cast<int>(from - rows_on * a.row_vectors) * N;
         const int64_t row = begin_row + rows_on;
         const bool live = begin + threadIdx.x < a.vectors;
-        const float scale = live ? a.scale[row * a.groups + column / a.group] : 0.0f;
+        const float scale = live ? a.scale[row * a.groups + (column >> a.group_shift)] : 0.0f;
         // Whole vectors lie one after another over the rows, so the block's are
         // one run that starts at a uniform address; short ones go row by row.
         const int64_t left = a.vectors - begin;
@@ -277,6 +286,11 @@ int rln_rms_forward(
         return fail(RLN_ERR_INVALID,
                     "checkpoint and checkpoint_scale must both be given or both be null");
     }
+    if ((status = check_alignment("rstd", rstd, RLN_DTYPE_F32)) != RLN_OK
+        || (status = check_alignment("checkpoint_scale", checkpoint_scale, RLN_DTYPE_F32))
+            != RLN_OK) {
+        return status;
+    }
     a.output_dtype = normalized_dtype;
     a.rstd = rstd;
     a.checkpoint = checkpoint;
@@ -294,9 +308,8 @@ int rln_rms_quantize(
     int64_t rows, int64_t hidden, double eps, void* stream) {
     clear_error();
     ForwardArgs a;
-    const int status = forward_args(x, x_dtype, x_stride, branch, branch_dtype, branch_stride,
-                                    weight, weight_dtype, updated, quantized, rows, hidden, eps,
-                                    stream, &a);
+    int status = forward_args(x, x_dtype, x_stride, branch, branch_dtype, branch_stride, weight,
+                              weight_dtype, updated, quantized, rows, hidden, eps, stream, &a);
     if (status != RLN_OK) {
         return status;
     }
@@ -309,11 +322,14 @@ int rln_rms_quantize(
     if (!scale) {
         return fail(RLN_ERR_INVALID, "forward tensors must not be null");
     }
+    if ((status = check_alignment("scale", scale, RLN_DTYPE_F32)) != RLN_OK) {
+        return status;
+    }
     a.output_dtype = quantized_dtype;
     a.scale = scale;
     a.groups = static_cast<int>(groups_of(hidden, group));
     // One scale per row, also where a group is as long as the row.
-    a.group = a.groups == 1 ? static_cast<int>(kMaxHidden) : static_cast<int>(group);
+    a.group_shift = a.groups == 1 ? kWholeRow : group_shift(group);
     return launch(a, x_dtype, branch_dtype, Mode::kQuantize, stream);
 }
 
@@ -366,6 +382,9 @@ int rln_rms_backward(
         || (status = check_alignment("grad_x", grad_x, x_dtype)) != RLN_OK
         || (status = check_alignment("grad_branch", grad_branch, branch_dtype)) != RLN_OK
         || (status = check_alignment("grad_weight", grad_weight, weight_dtype)) != RLN_OK
+        || (status = check_alignment("rstd", rstd, RLN_DTYPE_F32)) != RLN_OK
+        || (status = check_alignment("checkpoint_scale", checkpoint_scale, RLN_DTYPE_F32))
+            != RLN_OK
         || (status = check_alignment("workspace", workspace, RLN_DTYPE_F32)) != RLN_OK) {
         return status;
     }
@@ -468,7 +487,7 @@ int rln_dequantize(
     a.vectors = rows * a.row_vectors;
     a.hidden = static_cast<int>(hidden);
     a.groups = static_cast<int>(groups_of(hidden, group));
-    a.group = group == 0 ? INT32_MAX : static_cast<int>(group);
+    a.group_shift = group == 0 ? kWholeRow : group_shift(group);
     a.code_dtype = quantized_dtype;
     a.value_dtype = values_dtype;
     int64_t blocks = (a.vectors + kDequantizeThreads - 1) / kDequantizeThreads;

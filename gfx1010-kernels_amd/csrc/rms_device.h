@@ -58,6 +58,8 @@ constexpr int kWave = 64;
 constexpr int64_t kMaxHidden = 16384;
 constexpr int kMaxParts = 16;
 constexpr int kCheckpointGroup = 128;
+// As the shift of a column to its group: every column is in group 0.
+constexpr int kWholeRow = 31;
 // The least maximum of a group: keeps Q / max finite where a group is all
 // zeros (or below 2^-100, far under any value a norm is fed).
 constexpr float kLeastMaximum = 0x1p-100f;
@@ -93,7 +95,7 @@ struct ForwardArgs {
     int words;          // Access::kWords serves every tensor
     int weight_dtype;
     int output_dtype;   // normalized's, or the codes'
-    int group;          // columns under one scale, a multiple of the vector
+    int group_shift;    // log2 of the columns under one scale, or kWholeRow
     int groups;         // scales per row
     float eps;
     float inv_hidden;
@@ -639,7 +641,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
                     maximum[v] = whole;
                 }
             } else {
-                const int lanes = kMode == Mode::kCheckpoint ? kCheckpointGroup / N : a.group / N;
+                const int lanes = kMode == Mode::kCheckpoint ? kCheckpointGroup / N : (1 << a.group_shift) / N;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     maximum[v] = lanes_max(maximum[v], lanes);
@@ -681,8 +683,9 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const GroupScale scale = group_scale(maximum[v], top);
-                if (column[v] < hidden && column[v] % a.group == 0) {
-                    a.scale[row * a.groups + column[v] / a.group] = scale.step * rstd;
+                const int group = column[v] >> a.group_shift;
+                if (column[v] < hidden && group << a.group_shift == column[v]) {
+                    a.scale[row * a.groups + group] = scale.step * rstd;
                 }
                 float steps[N];
 #pragma unroll

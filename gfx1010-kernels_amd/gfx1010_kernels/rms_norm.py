@@ -18,8 +18,8 @@ no dropout: models that norm by the root mean square train without it, and
 ``F.dropout(branch)`` before the call is the same computation.
 
 The PyTorch decomposition (``implementation="torch"``, and what ``"auto"`` falls
-back to with a ``RuntimeWarning``) computes the same formulas in fp32, 8-bit
-codes and checkpoints included.
+back to with a ``RuntimeWarning``) computes the same formulas in fp32 (fp64 for
+fp64 tensors), 8-bit codes and checkpoints included.
 """
 
 from __future__ import annotations
@@ -68,7 +68,7 @@ def _codes(values, group, dtype):
     steps = (values * inverse[..., :values.shape[-1]]).clamp(-_LARGEST_CODE[dtype],
                                                              _LARGEST_CODE[dtype])
     steps = steps.nan_to_num(nan=0.0)
-    codes = (steps.round() if dtype == torch.int8 else steps).to(dtype)
+    codes = (steps.round() if dtype == torch.int8 else steps.float()).to(dtype)
     return codes, torch.where(finite, largest / top, torch.nan)
 
 
@@ -76,8 +76,13 @@ def _widened(codes, step, group):
     return codes.float() * step.repeat_interleave(group, -1)[..., :codes.shape[-1]]
 
 
+def _wide(tensor):
+    """fp32, or fp64 for an fp64 tensor (which only this path serves)."""
+    return tensor if tensor.dtype == torch.float64 else tensor.float()
+
+
 def _torch_update(x, branch):
-    return x if branch is None else (x.float() + branch.float()).to(x.dtype)
+    return x if branch is None else (_wide(x) + _wide(branch)).to(x.dtype)
 
 
 def _rstd(values, eps):
@@ -89,20 +94,20 @@ class _TorchCheckpointNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, updated, weight, eps, dtype):
-        values = updated.float()
+        values = _wide(updated)
         rstd = _rstd(values, eps)
         codes, step = _codes(values, CHECKPOINT_GROUP, torch.int8)
         ctx.save_for_backward(codes, step, rstd, weight)
         ctx.dtype = updated.dtype
-        return (values * rstd * weight.float()).to(dtype)
+        return (values * rstd * _wide(weight)).to(dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_normalized):
         codes, step, rstd, weight = ctx.saved_tensors
         unit = _widened(codes, step, CHECKPOINT_GROUP) * rstd
-        upstream = grad_normalized.float()
-        product = upstream * weight.float()
+        upstream = _wide(grad_normalized)
+        product = upstream * _wide(weight)
         shared = (product * unit).mean(-1, keepdim=True)
         grad_weight = (upstream * unit).flatten(0, -2).sum(0) if unit.ndim > 1 else upstream * unit
         return ((rstd * (product - unit * shared)).to(ctx.dtype), grad_weight.to(weight.dtype),
@@ -114,16 +119,16 @@ def _torch_residual_rms_norm(x, branch, weight, eps, normalized_dtype, checkpoin
     dtype = normalized_dtype or x.dtype
     if checkpoint:
         return updated, _TorchCheckpointNorm.apply(updated, weight, eps, dtype)
-    values = updated.float()
-    return updated, (values * _rstd(values, eps) * weight.float()).to(dtype)
+    values = _wide(updated)
+    return updated, (values * _rstd(values, eps) * _wide(weight)).to(dtype)
 
 
 def _torch_quantized(x, branch, weight, eps, dtype, group_size):
     updated = _torch_update(x, branch)
-    values = updated.float()
+    values = _wide(updated)
     group = group_size or max(1, values.shape[-1])
-    codes, step = _codes(values * weight.float(), group, dtype)
-    return updated, codes, step * _rstd(values, eps)
+    codes, step = _codes(values * _wide(weight), group, dtype)
+    return updated, codes, (step * _rstd(values, eps)).float()
 
 
 def _torch_dequantize(quantized, scale, group_size, dtype):

@@ -16,10 +16,14 @@
  * csrc/residual_layer_norm_kernel.hip:425-545 (forward), :548-618 (input
  * gradients), :727-869 (weight/bias gradients).
  *
+ * The same operator with a root-mean-square norm, its 8-bit output and its 8-bit
+ * checkpoint are the rln_rms_* entry points and rln_dequantize below.
+ *
  * Conventions shared by every entry point:
  *  - All pointers are device pointers on the calling thread's current HIP
  *    device, except `philox` (host pointer to a descriptor).
- *  - Tensors are dense row-major [rows, hidden]; mean/rstd are [rows].
+ *  - Tensors are dense row-major [rows, hidden] (rln_rms_*: where not given a
+ *    stride); mean/rstd are [rows].
  *  - The dropout mask is `rows * hidden / 32` uint32 words: keep(r, c) is
  *    bit (c % 32) of word r * hidden / 32 + c / 32 - the reference's layout
  *    (csrc/residual_layer_norm_kernel.hip:500-511, :162-164).

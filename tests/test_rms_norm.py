@@ -103,6 +103,26 @@ def test_torch_path_quantizes_as_defined(hidden, group, dtype):
     assert ((values.double() - wide).abs() <= half * 1.0001 * steps + 1e-30).all()
 
 
+@pytest.mark.parametrize("hidden", [5, 200])
+def test_torch_path_keeps_fp64(hidden):
+    """fp64 tensors, which the kernels do not take, are computed in fp64."""
+    x, branch, weight = (t.double() for t in make((4, hidden)))
+    branch = branch + 2.0 ** -40
+    updated, normalized = residual_rms_norm(x, branch, weight, EPS, implementation="torch")
+    assert torch.equal(updated, x + branch) and normalized.dtype == torch.float64
+    torch.testing.assert_close(normalized, F.rms_norm(x + branch, (hidden,), weight, EPS),
+                               rtol=1e-14, atol=1e-14)
+    assert torch.autograd.gradcheck(
+        lambda *t: residual_rms_norm(*t, EPS, implementation="torch"),
+        [t.requires_grad_() for t in (x, branch, weight)], atol=1e-6)
+    with torch.no_grad():
+        _, codes, scale = residual_rms_norm_quantized(x, branch, weight, EPS,
+                                                      implementation="torch")
+    assert scale.dtype == torch.float32
+    assert (dequantize(codes, scale, dtype=torch.float32, implementation="torch") - normalized
+            ).abs().max() <= 16.001 * scale.max()
+
+
 def test_torch_path_marks_groups_that_are_not_finite():
     x = torch.randn(2, 256)
     x[0, 130] = float("inf")
@@ -258,6 +278,8 @@ SHARED = [
     (dict(normalized=None), "must not be null"),
     (dict(normalized_dtype=E4M3), "normalized must use"),
     (dict(normalized=FAKE + 1), "normalized is not aligned"),
+    (dict(rstd=FAKE + 2), "rstd is not aligned"),
+    (dict(checkpoint=FAKE, checkpoint_scale=FAKE + 1), "checkpoint_scale is not aligned"),
     (dict(checkpoint=FAKE), "checkpoint and checkpoint_scale must both"),
 ])
 def test_forward_refusals(changes, message):
@@ -271,6 +293,7 @@ def test_forward_refusals(changes, message):
     (dict(quantized_dtype=BF16), "quantized must use"),
     (dict(group=48), "group must be"),
     (dict(group=-32), "group must be"),
+    (dict(scale=FAKE + 1), "scale is not aligned"),
 ])
 def test_quantize_refusals(changes, message):
     with pytest.raises(_cabi.RlnError, match=message):
@@ -295,6 +318,9 @@ def test_quantize_refusals(changes, message):
     (dict(grad_weight=FAKE), "workspace too small"),
     (dict(grad_weight=FAKE, workspace=FAKE, workspace_bytes=8), "workspace too small"),
     (dict(workspace=FAKE + 2), "workspace is not aligned"),
+    (dict(rstd=FAKE + 1), "rstd is not aligned"),
+    (dict(updated=None, checkpoint=FAKE, checkpoint_scale=FAKE + 3),
+     "checkpoint_scale is not aligned"),
     (dict(updated_stride=1 << 61), "updated: the row stride overflows"),
 ])
 def test_backward_refusals(changes, message):
