@@ -234,7 +234,8 @@ __global__ __launch_bounds__(kDequantizeThreads) void dequantize_kernel(Dequanti
         const int extent = kRun
             ? static_cast<int>(left < kDequantizeThreads ? left : kDequantizeThreads) * N
             : live ? a.hidden : 0;
-        const Raw<int8_t, N> raw = load<kAccess, int8_t, N>(a.codes + first, place, extent);
+        auto raw = load<kAccess, int8_t, N>(a.codes + first, place, extent);
+        settle<kAccess>(raw, place, extent);
         float values[N];
         if (a.code_dtype == RLN_DTYPE_E4M3) {
             widen_e4m3<N>(raw, values);

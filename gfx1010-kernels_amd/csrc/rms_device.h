@@ -140,11 +140,17 @@ RMS_WORDS(2, 4);
 RMS_WORDS(2, 2);
 RMS_WORDS(2, 1);
 #undef RMS_WORDS
-template <>
-struct WordVector<1, 1> {
-    typedef uint32_t plain;
-    typedef uint32_t type __attribute__((aligned(1)));
-};
+#define RMS_WORD(alignment)                                                             \
+    template <>                                                                         \
+    struct WordVector<1, alignment> {                                                   \
+        typedef uint32_t plain;                                                         \
+        typedef uint32_t type __attribute__((aligned(alignment)));                      \
+    }
+RMS_WORD(4);
+RMS_WORD(2);
+RMS_WORD(1);
+#undef RMS_WORD
+typedef uint16_t AnyHalf __attribute__((aligned(1)));
 
 // N elements of T as 32-bit words.
 template <typename T, int N>
@@ -179,7 +185,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const T* row, int c
 }
 
 // Elements [column, column + N) of a row of `hidden` (both wave-uniform but for
-// the column), zeros past its end.
+// the column), zeros past its end; settle() has to follow before they are used.
 template <Access kAccess, typename T, int N, int Policy = kOnce>
 __device__ __forceinline__ Raw<T, N> load(const T* __restrict__ row, int column, int hidden) {
     Raw<T, N> raw;
@@ -207,59 +213,81 @@ __device__ __forceinline__ Raw<T, N> load(const T* __restrict__ row, int column,
         return raw;
     }
     // Vectors of up to 16 bytes; one that crosses the row's end is read from the
-    // row's last whole vector and shifted down, so that no lane branches around
-    // memory (by elements, each load waited for the one before: [8192, 4095] bf16
-    // backward 121 us, 85 so).
+    // row's last whole vector, so that no lane branches around memory, and shifted
+    // down by settle(), so that no load waits for another.
     constexpr int kElements = 4 * kChunk / static_cast<int>(sizeof(T));
     using W = WordVector<kChunk, static_cast<int>(sizeof(T))>;
 #pragma unroll
     for (int i = 0; i < kWords; i += kChunk) {
         const int begin = column + i / kChunk * kElements;
-        unsigned __int128 bits = 0;
+        typename W::plain words{};
         if (hidden >= kElements) {
             const int start = begin < hidden - kElements ? begin : hidden - kElements;
             const typename W::type* from = reinterpret_cast<const typename W::type*>(row + start);
-            typename W::plain words;
             if constexpr (Policy == kOnce) {
                 words = __builtin_nontemporal_load(from);
             } else {
                 words = *from;
             }
-            if constexpr (kChunk == 1) {
-                bits = words;
-            } else {
+        }
+        if constexpr (kChunk == 1) {
+            raw.words[i] = words;
+        } else {
 #pragma unroll
-                for (int k = kChunk - 1; k >= 0; --k) {
-                    bits = bits << 32 | words[k];
-                }
-            }
-            if (begin != start) {
-                const int shift = (begin - start) * 8 * static_cast<int>(sizeof(T));
-                bits = begin < hidden ? bits >> shift : 0;
-            }
-        } else {  // rows shorter than a vector, and no row at all
-#pragma unroll
-            for (int e = 0; e < kElements - 1; ++e) {
-                if (begin + e < hidden) {
-                    uint32_t element;
-                    if constexpr (sizeof(T) == 4) {
-                        element = reinterpret_cast<const uint32_t*>(row)[begin + e];
-                    } else if constexpr (sizeof(T) == 2) {
-                        element = reinterpret_cast<const uint16_t*>(row)[begin + e];
-                    } else {
-                        element = reinterpret_cast<const uint8_t*>(row)[begin + e];
-                    }
-                    bits |= static_cast<unsigned __int128>(element)
-                        << (e * 8 * static_cast<int>(sizeof(T)));
-                }
+            for (int k = 0; k < kChunk; ++k) {
+                raw.words[i + k] = words[k];
             }
         }
+    }
+    if (hidden < kElements) {  // rows shorter than a vector, and no row at all
 #pragma unroll
-        for (int k = 0; k < kChunk; ++k) {
-            raw.words[i + k] = static_cast<uint32_t>(bits >> (32 * k));
+        for (int e = 0; e < kElements - 1; ++e) {
+            if (column + e < hidden) {
+                uint32_t element;
+                if constexpr (sizeof(T) == 4) {
+                    element = reinterpret_cast<const uint32_t*>(row)[column + e];
+                } else if constexpr (sizeof(T) == 2) {
+                    element = reinterpret_cast<const uint16_t*>(row)[column + e];
+                } else {
+                    element = reinterpret_cast<const uint8_t*>(row)[column + e];
+                }
+                constexpr int kPerWord = 4 / static_cast<int>(sizeof(T));
+                raw.words[e / kPerWord] |=
+                    element << (e % kPerWord * 8 * static_cast<int>(sizeof(T)));
+            }
         }
     }
     return raw;
+}
+
+// The second half of load(): moves the vectors that were read from an earlier
+// column to their place, zeros behind them. By elements under branches, or
+// shifted right after each load, the loads of a row waited for one another
+// ([8192, 4095] bf16 backward 121 and 85 us).
+template <Access kAccess, typename T, int N>
+__device__ __forceinline__ void settle(Raw<T, N>& raw, int column, int hidden) {
+    if constexpr (!kBuffer<kAccess, T>) {
+        constexpr int kWords = Raw<T, N>::kWords;
+        constexpr int kChunk = kWords < 4 ? kWords : 4;
+        constexpr int kElements = 4 * kChunk / static_cast<int>(sizeof(T));
+#pragma unroll
+        for (int i = 0; i < kWords; i += kChunk) {
+            const int begin = column + i / kChunk * kElements;
+            if (hidden >= kElements && begin > hidden - kElements) {
+                unsigned __int128 bits = 0;
+#pragma unroll
+                for (int k = kChunk - 1; k >= 0; --k) {
+                    bits = bits << 32 | raw.words[i + k];
+                }
+                const int shift = (begin - hidden + kElements) * 8 * static_cast<int>(sizeof(T));
+                bits = begin < hidden ? bits >> shift : 0;
+#pragma unroll
+                for (int k = 0; k < kChunk; ++k) {
+                    raw.words[i + k] = static_cast<uint32_t>(bits >> (32 * k));
+                }
+            }
+        }
+    }
 }
 
 template <typename T, int N>
@@ -340,20 +368,43 @@ __device__ __forceinline__ void store(T* __restrict__ row, int column, int hidde
             __builtin_nontemporal_store(
                 words, reinterpret_cast<typename W::type*>(row + column) + i / kChunk);
         }
-    } else {
-        constexpr int kPerWord = 4 / static_cast<int>(sizeof(T));
+    } else if (column >= hidden) {
+        return;
+    } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int e = 0; e < N - 1; ++e) {
             if (column + e < hidden) {
-                const uint32_t bits =
-                    raw.words[e / kPerWord] >> (e % kPerWord * 8 * static_cast<int>(sizeof(T)));
-                if constexpr (sizeof(T) == 4) {
-                    reinterpret_cast<uint32_t*>(row)[column + e] = bits;
-                } else if constexpr (sizeof(T) == 2) {
-                    reinterpret_cast<uint16_t*>(row)[column + e] = static_cast<uint16_t>(bits);
+                reinterpret_cast<uint32_t*>(row)[column + e] = raw.words[e];
+            }
+        }
+    } else {
+        // The row's last elements, in at most three pieces of falling size.
+        unsigned __int128 bits = 0;
+#pragma unroll
+        for (int k = kWords - 1; k >= 0; --k) {
+            bits = bits << 32 | raw.words[k];
+        }
+        const int count = hidden - column;
+        int place = column;
+#pragma unroll
+        for (int piece = N / 2; piece >= 1; piece /= 2) {
+            if (count & piece) {
+                const int bytes = piece * static_cast<int>(sizeof(T));
+                if (bytes == 8) {
+                    using W = WordVector<2, static_cast<int>(sizeof(T))>;
+                    const typename W::plain words = {static_cast<uint32_t>(bits),
+                                                     static_cast<uint32_t>(bits >> 32)};
+                    *reinterpret_cast<typename W::type*>(row + place) = words;
+                } else if (bytes == 4) {
+                    *reinterpret_cast<typename WordVector<1, static_cast<int>(sizeof(T))>::type*>(
+                        row + place) = static_cast<uint32_t>(bits);
+                } else if (bytes == 2) {
+                    *reinterpret_cast<AnyHalf*>(row + place) = static_cast<uint16_t>(bits);
                 } else {
-                    reinterpret_cast<uint8_t*>(row)[column + e] = static_cast<uint8_t>(bits);
+                    *reinterpret_cast<uint8_t*>(row + place) = static_cast<uint8_t>(bits);
                 }
+                bits >>= 8 * bytes;
+                place += piece;
             }
         }
     }
@@ -365,14 +416,20 @@ template <Access kAccess, int N>
 __device__ __forceinline__ void load_weight(const void* weight, int dtype, int column, int hidden,
                                             float (&out)[N]) {
     if (dtype == RLN_DTYPE_F32) {
-        widen<float, N>(
-            load<kAccess, float, N, kCached>(static_cast<const float*>(weight), column, hidden), out);
+        auto raw = load<kAccess, float, N, kCached>(static_cast<const float*>(weight), column,
+                                                    hidden);
+        settle<kAccess>(raw, column, hidden);
+        widen<float, N>(raw, out);
     } else if (dtype == RLN_DTYPE_F16) {
-        widen<half_t, N>(
-            load<kAccess, half_t, N, kCached>(static_cast<const half_t*>(weight), column, hidden), out);
+        auto raw = load<kAccess, half_t, N, kCached>(static_cast<const half_t*>(weight), column,
+                                                     hidden);
+        settle<kAccess>(raw, column, hidden);
+        widen<half_t, N>(raw, out);
     } else {
-        widen<bf16_t, N>(
-            load<kAccess, bf16_t, N, kCached>(static_cast<const bf16_t*>(weight), column, hidden), out);
+        auto raw = load<kAccess, bf16_t, N, kCached>(static_cast<const bf16_t*>(weight), column,
+                                                     hidden);
+        settle<kAccess>(raw, column, hidden);
+        widen<bf16_t, N>(raw, out);
     }
 }
 
@@ -579,6 +636,8 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 float added[N];
+                settle<kAccess>(raw_x[v], column[v], hidden);
+                settle<kAccess>(raw_branch[v], column[v], hidden);
                 widen<X, N>(raw_x[v], u[v]);
                 widen<B, N>(raw_branch[v], added);
 #pragma unroll
@@ -595,6 +654,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 load_weight<kAccess, N>(a.weight, a.weight_dtype, column[v], hidden, weight[v]);
+                settle<kAccess>(raw_x[v], column[v], hidden);
                 widen<X, N>(raw_x[v], u[v]);
             }
         }
@@ -798,14 +858,17 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float upstream[N];
+            settle<kAccess>(raw_y[v], column[v], hidden);
             widen<Y, N>(raw_y[v], upstream);
             if constexpr (Checkpoint) {
+                settle<kAccess>(raw_kept[v], column[v], hidden);
                 widen<int8_t, N>(raw_kept[v], unit[v]);
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
                     unit[v][e] = unit[v][e] * kept_step[v];
                 }
             } else {
+                settle<kAccess>(raw_u[v], column[v], hidden);
                 widen<X, N>(raw_u[v], unit[v]);
             }
 #pragma unroll
@@ -833,6 +896,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float gradient[N];
+            settle<kAccess>(raw_grad[v], column[v], hidden);
             widen<X, N>(raw_grad[v], gradient);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
