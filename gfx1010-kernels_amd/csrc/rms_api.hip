@@ -220,7 +220,8 @@ __global__ __launch_bounds__(kDequantizeThreads) void dequantize_kernel(Dequanti
     for (int64_t begin = static_cast<int64_t>(blockIdx.x) * kDequantizeThreads;
          begin < a.vectors; begin += step) {
         const int64_t begin_row = begin / a.row_vectors;
-        const uint32_t from = static_cast<uint32_t>(begin - begin_row * a.row_vectors) + threadIdx.x;
+        const uint32_t from =
+            static_cast<uint32_t>(begin - begin_row * a.row_vectors) + threadIdx.x;
         const uint32_t rows_on = from / static_cast<uint32_t>(a.row_vectors);
         const int column = static_cast<int>(from - rows_on * a.row_vectors) * N;
         const int64_t row = begin_row + rows_on;
@@ -246,7 +247,8 @@ __global__ __launch_bounds__(kDequantizeThreads) void dequantize_kernel(Dequanti
         for (int e = 0; e < N; ++e) {
             values[e] *= scale;
         }
-        store_as<kAccess, kBackwardStores, N>(a.values, a.value_dtype, first, place, extent, values);
+        store_as<kAccess, kBackwardStores, N>(a.values, a.value_dtype, first, place, extent,
+                                              values);
     }
 }
 
@@ -496,11 +498,11 @@ int rln_dequantize(
     const hipStream_t queue = static_cast<hipStream_t>(stream);
     if (hidden % 8 == 0 && whole_words(quantized, quantized_dtype, 0, 8)
         && whole_words(values, values_dtype, 0, 8)) {
-        dequantize_kernel<Access::kWords><<<dim3(static_cast<unsigned>(blocks)), kDequantizeThreads, 0,
-                                  queue>>>(a);
+        dequantize_kernel<Access::kWords>
+            <<<dim3(static_cast<unsigned>(blocks)), kDequantizeThreads, 0, queue>>>(a);
     } else {
-        dequantize_kernel<Access::kLanes><<<dim3(static_cast<unsigned>(blocks)), kDequantizeThreads, 0,
-                                   queue>>>(a);
+        dequantize_kernel<Access::kLanes>
+            <<<dim3(static_cast<unsigned>(blocks)), kDequantizeThreads, 0, queue>>>(a);
     }
     return check_launch("rms dequantize_kernel");
 }

@@ -438,13 +438,13 @@ __device__ __forceinline__ void store_as(void* tensor, int dtype, int64_t first,
                                          int hidden, const float (&values)[N]) {
     if (dtype == RLN_DTYPE_F32) {
         store<kAccess, Policy, float, N>(static_cast<float*>(tensor) + first, column, hidden,
-                              narrow<float, N>(values));
+                                         narrow<float, N>(values));
     } else if (dtype == RLN_DTYPE_F16) {
         store<kAccess, Policy, half_t, N>(static_cast<half_t*>(tensor) + first, column, hidden,
-                               narrow<half_t, N>(values));
+                                          narrow<half_t, N>(values));
     } else {
         store<kAccess, Policy, bf16_t, N>(static_cast<bf16_t*>(tensor) + first, column, hidden,
-                               narrow<bf16_t, N>(values));
+                                          narrow<bf16_t, N>(values));
     }
 }
 
@@ -461,7 +461,8 @@ __device__ __forceinline__ Raw<int8_t, N> narrow_int8(const float (&steps)[N]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float whole = __builtin_rintf(steps[4 * w + e]);
-            const int code = static_cast<int>(__builtin_fminf(__builtin_fmaxf(whole, -127.0f), 127.0f));
+            const int code =
+                static_cast<int>(__builtin_fminf(__builtin_fmaxf(whole, -127.0f), 127.0f));
             word |= (static_cast<uint32_t>(code) & 0xffu) << (8 * e);
         }
         raw.words[w] = word;
@@ -752,9 +753,9 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
                 for (int e = 0; e < N; ++e) {
                     steps[e] = u[v][e] * scale.inverse;
                 }
-                store<kAccess, kForwardStores, int8_t, N>(static_cast<int8_t*>(a.normalized) + first, column[v],
-                                       hidden,
-                                       e4m3 ? narrow_e4m3<N>(steps) : narrow_int8<N>(steps));
+                store<kAccess, kForwardStores, int8_t, N>(
+                    static_cast<int8_t*>(a.normalized) + first, column[v], hidden,
+                    e4m3 ? narrow_e4m3<N>(steps) : narrow_int8<N>(steps));
             }
         } else {
 #pragma unroll
@@ -769,16 +770,16 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
                     for (int e = 0; e < N; ++e) {
                         steps[e] = u[v][e] * scale.inverse;
                     }
-                    store<kAccess, kForwardStores, int8_t, N>(a.checkpoint + first, column[v], hidden,
-                                           narrow_int8<N>(steps));
+                    store<kAccess, kForwardStores, int8_t, N>(
+                        a.checkpoint + first, column[v], hidden, narrow_int8<N>(steps));
                 }
                 float normalized[N];
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
                     normalized[e] = u[v][e] * rstd * weight[v][e];
                 }
-                store_as<kAccess, kForwardStores, N>(a.normalized, a.output_dtype, first, column[v], hidden,
-                                  normalized);
+                store_as<kAccess, kForwardStores, N>(a.normalized, a.output_dtype, first,
+                                                     column[v], hidden, normalized);
             }
         }
     }
@@ -826,7 +827,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             raw_y[v] = load<kAccess, Y, N>(static_cast<const Y*>(a.grad_normalized) + first,
-                                        column[v], hidden);
+                                           column[v], hidden);
             if constexpr (Checkpoint) {
                 raw_kept[v] = load<kAccess, int8_t, N>(a.checkpoint + first, column[v], hidden);
                 kept_step[v] = column[v] < hidden
@@ -840,7 +841,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 raw_grad[v] = load<kAccess, X, N>(static_cast<const X*>(a.grad_updated) + first,
-                                               column[v], hidden);
+                                                  column[v], hidden);
             }
         } else {
 #pragma unroll
@@ -865,7 +866,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
                 widen<int8_t, N>(raw_kept[v], unit[v]);
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    unit[v][e] = unit[v][e] * kept_step[v];
+                    unit[v][e] *= kept_step[v];
                 }
             } else {
                 settle<kAccess>(raw_u[v], column[v], hidden);
@@ -902,11 +903,11 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
             for (int e = 0; e < N; ++e) {
                 gradient[e] += rstd * (product[v][e] - unit[v][e] * shared);
             }
-            store<kAccess, kBackwardStores, X, N>(static_cast<X*>(a.grad_x) + first, column[v], hidden,
-                              narrow<X, N>(gradient));
+            store<kAccess, kBackwardStores, X, N>(static_cast<X*>(a.grad_x) + first, column[v],
+                                                  hidden, narrow<X, N>(gradient));
             if (a.grad_branch != nullptr) {
-                store_as<kAccess, kBackwardStores, N>(a.grad_branch, a.branch_dtype, first, column[v], hidden,
-                                  gradient);
+                store_as<kAccess, kBackwardStores, N>(a.grad_branch, a.branch_dtype, first,
+                                                      column[v], hidden, gradient);
             }
         }
     }
@@ -940,7 +941,8 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
                     }
                 }
             }
-            store<kAccess, kBackwardStores, float, N>(partial, column[v], a.hidden, narrow<float, N>(grad_weight[v]));
+            store<kAccess, kBackwardStores, float, N>(partial, column[v], a.hidden,
+                                                      narrow<float, N>(grad_weight[v]));
         }
     }
 }

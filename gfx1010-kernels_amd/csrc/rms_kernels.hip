@@ -19,11 +19,9 @@ int launch(Kernel kernel, const Args& a, int64_t blocks, int threads, size_t lds
 template <typename X, typename B, int V, Mode kMode>
 int forward_access(const ForwardArgs& a, const Shape& shape, hipStream_t stream) {
     const int64_t blocks = forward_blocks(a.rows, shape);
-    return a.words
-        ? launch(forward_kernel<X, B, V, kMode, Access::kWords>, a, blocks, shape.threads, 0, stream,
-                 "rms forward_kernel")
-        : launch(forward_kernel<X, B, V, kMode, Access::kElements>, a, blocks, shape.threads, 0, stream,
-                 "rms forward_kernel");
+    const auto kernel = a.words ? forward_kernel<X, B, V, kMode, Access::kWords>
+                                : forward_kernel<X, B, V, kMode, Access::kElements>;
+    return launch(kernel, a, blocks, shape.threads, 0, stream, "rms forward_kernel");
 }
 
 template <typename X, typename B, Mode kMode>
@@ -62,11 +60,9 @@ int backward_access(const BackwardArgs& a, const Shape& shape, hipStream_t strea
     const int64_t blocks = backward_blocks(a.rows, shape);
     const size_t lds = a.partials == nullptr
         ? 0 : static_cast<size_t>(teams_of(shape) - 1) * a.hidden * sizeof(float);
-    return a.words
-        ? launch(backward_kernel<X, Y, V, Checkpoint, Access::kWords>, a, blocks, shape.threads, lds,
-                 stream, "rms backward_kernel")
-        : launch(backward_kernel<X, Y, V, Checkpoint, Access::kElements>, a, blocks, shape.threads, lds,
-                 stream, "rms backward_kernel");
+    const auto kernel = a.words ? backward_kernel<X, Y, V, Checkpoint, Access::kWords>
+                                : backward_kernel<X, Y, V, Checkpoint, Access::kElements>;
+    return launch(kernel, a, blocks, shape.threads, lds, stream, "rms backward_kernel");
 }
 
 template <typename X, typename Y, bool Checkpoint>

@@ -272,8 +272,9 @@ int rln_supported_hidden_sizes(int64_t* out, int capacity);
  *   normalized = updated * rstd * weight          (fp32, rounded to normalized's type)
  *
  * x, branch, weight and normalized each use fp32, fp16 or bf16; updated has x's
- * type. No output may overlap an input. x and branch are rows of consecutive elements, `x_stride` and
- * `branch_stride` elements apart (any value, 0 for one row read by all);
+ * type. No output may overlap an input. x and branch are rows of consecutive
+ * elements, `x_stride` and `branch_stride` elements apart (any value, 0 for one
+ * row read by all);
  * updated and normalized are dense. Every address is aligned to its elements; more
  * is not asked. Any hidden from 1 to 16384 (rln_rms_hidden_supported).
  * branch and updated are both NULL for a norm without an addition (updated = x).

@@ -28,9 +28,10 @@ pytestmark = pytest.mark.gpu
 EPS = 1e-6
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 CODE = {F32: 0, F16: 1, BF16: 2, torch.int8: 3, torch.float8_e4m3fn: 4}
-LENGTHS = [1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 31, 64, 100, 127, 128, 129, 200, 254, 255, 256, 257,
-           384, 510, 511, 512, 513, 514, 516, 768, 1000, 1001, 1023, 1024, 1025, 1030, 1280, 1600, 2046, 2047, 2048, 2049, 2880, 4094, 4095, 4096, 4097, 4100,
-           5120, 6000, 8191, 8192, 8193, 8194, 11008, 12289, 16383, 16384]
+LENGTHS = [1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 31, 64, 100, 127, 128, 129, 200, 254, 255, 256, 257, 384,
+           510, 511, 512, 513, 514, 516, 768, 1000, 1001, 1023, 1024, 1025, 1030, 1280, 1600, 2046,
+           2047, 2048, 2049, 2880, 4094, 4095, 4096, 4097, 4100, 5120, 6000, 8191, 8192, 8193,
+           8194, 11008, 12289, 16383, 16384]
 TYPES = list(itertools.product([F32, F16, BF16], repeat=2))
 
 
