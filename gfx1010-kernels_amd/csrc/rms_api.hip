@@ -183,13 +183,7 @@ __global__ __launch_bounds__(kReduceColumns * kReduceGroups) void reduce_kernel(
         for (int other = 0; other < kReduceGroups; ++other) {
             sum += totals[other][lane];
         }
-        if (dtype == RLN_DTYPE_F32) {
-            static_cast<float*>(grad_weight)[column] = sum;
-        } else if (dtype == RLN_DTYPE_F16) {
-            static_cast<half_t*>(grad_weight)[column] = static_cast<half_t>(sum);
-        } else {
-            static_cast<bf16_t*>(grad_weight)[column] = static_cast<bf16_t>(sum);
-        }
+        store_one(grad_weight, dtype, column, sum);
     }
 }
 
@@ -337,7 +331,8 @@ int rln_rms_quantize(
 }
 
 size_t rln_rms_backward_workspace_bytes(int64_t rows, int64_t hidden, int x_dtype) {
-    if (rows <= 0 || !rln_rms_hidden_supported(hidden) || !float_dtype(x_dtype)) {
+    if (rows <= 0 || !rln_rms_hidden_supported(hidden) || !float_dtype(x_dtype)
+        || backward_slabs(rows, hidden)) {
         return 0;
     }
     return static_cast<size_t>(backward_blocks(rows, backward_shape(hidden, x_dtype)))
@@ -411,7 +406,11 @@ int rln_rms_backward(
     a.rstd = rstd;
     a.grad_x = grad_x;
     a.grad_branch = grad_branch;
-    a.partials = grad_weight != nullptr ? static_cast<float*>(workspace) : nullptr;
+    const bool slabs = grad_weight != nullptr && backward_slabs(rows, hidden);
+    a.partials = grad_weight != nullptr && !slabs ? static_cast<float*>(workspace) : nullptr;
+    a.grad_weight = grad_weight;
+    const int slab_columns = kSlabLanes * columns_of(x_dtype);
+    a.slabs = slabs ? static_cast<int>((hidden + slab_columns - 1) / slab_columns) : 0;
     a.updated_stride = updated_stride;
     a.rows = rows;
     a.hidden = static_cast<int>(hidden);
@@ -439,7 +438,7 @@ int rln_rms_backward(
             status = launch_backward<bf16_t>(a, shape, grad_normalized_dtype, queue);
             break;
     }
-    if (status != RLN_OK || grad_weight == nullptr) {
+    if (status != RLN_OK || grad_weight == nullptr || slabs) {
         return status;
     }
     const unsigned blocks =
@@ -494,7 +493,7 @@ int rln_dequantize(
     a.code_dtype = quantized_dtype;
     a.value_dtype = values_dtype;
     int64_t blocks = (a.vectors + kDequantizeThreads - 1) / kDequantizeThreads;
-    blocks = blocks < kForwardMaxBlocks ? blocks : kForwardMaxBlocks;
+    blocks = blocks < kMaxBlocks ? blocks : kMaxBlocks;
     const hipStream_t queue = static_cast<hipStream_t>(stream);
     if (hidden % 8 == 0 && whole_words(quantized, quantized_dtype, 0, 8)
         && whole_words(values, values_dtype, 0, 8)) {

@@ -111,7 +111,9 @@ struct BackwardArgs {
     const float* rstd;
     void* grad_x;
     void* grad_branch;  // null where it equals grad_x
-    float* partials;    // [blocks][hidden], null without the weight's gradient
+    float* partials;    // [blocks][hidden] of a walk, or null
+    void* grad_weight;  // of a launch with slab blocks
+    int slabs;          // its first blocks
     int64_t updated_stride;
     int64_t rows;
     int hidden;
@@ -448,6 +450,17 @@ __device__ __forceinline__ void store_as(void* tensor, int dtype, int64_t first,
     }
 }
 
+// One value of a small tensor.
+__device__ __forceinline__ void store_one(void* tensor, int dtype, int64_t index, float value) {
+    if (dtype == RLN_DTYPE_F32) {
+        static_cast<float*>(tensor)[index] = value;
+    } else if (dtype == RLN_DTYPE_F16) {
+        static_cast<half_t*>(tensor)[index] = static_cast<half_t>(value);
+    } else {
+        static_cast<bf16_t*>(tensor)[index] = static_cast<bf16_t>(value);
+    }
+}
+
 // ----------------------------------------------------------------------------
 // 8-bit codes.
 
@@ -592,7 +605,7 @@ __device__ __forceinline__ Team team_of(int parts) {
 
 // ----------------------------------------------------------------------------
 // Forward: one row per team and turn. The grid covers the rows up to
-// kForwardMaxBlocks (a launch holds fewer than 2^32 threads); past that the
+// kMaxBlocks (a launch holds fewer than 2^32 threads); past that the
 // teams walk.
 
 template <typename X, typename B, int V, Mode kMode, Access kAccess>
@@ -786,14 +799,120 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
 }
 
 // ----------------------------------------------------------------------------
-// Backward: a block's teams walk the rows block by block; each lane keeps its
+// Backward, in two forms; neither uses atomics, both give the same bits on every
+// run.
+//
+// Walk: a block's teams walk the rows block by block; each lane keeps its
 // columns' share of the weight's gradient in registers, the block adds its
 // teams' shares through LDS and writes them to its row of the partials, which
-// reduce_kernel adds in a fixed order (no atomics: the same bits on every run).
+// reduce_kernel adds in a fixed order.
+//
+// Slabs, for small launches, whose rows stay in the caches: each team takes one
+// row, and the launch's first blocks sum the weight's gradient, each over all rows
+// of a slab of columns, from a second reading. One launch and no workspace.
 
-template <typename X, typename Y, int V, bool Checkpoint, Access kAccess>
+constexpr int kSlabLanes = 4;  // 64 bytes of the stream per row
+template <typename X>
+constexpr int kSlabColumns = kSlabLanes * kColumns<X>;
+
+template <typename X, typename Y, bool Checkpoint>
+__device__ __forceinline__ void sum_slab(const BackwardArgs& a) {
+    constexpr int N = kColumns<X>;
+    constexpr int kRows = 4;  // rows in flight per thread
+    __shared__ float totals[kMaxParts][kSlabColumns<X>];
+    const int groups = static_cast<int>(blockDim.x) / kSlabLanes;
+    const int place = threadIdx.x % kSlabLanes * N;
+    const int column = static_cast<int>(blockIdx.x) * kSlabColumns<X> + place;
+    float total[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        total[e] = 0.0f;
+    }
+    for (int64_t base = threadIdx.x / kSlabLanes; base < a.rows;
+         base += static_cast<int64_t>(groups) * kRows) {
+        Raw<Y, N> raw_y[kRows];
+        Raw<X, N> raw_u[kRows];
+        Raw<int8_t, N> raw_kept[kRows];
+        float scale[kRows];
+        float kept_step[kRows];
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            const int64_t row = base + static_cast<int64_t>(k) * groups;
+            const int hidden = row < a.rows ? a.hidden : 0;
+            raw_y[k] = load<Access::kLanes, Y, N, kCached>(
+                static_cast<const Y*>(a.grad_normalized) + row * a.hidden, column, hidden);
+            if constexpr (Checkpoint) {
+                raw_kept[k] = load<Access::kLanes, int8_t, N, kCached>(
+                    a.checkpoint + row * a.hidden, column, hidden);
+                kept_step[k] = column < hidden
+                    ? a.scale[row * a.groups + column / kCheckpointGroup] : 0.0f;
+            } else {
+                raw_u[k] = load<Access::kLanes, X, N, kCached>(
+                    static_cast<const X*>(a.updated) + row * a.updated_stride, column, hidden);
+            }
+            scale[k] = hidden > 0 ? a.rstd[row] : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            const int hidden = base + static_cast<int64_t>(k) * groups < a.rows ? a.hidden : 0;
+            float upstream[N];
+            float unit[N];
+            settle<Access::kLanes>(raw_y[k], column, hidden);
+            widen<Y, N>(raw_y[k], upstream);
+            if constexpr (Checkpoint) {
+                settle<Access::kLanes>(raw_kept[k], column, hidden);
+                widen<int8_t, N>(raw_kept[k], unit);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    unit[e] *= kept_step[k];
+                }
+            } else {
+                settle<Access::kLanes>(raw_u[k], column, hidden);
+                widen<X, N>(raw_u[k], unit);
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                total[e] += upstream[e] * (unit[e] * scale[k]);
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+#pragma unroll
+        for (int other = kSlabLanes; other < kWave; other *= 2) {
+            total[e] += __shfl_xor(total[e], other);
+        }
+    }
+    const int wave = threadIdx.x / kWave;
+    if (threadIdx.x % kWave < kSlabLanes) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            totals[wave][place + e] = total[e];
+        }
+    }
+    __syncthreads();
+    const int own = blockIdx.x * kSlabColumns<X> + static_cast<int>(threadIdx.x);
+    if (threadIdx.x < kSlabColumns<X> && own < a.hidden) {
+        float sum = 0.0f;
+        for (int other = 0; other < static_cast<int>(blockDim.x) / kWave; ++other) {
+            sum += totals[other][threadIdx.x];
+        }
+        store_one(a.grad_weight, a.weight_dtype, own, sum);
+    }
+}
+
+template <typename X, typename Y, int V, bool Checkpoint, Access kAccess, bool kSlabs>
 __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArgs a) {
     constexpr int N = kColumns<X>;
+    // What a slab block reads again stays cached.
+    constexpr int kPolicy = kSlabs ? kCached : kOnce;
+    const int slabs = kSlabs ? a.slabs : 0;
+    if constexpr (kSlabs) {
+        if (static_cast<int>(blockIdx.x) < slabs) {
+            sum_slab<X, Y, Checkpoint>(a);
+            return;
+        }
+    }
     extern __shared__ float shares[];  // [teams - 1][hidden], the weight's gradient
     __shared__ float sums[2][kMaxParts];
     const Team team = team_of(a.parts);
@@ -810,10 +929,10 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
             grad_weight[v][e] = 0.0f;
         }
     }
-    const int64_t step = static_cast<int64_t>(gridDim.x) * team.teams;
+    const int64_t step = (static_cast<int64_t>(gridDim.x) - slabs) * team.teams;
     int turn = 0;
     // Every team of the block makes the same number of turns (barriers inside).
-    for (int64_t base = static_cast<int64_t>(blockIdx.x) * team.teams; base < a.rows;
+    for (int64_t base = (static_cast<int64_t>(blockIdx.x) - slabs) * team.teams; base < a.rows;
          base += step) {
         const int64_t row = base + team.index;
         const bool live = row < a.rows;
@@ -826,14 +945,15 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
         Raw<X, N> raw_grad[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            raw_y[v] = load<kAccess, Y, N>(static_cast<const Y*>(a.grad_normalized) + first,
-                                           column[v], hidden);
+            raw_y[v] = load<kAccess, Y, N, kPolicy>(
+                static_cast<const Y*>(a.grad_normalized) + first, column[v], hidden);
             if constexpr (Checkpoint) {
-                raw_kept[v] = load<kAccess, int8_t, N>(a.checkpoint + first, column[v], hidden);
+                raw_kept[v] = load<kAccess, int8_t, N, kPolicy>(a.checkpoint + first, column[v],
+                                                               hidden);
                 kept_step[v] = column[v] < hidden
                     ? a.scale[row * a.groups + column[v] / kCheckpointGroup] : 0.0f;
             } else {
-                raw_u[v] = load<kAccess, X, N>(
+                raw_u[v] = load<kAccess, X, N, kPolicy>(
                     static_cast<const X*>(a.updated) + row * a.updated_stride, column[v], hidden);
             }
         }
@@ -877,7 +997,9 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
                 unit[v][e] *= rstd;
                 product[v][e] = upstream[e] * weight[v][e];
                 sum += product[v][e] * unit[v][e];
-                grad_weight[v][e] += upstream[e] * unit[v][e];
+                if constexpr (!kSlabs) {
+                    grad_weight[v][e] += upstream[e] * unit[v][e];
+                }
             }
         }
         sum = wave_sum(sum);
@@ -911,7 +1033,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
             }
         }
     }
-    if (a.partials == nullptr) {
+    if (kSlabs || a.partials == nullptr) {
         return;
     }
     // Teams 1, 2, ... leave their shares; team 0 adds them in that order.
@@ -968,6 +1090,11 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 //    each adds a row of partial sums ([16384, 4096] bf16: 90 us at 16 waves per CU,
 //    104 at 8, 104 at 32).
 
+//  * Slab blocks sum the weight's gradient of launches of up to 1024 rows and 2^21
+//    elements, whose time is launches more than bytes: [256, 384] fp32 3.5 against
+//    6.0 us for the walk and its reduction, [1024, 768] 7.1 against 9.5, [512, 4096]
+//    bf16 8.3 against 12.6. Past that their second reading costs more: [2048, 2048]
+//    bf16 15.3 against 14.1, [4096, 384] fp32 17.1 against 11.4.
 //  * Decode-sized forwards, at most a row for each CU, wait for one row's chain of
 //    steps: one slot up to 12 waves ([64, 5120] bf16 e4m3: 4.1 against 4.4 us,
 //    [256, 2048] fp32 3.5 against 3.8), longer rows as above ([8, 4096] fp32:
@@ -1025,17 +1152,24 @@ inline Shape forward_shape(int64_t rows, int64_t hidden, int x_dtype) {
     return shape_of(vectors, slots, 4);
 }
 
-constexpr int64_t kForwardMaxBlocks = 1 << 21;
+constexpr int64_t kMaxBlocks = 1 << 21;
 
 inline int64_t forward_blocks(int64_t rows, const Shape& shape) {
     const int64_t blocks = blocks_of(rows, shape);
-    return blocks < kForwardMaxBlocks ? blocks : kForwardMaxBlocks;
+    return blocks < kMaxBlocks ? blocks : kMaxBlocks;
 }
 
 inline Shape backward_shape(int64_t hidden, int x_dtype) {
     const int64_t vectors = wave_vectors(hidden, x_dtype);
     const int slots = vectors <= 8 ? 1 : vectors <= 2 * kMaxParts ? 2 : 4;
     return shape_of(vectors, slots, 8);
+}
+
+constexpr int64_t kSlabRows = 1024;
+constexpr int64_t kSlabElements = 1 << 21;
+
+inline bool backward_slabs(int64_t rows, int64_t hidden) {
+    return rows <= kSlabRows && rows * hidden <= kSlabElements;
 }
 
 inline int64_t backward_blocks(int64_t rows, const Shape& shape) {

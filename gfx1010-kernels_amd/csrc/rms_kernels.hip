@@ -57,11 +57,18 @@ int forward_branch(const ForwardArgs& a, const Shape& shape, int branch_dtype,
 #else
 template <typename X, typename Y, int V, bool Checkpoint>
 int backward_access(const BackwardArgs& a, const Shape& shape, hipStream_t stream) {
+    if (a.slabs > 0) {
+        const auto kernel = a.words
+            ? backward_kernel<X, Y, V, Checkpoint, Access::kWords, true>
+            : backward_kernel<X, Y, V, Checkpoint, Access::kElements, true>;
+        return launch(kernel, a, a.slabs + blocks_of(a.rows, shape), shape.threads, 0, stream,
+                      "rms backward_kernel");
+    }
     const int64_t blocks = backward_blocks(a.rows, shape);
     const size_t lds = a.partials == nullptr
         ? 0 : static_cast<size_t>(teams_of(shape) - 1) * a.hidden * sizeof(float);
-    const auto kernel = a.words ? backward_kernel<X, Y, V, Checkpoint, Access::kWords>
-                                : backward_kernel<X, Y, V, Checkpoint, Access::kElements>;
+    const auto kernel = a.words ? backward_kernel<X, Y, V, Checkpoint, Access::kWords, false>
+                                : backward_kernel<X, Y, V, Checkpoint, Access::kElements, false>;
     return launch(kernel, a, blocks, shape.threads, lds, stream, "rms backward_kernel");
 }
 

@@ -234,7 +234,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> backward_impl(
         } else {
             grad_weight = empty_device({hidden}, weight.scalar_type(), device);
             bytes = rln_rms_backward_workspace_bytes(rows, hidden, dtype_of(x_type));
-            workspace = empty_device({static_cast<int64_t>(bytes)}, at::kByte, device);
+            if (bytes > 0) {
+                workspace = empty_device({static_cast<int64_t>(bytes)}, at::kByte, device);
+            }
         }
     }
     if (rows == 0) {

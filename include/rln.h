@@ -322,8 +322,8 @@ int rln_rms_forward(
  * (no addition, or a branch of x's type, whose gradient is grad_x itself), and
  * so may grad_weight. workspace: device scratch of
  * rln_rms_backward_workspace_bytes(rows, hidden, x_dtype) bytes, aligned to 4
- * (unused, may be NULL, without grad_weight); nothing in it needs clearing, and
- * calls that overlap need one each.
+ * (unused, may be NULL, without grad_weight or where that size is 0); nothing in
+ * it needs clearing, and calls that overlap need one each.
  */
 int rln_rms_backward(
     const void* grad_updated,
@@ -348,7 +348,8 @@ int rln_rms_backward(
     void* stream);
 
 /* Workspace bytes rln_rms_backward needs for grad_weight: the per-block sums
- * of its fixed-order reduction (no counterpart in the reference). */
+ * of its fixed-order reduction (no counterpart in the reference); 0 for launches of at
+ * most 1024 rows and 2^21 elements, which sum it in blocks of their own. */
 size_t rln_rms_backward_workspace_bytes(
     int64_t rows,
     int64_t hidden,

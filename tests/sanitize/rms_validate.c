@@ -76,8 +76,9 @@ int main(void) {
     UNSUPPORTED(backward(FAKE, NULL, NULL, NULL, 0, 4, 16385), "hidden size");
     REFUSED(backward(NULL, NULL, NULL, NULL, 0, 4, 8), "either updated");
     REFUSED(backward(NULL, FAKE, NULL, NULL, 0, 4, 8), "either updated");
-    REFUSED(backward(FAKE, NULL, FAKE, NULL, 0, 4, 8), "workspace too small");
-    REFUSED(backward(FAKE, NULL, FAKE, FAKE, 31, 4, 8), "workspace too small");
+    REFUSED(backward(FAKE, NULL, FAKE, NULL, 0, 1 << 24, 8), "workspace too small");
+    REFUSED(backward(FAKE, NULL, FAKE, FAKE, 31, 1 << 24, 8), "workspace too small");
+    REFUSED(backward(FAKE, NULL, FAKE, FAKE, 31, huge / 64, 8), "workspace too small");
     REFUSED(backward(FAKE, NULL, FAKE, (char*)FAKE + 1, 4096, 4, 8), "aligned");
 
     REFUSED(dequantize(RLN_DTYPE_INT8, 0, FAKE, 0, 8), "empty");
@@ -94,7 +95,10 @@ int main(void) {
                 const size_t bytes = rln_rms_backward_workspace_bytes(rows, hidden, dtype);
                 const int served = rows > 0 && rln_rms_hidden_supported(hidden)
                     && dtype >= RLN_DTYPE_F32 && dtype <= RLN_DTYPE_BF16;
-                if (served ? bytes == 0 || bytes > 4 * 4096 * (size_t)hidden : bytes != 0) {
+                /* none for launches of at most 1024 rows and 2^21 elements */
+                const int wanted =
+                    served && (rows > 1024 || rows * hidden > (int64_t)1 << 21);
+                if (wanted ? bytes == 0 || bytes > 4 * 512 * (size_t)hidden : bytes != 0) {
                     fprintf(stderr, "workspace of %lld x %lld, dtype %d: %zu\n", (long long)rows,
                             (long long)hidden, dtype, bytes);
                     ++failures;

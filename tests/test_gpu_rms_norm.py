@@ -350,8 +350,9 @@ def test_backward_types(x_dtype, branch_dtype, weight_dtype, dtype, checkpoint):
                         shape)
 
 
-@pytest.mark.parametrize("rows", [1, 2, 5, 127, 1025, 4099, 20011])
-@pytest.mark.parametrize("hidden,x_dtype", [(65, F32), (384, F32), (1024, BF16), (2056, BF16)])
+@pytest.mark.parametrize("rows", [1, 2, 5, 127, 511, 512, 513, 1023, 1024, 1025, 4099, 20011])
+@pytest.mark.parametrize("hidden,x_dtype", [(3, BF16), (65, F32), (384, F32), (1024, BF16),
+                                            (2056, BF16), (4096, F16), (4097, BF16)])
 def test_backward_rows(rows, hidden, x_dtype):
     if rows * hidden > 1 << 23:
         rows = (1 << 23) // hidden | 1
