@@ -133,6 +133,7 @@ int forward_args(const void* x, int x_dtype, int64_t x_stride, const void* branc
 int launch(ForwardArgs& a, int x_dtype, int branch_dtype, Mode mode, void* stream) {
     const Shape shape = forward_shape(a.rows, a.hidden, x_dtype);
     a.parts = shape.parts;
+    a.row_lanes = shape.row_lanes;
     const int64_t hidden = a.hidden;
     a.words = whole_words(a.x, x_dtype, a.x_stride, hidden)
         && (a.branch == nullptr || whole_words(a.branch, branch_dtype, a.branch_stride, hidden))
@@ -415,6 +416,7 @@ int rln_rms_backward(
     a.rows = rows;
     a.hidden = static_cast<int>(hidden);
     a.parts = shape.parts;
+    a.row_lanes = shape.row_lanes;
     a.groups = static_cast<int>(groups_of(hidden, kCheckpointGroup));
     a.weight_dtype = weight_dtype;
     a.branch_dtype = branch_dtype;

@@ -20,7 +20,8 @@
 // from there. A row belongs to `parts` waves; vector j of the row (8 columns of
 // a 16-bit stream, 4 of a 32-bit one: 16 bytes of the stream per lane) sits in
 // slot v of lane l of part p with j = (v * parts + p) * 64 + l. `parts` is a
-// run-time value, so any row length gets a team without idle waves.
+// run-time value, so any row length gets a team without idle waves. Short rows, of
+// at most half a wave's vectors, take 8, 16 or 32 lanes each instead (Access::kLanes).
 //
 // A row is read and written in vectors, through one buffer descriptor per row and
 // tensor where its rows start and end on whole 32-bit words (Access::kWords; 32-bit
@@ -68,8 +69,8 @@ constexpr float kLeastMaximum = 0x1p-100f;
 template <typename X>
 constexpr int kColumns = 16 / static_cast<int>(sizeof(X));
 
-// How rows are accessed (see above); kLanes: as kElements, and each lane has a
-// row of its own, where the others ask for one row per wave.
+// How rows are accessed (see above); kLanes: as kElements, for waves whose lanes
+// hold several rows, where the others ask for one row per wave.
 enum class Access { kWords, kElements, kLanes };
 
 template <Access kAccess, typename T>
@@ -92,6 +93,7 @@ struct ForwardArgs {
     int64_t rows;
     int hidden;
     int parts;
+    int row_lanes;      // of Access::kLanes
     int words;          // Access::kWords serves every tensor
     int weight_dtype;
     int output_dtype;   // normalized's, or the codes'
@@ -118,6 +120,7 @@ struct BackwardArgs {
     int64_t rows;
     int hidden;
     int parts;
+    int row_lanes;
     int words;
     int groups;
     int weight_dtype;
@@ -563,6 +566,20 @@ __device__ __forceinline__ float wave_sum(float value) {
     return low + high;
 }
 
+// Sum over each aligned run of `lanes` lanes (8, 16 or 32).
+__device__ __forceinline__ float lanes_sum(float value, int lanes) {
+#define RMS_ADD(control) \
+    value += __builtin_bit_cast(float, RMS_DPP(__builtin_bit_cast(uint32_t, value), control))
+    RMS_ADD(kXor1);
+    RMS_ADD(kXor2);
+    RMS_ADD(kHalfMirror);
+    if (lanes > 8) {
+        RMS_ADD(kMirror);
+    }
+#undef RMS_ADD
+    return lanes > 16 ? value + __shfl_xor(value, 16) : value;
+}
+
 __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
     return a > b ? a : b;
 }
@@ -594,6 +611,25 @@ struct Team {
     int teams;
 };
 
+// A lane's place: its row among those its wave holds, and its lane of that row.
+// A wave holds one row (or a part of one), or 64 / row_lanes short ones (kLanes).
+struct Place {
+    int rows;
+    int row;
+    int lane;
+};
+
+template <Access kAccess>
+__device__ __forceinline__ Place place_of(int row_lanes) {
+    const int lane = threadIdx.x % kWave;
+    if constexpr (kAccess == Access::kLanes) {
+        const int row = lane / row_lanes;
+        return Place{kWave / row_lanes, row, lane - row * row_lanes};
+    } else {
+        return Place{1, 0, lane};
+    }
+}
+
 __device__ __forceinline__ Team team_of(int parts) {
     Team team;
     team.wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
@@ -615,13 +651,14 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
     __shared__ float sums[2][kMaxParts];
     __shared__ uint32_t maxima[2][kMaxParts];
     const Team team = team_of(a.parts);
-    const int lane = threadIdx.x % kWave;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * team.teams;
+    const Place place = place_of<kAccess>(a.row_lanes);
+    const int block_rows = team.teams * place.rows;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * block_rows;
     int turn = 0;
     // Every team of the block makes the same number of turns (a barrier inside).
-    for (int64_t base = static_cast<int64_t>(blockIdx.x) * team.teams; base < a.rows;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * block_rows; base < a.rows;
          base += step) {
-        const int64_t row = base + team.index;
+        const int64_t row = base + team.index * place.rows + place.row;
         const bool live = row < a.rows;  // the block's last teams may have no row
         const int hidden = live ? a.hidden : 0;
         const int64_t first = row * a.hidden;
@@ -632,7 +669,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
         float weight[V][N];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            column[v] = ((v * a.parts + team.part) * kWave + lane) * N;
+            column[v] = ((v * a.parts + team.part) * kWave + place.lane) * N;
             raw_x[v] = load<kAccess, X, N>(x, column[v], hidden);
         }
         if constexpr (kBranch) {
@@ -681,7 +718,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
                 sum += u[v][e] * u[v][e];
             }
         }
-        sum = wave_sum(sum);
+        sum = kAccess == Access::kLanes ? lanes_sum(sum, a.row_lanes) : wave_sum(sum);
         // The 8-bit steps' values: u itself for the checkpoint, u * weight for codes.
         uint32_t maximum[V];
         const bool whole_row = kMode == Mode::kQuantize && a.groups == 1;
@@ -709,13 +746,17 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
                 for (int v = 1; v < V; ++v) {
                     whole = larger(whole, maximum[v]);
                 }
-                whole = lanes_max(whole, kWave);
+                whole = lanes_max(whole, kAccess == Access::kLanes ? a.row_lanes : kWave);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     maximum[v] = whole;
                 }
             } else {
-                const int lanes = kMode == Mode::kCheckpoint ? kCheckpointGroup / N : (1 << a.group_shift) / N;
+                int lanes = kMode == Mode::kCheckpoint ? kCheckpointGroup / N
+                                                       : (1 << a.group_shift) / N;
+                if (kAccess == Access::kLanes && a.row_lanes < lanes) {
+                    lanes = a.row_lanes;  // the lanes past it hold another row
+                }
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     maximum[v] = lanes_max(maximum[v], lanes);
@@ -748,7 +789,8 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
             turn ^= 1;
         }
         const float rstd = 1.0f / __builtin_sqrtf(sum * a.inv_hidden + a.eps);
-        if (kMode != Mode::kQuantize && a.rstd != nullptr && live && team.part == 0 && lane == 0) {
+        if (kMode != Mode::kQuantize && a.rstd != nullptr && live && team.part == 0 &&
+            place.lane == 0) {
             a.rstd[row] = rstd;
         }
         if constexpr (kMode == Mode::kQuantize) {
@@ -916,25 +958,26 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
     extern __shared__ float shares[];  // [teams - 1][hidden], the weight's gradient
     __shared__ float sums[2][kMaxParts];
     const Team team = team_of(a.parts);
-    const int lane = threadIdx.x % kWave;
+    const Place place = place_of<kAccess>(a.row_lanes);
+    const int block_rows = team.teams * place.rows;
     int column[V];
     float weight[V][N];
     float grad_weight[V][N];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        column[v] = ((v * a.parts + team.part) * kWave + lane) * N;
+        column[v] = ((v * a.parts + team.part) * kWave + place.lane) * N;
         load_weight<kAccess, N>(a.weight, a.weight_dtype, column[v], a.hidden, weight[v]);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             grad_weight[v][e] = 0.0f;
         }
     }
-    const int64_t step = (static_cast<int64_t>(gridDim.x) - slabs) * team.teams;
+    const int64_t step = (static_cast<int64_t>(gridDim.x) - slabs) * block_rows;
     int turn = 0;
     // Every team of the block makes the same number of turns (barriers inside).
-    for (int64_t base = (static_cast<int64_t>(blockIdx.x) - slabs) * team.teams; base < a.rows;
+    for (int64_t base = (static_cast<int64_t>(blockIdx.x) - slabs) * block_rows; base < a.rows;
          base += step) {
-        const int64_t row = base + team.index;
+        const int64_t row = base + team.index * place.rows + place.row;
         const bool live = row < a.rows;
         const int hidden = live ? a.hidden : 0;
         const int64_t first = row * a.hidden;
@@ -1002,7 +1045,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
                 }
             }
         }
-        sum = wave_sum(sum);
+        sum = kAccess == Access::kLanes ? lanes_sum(sum, a.row_lanes) : wave_sum(sum);
         if (a.parts > 1) {
             // Two buffers: a team's next turn writes the other one while
             // slower waves still read this one.
@@ -1035,6 +1078,18 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
     }
     if (kSlabs || a.partials == nullptr) {
         return;
+    }
+    if constexpr (kAccess == Access::kLanes) {
+        // The wave's rows first; row 0's lanes stand for all of them.
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            for (int other = a.row_lanes; other < kWave; other *= 2) {
+                grad_weight[0][e] += __shfl_xor(grad_weight[0][e], other);
+            }
+        }
+        if (place.row > 0) {
+            column[0] = a.hidden;  // past the end: nothing to leave or to store
+        }
     }
     // Teams 1, 2, ... leave their shares; team 0 adds them in that order.
     if (team.index > 0) {
@@ -1080,6 +1135,9 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 //    against 5.9), and doubles them until a row fits 8 waves: in blocks of 16
 //    waves a CU idles while they wait for each other ([8192, 8192] fp32 with the
 //    checkpoint: 5.6 with four slots and 8 waves, 5.2 with two and 16).
+//  * Short rows share waves, 2, 4 or 8 in each ([262144, 128] bf16 forward 52 against
+//    83 us with a wave for each, with codes 44 against 110, backward 50 against 80;
+//    [524288, 64] 52 against 156, 71 with at least 16 lanes a row).
 //  * The backward holds the weight and its gradient's sums in registers besides
 //    and takes one slot up to 8 waves a row ([32768, 1024] fp32: 5.7 against 5.4
 //    with two). Longer 32-bit rows take two up to 16 waves ([8192, 8192]: 5.5
@@ -1089,7 +1147,6 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 //    52 us with two blocks of 5 waves per CU, 61 with three), and no more, since
 //    each adds a row of partial sums ([16384, 4096] bf16: 90 us at 16 waves per CU,
 //    104 at 8, 104 at 32).
-
 //  * Slab blocks sum the weight's gradient of launches of up to 1024 rows and 2^21
 //    elements, whose time is launches more than bytes: [256, 384] fp32 3.5 against
 //    6.0 us for the walk and its reduction, [1024, 768] 7.1 against 9.5, [512, 4096]
@@ -1106,6 +1163,7 @@ struct Shape {
     int slots;  // V
     int parts;
     int threads;
+    int row_lanes;  // below 64: several rows per wave
 };
 
 inline int columns_of(int dtype) {
@@ -1122,6 +1180,7 @@ inline int64_t wave_vectors(int64_t hidden, int x_dtype) {
 // `waves` waves (nearest; at least one team).
 inline Shape shape_of(int64_t vectors, int slots, int waves) {
     Shape shape;
+    shape.row_lanes = kWave;
     shape.slots = slots;
     shape.parts = static_cast<int>((vectors + slots - 1) / slots);
     const int teams = (waves + shape.parts / 2) / shape.parts;
@@ -1133,13 +1192,24 @@ inline int teams_of(const Shape& shape) {
     return shape.threads / (kWave * shape.parts);
 }
 
-// Blocks that give every row a team (no overflow for any row count).
+// Blocks that give every row its lanes (no overflow for any row count).
 inline int64_t blocks_of(int64_t rows, const Shape& shape) {
-    const int teams = teams_of(shape);
-    return rows / teams + (rows % teams != 0);
+    const int block_rows = teams_of(shape) * (kWave / shape.row_lanes);
+    return rows / block_rows + (rows % block_rows != 0);
+}
+
+// Rows of at most half a wave's columns share waves: 2, 4 or 8 in each.
+inline Shape short_shape(int64_t hidden, int x_dtype, int waves) {
+    const int columns = columns_of(x_dtype);
+    Shape shape = shape_of(1, 1, waves);
+    shape.row_lanes = hidden <= 8 * columns ? 8 : hidden <= 16 * columns ? 16 : 32;
+    return shape;
 }
 
 inline Shape forward_shape(int64_t rows, int64_t hidden, int x_dtype) {
+    if (hidden <= 32 * columns_of(x_dtype)) {
+        return short_shape(hidden, x_dtype, 4);
+    }
     const int64_t vectors = wave_vectors(hidden, x_dtype);
     if (rows <= kComputeUnits && vectors <= 12) {
         return shape_of(vectors, 1, 4);
@@ -1160,6 +1230,9 @@ inline int64_t forward_blocks(int64_t rows, const Shape& shape) {
 }
 
 inline Shape backward_shape(int64_t hidden, int x_dtype) {
+    if (hidden <= 32 * columns_of(x_dtype)) {
+        return short_shape(hidden, x_dtype, 8);
+    }
     const int64_t vectors = wave_vectors(hidden, x_dtype);
     const int slots = vectors <= 8 ? 1 : vectors <= 2 * kMaxParts ? 2 : 4;
     return shape_of(vectors, slots, 8);

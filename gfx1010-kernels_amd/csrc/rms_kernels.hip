@@ -19,8 +19,13 @@ int launch(Kernel kernel, const Args& a, int64_t blocks, int threads, size_t lds
 template <typename X, typename B, int V, Mode kMode>
 int forward_access(const ForwardArgs& a, const Shape& shape, hipStream_t stream) {
     const int64_t blocks = forward_blocks(a.rows, shape);
-    const auto kernel = a.words ? forward_kernel<X, B, V, kMode, Access::kWords>
-                                : forward_kernel<X, B, V, kMode, Access::kElements>;
+    auto kernel = a.words ? forward_kernel<X, B, V, kMode, Access::kWords>
+                          : forward_kernel<X, B, V, kMode, Access::kElements>;
+    if constexpr (V == 1) {
+        if (shape.row_lanes < kWave) {
+            kernel = forward_kernel<X, B, 1, kMode, Access::kLanes>;
+        }
+    }
     return launch(kernel, a, blocks, shape.threads, 0, stream, "rms forward_kernel");
 }
 
@@ -58,17 +63,26 @@ int forward_branch(const ForwardArgs& a, const Shape& shape, int branch_dtype,
 template <typename X, typename Y, int V, bool Checkpoint>
 int backward_access(const BackwardArgs& a, const Shape& shape, hipStream_t stream) {
     if (a.slabs > 0) {
-        const auto kernel = a.words
-            ? backward_kernel<X, Y, V, Checkpoint, Access::kWords, true>
-            : backward_kernel<X, Y, V, Checkpoint, Access::kElements, true>;
+        auto kernel = a.words ? backward_kernel<X, Y, V, Checkpoint, Access::kWords, true>
+                              : backward_kernel<X, Y, V, Checkpoint, Access::kElements, true>;
+        if constexpr (V == 1) {
+            if (shape.row_lanes < kWave) {
+                kernel = backward_kernel<X, Y, 1, Checkpoint, Access::kLanes, true>;
+            }
+        }
         return launch(kernel, a, a.slabs + blocks_of(a.rows, shape), shape.threads, 0, stream,
                       "rms backward_kernel");
     }
     const int64_t blocks = backward_blocks(a.rows, shape);
     const size_t lds = a.partials == nullptr
         ? 0 : static_cast<size_t>(teams_of(shape) - 1) * a.hidden * sizeof(float);
-    const auto kernel = a.words ? backward_kernel<X, Y, V, Checkpoint, Access::kWords, false>
-                                : backward_kernel<X, Y, V, Checkpoint, Access::kElements, false>;
+    auto kernel = a.words ? backward_kernel<X, Y, V, Checkpoint, Access::kWords, false>
+                          : backward_kernel<X, Y, V, Checkpoint, Access::kElements, false>;
+    if constexpr (V == 1) {
+        if (shape.row_lanes < kWave) {
+            kernel = backward_kernel<X, Y, 1, Checkpoint, Access::kLanes, false>;
+        }
+    }
     return launch(kernel, a, blocks, shape.threads, lds, stream, "rms backward_kernel");
 }
 

@@ -779,9 +779,18 @@ def test_rows_past_two_to_the_31_elements():
 
 
 def test_more_rows_than_one_grid():
-    """A launch has at most 2^21 blocks; teams walk over the rows past that, and
-    so do the widening's."""
-    rows, hidden = (1 << 23) + 5, 4
+    """A launch has at most 2^21 blocks; teams walk over the rows past that (of 32
+    short rows or 4 longer ones per block), and so do the widening's."""
+    rows, hidden = (1 << 23) + 3, 258
+    row, branch, scale = make((1, hidden), BF16, BF16, BF16, 15)
+    x = torch.zeros(rows, hidden, device="cuda", dtype=BF16)
+    x[-1] = row[0]
+    outputs = residual_rms_norm(x, branch.cuda().expand(rows, hidden), scale.cuda(), EPS,
+                                implementation="gfx950")
+    check_forward([t[-1:] for t in outputs], row, branch, scale, BF16, "last row")
+    check_forward([t[:1] for t in outputs], torch.zeros_like(row), branch, scale, BF16, "first")
+    del x, outputs
+    rows, hidden = (1 << 26) + 5, 4
     generator = torch.Generator(device="cuda").manual_seed(3)
     x = torch.randn(rows, hidden, device="cuda", generator=generator)
     weight = torch.randn(hidden, device="cuda", generator=generator)
@@ -799,10 +808,10 @@ def test_more_rows_than_one_grid():
     ones = torch.ones_like(x)
     grads = torch.autograd.grad(residual_rms_norm(leaf, None, scale_leaf, EPS)[1],
                                 [leaf, scale_leaf], ones)
-    # 4096 teams of rows/4096 = 2049 rows each, then 4 teams and 512 blocks.
+    # 32768 places of rows/32768 = 2049 rows each, then 8 rows, 8 teams and 512 blocks.
     g, gw, size, terms = reference.gradients(x, x, weight, EPS, None, ones)
     assert ((grads[0].double() - g).abs() <= 128 * reference.U * size + reference.U * g.abs()).all()
-    assert ((grads[1].double() - gw).abs() <= (32 + 2049 + 516) * reference.U * terms).all()
+    assert ((grads[1].double() - gw).abs() <= (32 + 2049 + 528) * reference.U * terms).all()
     del grads, g, size, ones
     rows = (1 << 29) + 1000
     codes = torch.randint(-127, 128, (rows, 1), device="cuda", dtype=torch.int8)
