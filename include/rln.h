@@ -320,7 +320,8 @@ int rln_rms_forward(
  * grad_updated (x's type) may be NULL, meaning zero. Gradients are dense;
  * updated is rows `updated_stride` elements apart. grad_branch may be NULL
  * (no addition, or a branch of x's type, whose gradient is grad_x itself), and
- * so may grad_weight. workspace: device scratch of
+ * so may grad_weight. No output may overlap an input (other blocks still read them
+ * for grad_weight while grad_x is written). workspace: device scratch of
  * rln_rms_backward_workspace_bytes(rows, hidden, x_dtype) bytes, aligned to 4
  * (unused, may be NULL, without grad_weight or where that size is 0); nothing in
  * it needs clearing, and calls that overlap need one each.
