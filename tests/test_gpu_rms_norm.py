@@ -288,6 +288,42 @@ def test_gradients_of_rows_that_are_not_finite(checkpoint):
     assert grad_weight[8].isnan()
 
 
+@pytest.mark.parametrize("rows", [7, 1030])
+@pytest.mark.parametrize("hidden", [20, 33, 64, 90, 128, 200, 256])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_short_rows_are_independent(rows, hidden, dtype):
+    """Rows that share a wave: a row's bits are those it has among others, and a
+    NaN in one stays there."""
+    x, branch, weight = (t.cuda() for t in make((rows, hidden), dtype, dtype, dtype, hidden))
+    upstream = [torch.randn(rows, hidden, device="cuda").to(dtype) for _ in range(2)]
+
+    def run(order, x):
+        leaves = [x[order].requires_grad_(), branch[order].requires_grad_()]
+        results = []
+        for checkpoint in (None, torch.int8):
+            outputs = residual_rms_norm(*leaves, weight, EPS, implementation="gfx950",
+                                        checkpoint_dtype=checkpoint)
+            results += [*outputs, *torch.autograd.grad(outputs, leaves,
+                                                       [t[order] for t in upstream])]
+        for group in (None, 32, 128):
+            codes, scale = residual_rms_norm_quantized(
+                x[order], branch[order], weight, EPS, dtype=torch.int8, group_size=group,
+                implementation="gfx950")[1:]
+            results += [codes, scale, dequantize(codes, scale, group_size=group, dtype=F32)]
+        return [t.detach() for t in results]
+
+    straight = torch.arange(rows, device="cuda")
+    expected = run(straight, x)
+    order = torch.randperm(rows, device="cuda")
+    for got, want in zip(run(order, x), expected):
+        assert reference.same_bits(got, want[order])
+    spoiled = x.clone()
+    spoiled[2::5, hidden // 2] = float("nan")
+    rest = straight[straight % 5 != 2]
+    for got, want in zip(run(straight, spoiled), expected):
+        assert reference.same_bits(got[rest], want[rest])
+
+
 def test_extreme_magnitudes():
     """Rows whose squares overflow or vanish in fp32 go as the formula sends
     them; groups far under 2^-100 have zero codes."""
