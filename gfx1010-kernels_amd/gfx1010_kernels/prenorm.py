@@ -53,13 +53,21 @@ def _check_norm(norm: nn.Module, hidden: int) -> None:
                          + (" and bias" if kind == "LayerNorm" else ""))
 
 
+def _rms_eps(norm: nn.RMSNorm, dtype: torch.dtype) -> float:
+    """The module's eps. Its default, None, is the epsilon of the type that PyTorch
+    computes the norm of a ``dtype`` stream in: fp32's for 16-bit streams as well."""
+    if norm.eps is not None:
+        return norm.eps
+    return torch.finfo(torch.promote_types(dtype, torch.float32)).eps
+
+
 def _rms_norm(x, branch, norm: nn.RMSNorm, dropout_p, training, implementation, normalized_dtype,
               checkpoint_dtype):
     if branch is not None and training and dropout_p != 0.0:
         branch = F.dropout(branch, dropout_p, True)
-    eps = torch.finfo(x.dtype).eps if norm.eps is None else norm.eps
-    return residual_rms_norm(x, branch, norm.weight, eps, implementation=implementation,
-                             normalized_dtype=normalized_dtype, checkpoint_dtype=checkpoint_dtype)
+    return residual_rms_norm(x, branch, norm.weight, _rms_eps(norm, x.dtype),
+                             implementation=implementation, normalized_dtype=normalized_dtype,
+                             checkpoint_dtype=checkpoint_dtype)
 
 
 def _refuse_checkpoint(checkpoint_dtype) -> None:

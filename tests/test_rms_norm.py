@@ -504,3 +504,66 @@ def test_no_warning_on_the_torch_path():
     with warnings.catch_warnings():
         warnings.simplefilter("error")
         residual_rms_norm(x, branch, weight, implementation="torch")
+
+
+def check_default_eps(device, implementation, dtype, scale):
+    """A module without an eps: fp32's, which PyTorch adds to the mean of a 16-bit
+    stream too. Against the definition in 64 bits, and against the module: that may
+    round once more (before the weight), so both are within two steps of another."""
+    torch.manual_seed(4)
+    norm = nn.RMSNorm(96).to(device, dtype)
+    with torch.no_grad():
+        norm.weight.copy_(1.0 + 0.1 * torch.randn(96))
+    x, branch = ((scale * torch.randn(3, 7, 96)).to(dtype) for _ in range(2))
+    with torch.no_grad():
+        updated, normalized = residual_norm(x.to(device), branch.to(device), norm,
+                                            implementation=implementation)
+        module = norm(updated)
+    assert reference.same_bits(updated, reference.update(x, branch))
+    value = reference.normalized(updated.cpu(), norm.weight.detach().cpu(), 2.0 ** -23)
+    reference.assert_within(normalized, value, reference.normalized_bound(value, dtype),
+                            (dtype, scale))
+    step = torch.finfo(dtype).eps
+    torch.testing.assert_close(normalized, module, rtol=2 * step + 64 * reference.U,
+                               atol=2 * reference.SUBNORMAL[dtype])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scale", [1.0, 0.1, 0.02, 1e-4])
+def test_default_eps_is_the_modules(dtype, scale):
+    check_default_eps("cpu", "torch", dtype, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scale", [1.0, 0.1, 0.02, 1e-4])
+def test_default_eps_is_the_modules_on_the_gpu(dtype, scale):
+    check_default_eps("cuda", "gfx950", dtype, scale)
+
+
+def test_default_eps_of_an_fp64_stream():
+    norm = nn.RMSNorm(32).double()
+    x = 1e-8 * torch.randn(4, 32, dtype=torch.float64)
+    normalized = residual_norm(x, None, norm, implementation="torch")[1]
+    torch.testing.assert_close(normalized, norm(x), rtol=1e-12, atol=0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prenorm_stack_in_16_bits_is_the_unfused_model(dtype):
+    """Modules without an eps, a small stream. The unfused model rounds at the same
+    places, but for one rounding more that its 7 norms may make (half a step each);
+    taken as a whole step each through sublayers of gain about one."""
+    blocks, final = rms_stack()
+    for module in [*blocks.modules(), final]:
+        if isinstance(module, nn.RMSNorm):
+            module.eps = None
+        elif isinstance(module, nn.Linear):
+            nn.init.zeros_(module.bias)
+            module.weight.data.mul_(0.02)
+    blocks, final = blocks.to(dtype), final.to(dtype)
+    x = (0.02 * torch.randn(3, 5, 48)).to(dtype)
+    with torch.no_grad():
+        for fused, plain in zip(prenorm_forward(x, blocks, final, implementation="torch"),
+                                unfused(x, blocks, final)):
+            assert (fused - plain).double().norm() <= (
+                7 * torch.finfo(dtype).eps * plain.double().norm())
