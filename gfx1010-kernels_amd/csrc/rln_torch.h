@@ -29,6 +29,12 @@ inline int dtype_of(at::ScalarType type) {
     return RLN_DTYPE_F32;
 }
 
+// Whether a forward-mode derivative comes with `tensor` (the one level that
+// torch.autograd.forward_ad has). The kernels read addresses and know nothing of it.
+inline bool has_tangent(const at::Tensor& tensor) {
+    return tensor.defined() && tensor._fw_grad(/*level=*/0).defined();
+}
+
 // Whether something on this thread looks on at, or takes over, every operator:
 // a TorchDispatchMode (FakeTensorMode among them), a functorch transform, a
 // trace. Its dispatch key is then in the thread's included set.

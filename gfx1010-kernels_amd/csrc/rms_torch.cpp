@@ -24,6 +24,8 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <functional>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <optional>
@@ -69,9 +71,19 @@ at::Tensor as_rows(const at::Tensor& tensor, int64_t* stride) {
     return found ? tensor : tensor.contiguous();
 }
 
+// Raises where a forward-mode derivative would be dropped: these operators have
+// a backward, and no forward derivative.
+void refuse_tangents(std::initializer_list<std::reference_wrapper<const at::Tensor>> tensors) {
+    for (const at::Tensor& tensor : tensors) {
+        TORCH_CHECK(!has_tangent(tensor),
+                    "residual RMSNorm has no native forward-mode derivative");
+    }
+}
+
 void check_inputs(const at::Tensor& x, const at::Tensor& branch, const at::Tensor& weight,
                   double eps) {
     TORCH_CHECK(x.is_cuda(), "x must be a HIP tensor");
+    refuse_tangents({x, branch, weight});
     TORCH_CHECK((!branch.defined() || branch.is_cuda()) && weight.is_cuda(),
                 "branch and weight must be HIP tensors");
     TORCH_CHECK(
@@ -184,6 +196,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> backward_impl(
     bool checkpoint,
     bool weight_gradient) {
     TORCH_CHECK(grad_normalized_in.is_cuda(), "grad_normalized must be a HIP tensor");
+    refuse_tangents({grad_updated_in, grad_normalized_in, updated, weight});
     const auto device = grad_normalized_in.device();
     TORCH_CHECK(
         (!grad_updated_in.defined() || grad_updated_in.device() == device)
@@ -409,6 +422,9 @@ bool rms_inputs_supported(const at::Tensor& x, const at::Tensor& branch,
             || !supported_dtype(branch.scalar_type()))) {
         return false;
     }
+    if (has_tangent(x) || has_tangent(branch) || has_tangent(weight)) {
+        return false;
+    }
     const int64_t hidden = x.size(-1);
     return rln_rms_hidden_supported(hidden) && weight.sizes() == at::IntArrayRef({hidden})
         && eps >= 0.0;
@@ -535,6 +551,7 @@ residual_rms_norm_quantized_if_supported(
 at::Tensor dequantize(const at::Tensor& quantized, const at::Tensor& scale, int64_t group,
                       at::ScalarType dtype) {
     TORCH_CHECK(quantized.is_cuda(), "quantized must be a HIP tensor");
+    refuse_tangents({quantized, scale});
     TORCH_CHECK(scale.device() == quantized.device(),
                 "all tensors must be on the same HIP device");
     TORCH_CHECK(code_type(quantized.scalar_type()), "quantized must use int8 or float8_e4m3fn");
@@ -566,7 +583,8 @@ std::optional<at::Tensor> dequantize_if_supported(const at::Tensor& quantized,
         || !code_type(quantized.scalar_type()) || scale.scalar_type() != at::kFloat
         || quantized.size(-1) < 1
         || scale.sizes() != at::IntArrayRef(scale_sizes(quantized.sizes(), group))
-        || (at::GradMode::is_enabled() && scale.requires_grad())) {
+        || (at::GradMode::is_enabled() && scale.requires_grad())
+        || has_tangent(quantized) || has_tangent(scale)) {
         return std::nullopt;
     }
     return dequantize(quantized, scale, group, dtype);

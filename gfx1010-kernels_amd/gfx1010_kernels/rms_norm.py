@@ -27,6 +27,7 @@ from __future__ import annotations
 import warnings
 
 import torch
+from torch.autograd import forward_ad
 
 from ._normalization_native import TARGET_ARCHITECTURE, _extension
 from ._ops import dequantize_op, residual_rms_norm_op, residual_rms_norm_quantized_op
@@ -41,6 +42,7 @@ CHECKPOINT_GROUP = 128
 
 _STRICT_NATIVE = frozenset({TARGET_ARCHITECTURE, "gfx1010"})
 _UNAVAILABLE = f"{TARGET_ARCHITECTURE} native residual RMSNorm is unavailable"
+_NO_TANGENTS = "the kernels have no forward-mode derivative"
 _LARGEST_CODE = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
 _LEAST_MAXIMUM = 2.0 ** -100
 # Device indices whose backend status is known to be available.
@@ -137,6 +139,13 @@ def _torch_dequantize(quantized, scale, group_size, dtype):
 
 # Checks and dispatch.
 
+def _has_tangent(*tensors):
+    """Whether a forward-mode derivative (torch.autograd.forward_ad) comes with one
+    of the tensors, which the kernels would drop."""
+    return any(tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None
+               for tensor in tensors)
+
+
 def _input_reason(x, branch, weight, eps):
     """Why the native kernels cannot serve these inputs, or None if they can."""
     tensors = [tensor for tensor in (x, branch, weight) if tensor is not None]
@@ -154,6 +163,8 @@ def _input_reason(x, branch, weight, eps):
         return "x, branch and weight must use float16, bfloat16 or float32"
     if not eps >= 0.0:
         return "eps must not be negative"
+    if _has_tangent(*tensors):
+        return _NO_TANGENTS
     return None
 
 
@@ -214,7 +225,9 @@ def residual_rms_norm(
     fp32, fp16 or bf16; tensors whose rows are evenly spaced are read in place,
     others are copied first.
 
-    Supports first-order autograd, HIP graph capture and ``torch.compile``. The
+    Supports first-order autograd, HIP graph capture and ``torch.compile``; inputs
+    with a forward-mode tangent take the PyTorch path, which carries it (the native
+    modes raise). The
     weight's gradient is summed in a fixed order (bitwise reproducible with and
     without ``torch.use_deterministic_algorithms``). The gradients of ``x`` and
     of a branch of the same type are one tensor, as those of ``x + branch`` are.
@@ -234,7 +247,10 @@ def residual_rms_norm(
     if implementation == "torch":
         return _torch_residual_rms_norm(*args)
     if torch.compiler.is_compiling():
-        if implementation in _STRICT_NATIVE or _input_reason(x, branch, weight, eps) is None:
+        reason = _input_reason(x, branch, weight, eps)
+        if implementation in _STRICT_NATIVE and reason == _NO_TANGENTS:
+            raise RuntimeError(f"{_UNAVAILABLE}: {reason}")
+        if implementation in _STRICT_NATIVE or reason is None:
             return residual_rms_norm_op(*args)
         return _torch_residual_rms_norm(*args)
     # Inputs the kernels serve, on a device known to be ready: one C++ check and
@@ -285,7 +301,8 @@ def residual_rms_norm_quantized(
     infinity or a NaN has NaN for its scale.
 
     For serving: it records no gradient, and raises where one would be lost
-    (grad mode on and an input that requires grad).
+    (grad mode on and an input that requires grad, or an input with a
+    forward-mode tangent).
     """
     if (implementation == "auto" and x.is_cuda and dtype in QUANTIZED_DTYPES
             and group_size in GROUP_SIZES and x.get_device() in _READY_DEVICES
@@ -302,6 +319,9 @@ def residual_rms_norm_quantized(
             tensor is not None and tensor.requires_grad for tensor in (x, branch, weight)):
         raise RuntimeError("residual_rms_norm_quantized records no gradient: call it under "
                            "torch.no_grad(), or use residual_rms_norm")
+    if _has_tangent(x, branch, weight):
+        raise RuntimeError("residual_rms_norm_quantized has no forward-mode derivative: call it "
+                           "on tensors without a tangent, or use residual_rms_norm")
     args = (x, branch, weight, eps, dtype, group_size)
     if implementation == "torch":
         return _torch_quantized(*args)
@@ -352,6 +372,9 @@ def dequantize(quantized, scale, *, group_size=None, dtype=torch.bfloat16,
                          "for each group of columns")
     if torch.is_grad_enabled() and scale.requires_grad:
         raise RuntimeError("dequantize records no gradient: call it under torch.no_grad()")
+    if _has_tangent(quantized, scale):
+        raise RuntimeError("dequantize has no forward-mode derivative: call it on tensors without "
+                           "a tangent")
     args = (quantized, scale, group_size, dtype)
     if implementation == "torch":
         return _torch_dequantize(*args)
