@@ -56,6 +56,7 @@ void check_forward_inputs(
     double dropout_p,
     double eps,
     int64_t threads) {
+    refuse_tangents("residual LayerNorm", {x, branch, weight, bias});
     TORCH_CHECK(x.is_cuda(), "x must be a HIP tensor");
     TORCH_CHECK(
         branch.is_cuda() && weight.is_cuda() && bias.is_cuda(),
@@ -105,6 +106,10 @@ void check_backward_inputs(
     int64_t block_rows,
     int64_t parameter_threads,
     int64_t parameter_groups) {
+    const at::Tensor absent;
+    refuse_tangents("residual LayerNorm",
+                    {grad_updated ? *grad_updated : absent,
+                     grad_normalized ? *grad_normalized : absent, updated, weight});
     TORCH_CHECK(updated.is_cuda(), "updated must be a HIP tensor");
     const auto device = updated.device();
     const bool same_device = (!grad_updated || grad_updated->device() == device)
@@ -622,6 +627,9 @@ bool fused_inputs_supported(const at::Tensor& x, const at::Tensor& branch,
     }
     if (!(x.is_contiguous() && branch.is_contiguous() && weight.is_contiguous()
           && bias.is_contiguous())) {
+        return false;
+    }
+    if (has_tangent(x) || has_tangent(branch) || has_tangent(weight) || has_tangent(bias)) {
         return false;
     }
     // The Python comparisons exactly (`not 0 <= p < 1`, `eps <= 0`), NaN

@@ -7,6 +7,9 @@
 
 #include <ATen/hip/EmptyTensor.h>
 
+#include <functional>
+#include <initializer_list>
+
 #include "rln.h"
 
 namespace rln_glue {
@@ -33,6 +36,16 @@ inline int dtype_of(at::ScalarType type) {
 // torch.autograd.forward_ad has). The kernels read addresses and know nothing of it.
 inline bool has_tangent(const at::Tensor& tensor) {
     return tensor.defined() && tensor._fw_grad(/*level=*/0).defined();
+}
+
+// Raises where a forward-mode derivative would be dropped: the operators have a
+// backward, and no forward derivative.
+inline void refuse_tangents(
+    const char* what,
+    std::initializer_list<std::reference_wrapper<const at::Tensor>> tensors) {
+    for (const at::Tensor& tensor : tensors) {
+        TORCH_CHECK(!has_tangent(tensor), what, " has no native forward-mode derivative");
+    }
 }
 
 // Whether something on this thread looks on at, or takes over, every operator:

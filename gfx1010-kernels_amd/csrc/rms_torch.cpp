@@ -24,8 +24,6 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
-#include <functional>
-#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <optional>
@@ -71,19 +69,10 @@ at::Tensor as_rows(const at::Tensor& tensor, int64_t* stride) {
     return found ? tensor : tensor.contiguous();
 }
 
-// Raises where a forward-mode derivative would be dropped: these operators have
-// a backward, and no forward derivative.
-void refuse_tangents(std::initializer_list<std::reference_wrapper<const at::Tensor>> tensors) {
-    for (const at::Tensor& tensor : tensors) {
-        TORCH_CHECK(!has_tangent(tensor),
-                    "residual RMSNorm has no native forward-mode derivative");
-    }
-}
-
 void check_inputs(const at::Tensor& x, const at::Tensor& branch, const at::Tensor& weight,
                   double eps) {
     TORCH_CHECK(x.is_cuda(), "x must be a HIP tensor");
-    refuse_tangents({x, branch, weight});
+    refuse_tangents("residual RMSNorm", {x, branch, weight});
     TORCH_CHECK((!branch.defined() || branch.is_cuda()) && weight.is_cuda(),
                 "branch and weight must be HIP tensors");
     TORCH_CHECK(
@@ -196,7 +185,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> backward_impl(
     bool checkpoint,
     bool weight_gradient) {
     TORCH_CHECK(grad_normalized_in.is_cuda(), "grad_normalized must be a HIP tensor");
-    refuse_tangents({grad_updated_in, grad_normalized_in, updated, weight});
+    refuse_tangents("residual RMSNorm", {grad_updated_in, grad_normalized_in, updated, weight});
     const auto device = grad_normalized_in.device();
     TORCH_CHECK(
         (!grad_updated_in.defined() || grad_updated_in.device() == device)
@@ -551,7 +540,7 @@ residual_rms_norm_quantized_if_supported(
 at::Tensor dequantize(const at::Tensor& quantized, const at::Tensor& scale, int64_t group,
                       at::ScalarType dtype) {
     TORCH_CHECK(quantized.is_cuda(), "quantized must be a HIP tensor");
-    refuse_tangents({quantized, scale});
+    refuse_tangents("residual RMSNorm", {quantized, scale});
     TORCH_CHECK(scale.device() == quantized.device(),
                 "all tensors must be on the same HIP device");
     TORCH_CHECK(code_type(quantized.scalar_type()), "quantized must use int8 or float8_e4m3fn");

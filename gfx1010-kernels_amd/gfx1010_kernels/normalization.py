@@ -33,6 +33,7 @@ from functools import lru_cache
 import warnings
 
 import torch
+from torch.autograd import forward_ad
 from torch.nn import functional as F
 
 from ._normalization_native import (
@@ -52,6 +53,7 @@ MAX_HIDDEN_SIZE = MAX_NATIVE_HIDDEN_SIZE
 IMPLEMENTATIONS = ("auto", TARGET_ARCHITECTURE, "gfx1010", "triton", "torch")
 BRANCH_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 NORMALIZED_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+NO_TANGENTS = "the kernels have no forward-mode derivative"
 _STRICT_NATIVE = frozenset({TARGET_ARCHITECTURE, "gfx1010"})
 _NATIVE_SIZES = frozenset(NATIVE_HIDDEN_SIZES)
 _UNAVAILABLE = f"{TARGET_ARCHITECTURE} native residual LayerNorm is unavailable"
@@ -129,6 +131,13 @@ def residual_layer_norm_status(device=None):
     return _native_status(device_index)
 
 
+def has_tangent(*tensors):
+    """Whether a forward-mode derivative (torch.autograd.forward_ad) comes with one
+    of the tensors (None for one not given), which the kernels would drop."""
+    return any(tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None
+               for tensor in tensors)
+
+
 def _input_reason(x, branch, weight, bias, dropout_p, eps):
     """Why the fused path cannot serve these inputs, or None if it can."""
     if not x.is_cuda:
@@ -160,6 +169,8 @@ def _input_reason(x, branch, weight, bias, dropout_p, eps):
         return "eps must be positive"
     if x.numel() == 0:
         return "empty tensors use the PyTorch fallback"
+    if has_tangent(x, branch, weight, bias):
+        return NO_TANGENTS
     return None
 
 
@@ -220,6 +231,8 @@ def _traced(x, branch, weight, bias, dropout_p, eps, training, normalized_dtype,
             raise RuntimeError(
                 f"{_UNAVAILABLE}: native hidden size must be one of {NATIVE_HIDDEN_SIZES_TEXT}"
             )
+        if has_tangent(x, branch, weight, bias):
+            raise RuntimeError(f"{_UNAVAILABLE}: {NO_TANGENTS}")
         return residual_layer_norm_op(*args)
     if implementation == "triton":
         raise RuntimeError(
@@ -250,7 +263,8 @@ def residual_layer_norm(
     is ``torch.float16`` / ``torch.bfloat16``, rounded to that type for a
     half-precision consumer (the reference always returns fp32). ``branch``
     may be fp32, fp16 or bf16. Supports first-order autograd, HIP graph
-    capture and ``torch.compile``.
+    capture and ``torch.compile``; inputs with a forward-mode tangent take the
+    PyTorch path, which carries it (the native modes raise).
     """
     if implementation not in IMPLEMENTATIONS:
         raise ValueError(

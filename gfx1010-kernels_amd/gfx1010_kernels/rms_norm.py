@@ -27,11 +27,15 @@ from __future__ import annotations
 import warnings
 
 import torch
-from torch.autograd import forward_ad
 
 from ._normalization_native import TARGET_ARCHITECTURE, _extension
 from ._ops import dequantize_op, residual_rms_norm_op, residual_rms_norm_quantized_op
-from .normalization import IMPLEMENTATIONS, residual_layer_norm_status
+from .normalization import (
+    IMPLEMENTATIONS,
+    NO_TANGENTS,
+    has_tangent,
+    residual_layer_norm_status,
+)
 
 MAX_RMS_HIDDEN_SIZE = 16384
 STREAM_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
@@ -42,7 +46,6 @@ CHECKPOINT_GROUP = 128
 
 _STRICT_NATIVE = frozenset({TARGET_ARCHITECTURE, "gfx1010"})
 _UNAVAILABLE = f"{TARGET_ARCHITECTURE} native residual RMSNorm is unavailable"
-_NO_TANGENTS = "the kernels have no forward-mode derivative"
 _LARGEST_CODE = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
 _LEAST_MAXIMUM = 2.0 ** -100
 # Device indices whose backend status is known to be available.
@@ -139,13 +142,6 @@ def _torch_dequantize(quantized, scale, group_size, dtype):
 
 # Checks and dispatch.
 
-def _has_tangent(*tensors):
-    """Whether a forward-mode derivative (torch.autograd.forward_ad) comes with one
-    of the tensors, which the kernels would drop."""
-    return any(tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None
-               for tensor in tensors)
-
-
 def _input_reason(x, branch, weight, eps):
     """Why the native kernels cannot serve these inputs, or None if they can."""
     tensors = [tensor for tensor in (x, branch, weight) if tensor is not None]
@@ -163,8 +159,8 @@ def _input_reason(x, branch, weight, eps):
         return "x, branch and weight must use float16, bfloat16 or float32"
     if not eps >= 0.0:
         return "eps must not be negative"
-    if _has_tangent(*tensors):
-        return _NO_TANGENTS
+    if has_tangent(*tensors):
+        return NO_TANGENTS
     return None
 
 
@@ -248,7 +244,7 @@ def residual_rms_norm(
         return _torch_residual_rms_norm(*args)
     if torch.compiler.is_compiling():
         reason = _input_reason(x, branch, weight, eps)
-        if implementation in _STRICT_NATIVE and reason == _NO_TANGENTS:
+        if implementation in _STRICT_NATIVE and reason == NO_TANGENTS:
             raise RuntimeError(f"{_UNAVAILABLE}: {reason}")
         if implementation in _STRICT_NATIVE or reason is None:
             return residual_rms_norm_op(*args)
@@ -319,7 +315,7 @@ def residual_rms_norm_quantized(
             tensor is not None and tensor.requires_grad for tensor in (x, branch, weight)):
         raise RuntimeError("residual_rms_norm_quantized records no gradient: call it under "
                            "torch.no_grad(), or use residual_rms_norm")
-    if _has_tangent(x, branch, weight):
+    if has_tangent(x, branch, weight):
         raise RuntimeError("residual_rms_norm_quantized has no forward-mode derivative: call it "
                            "on tensors without a tangent, or use residual_rms_norm")
     args = (x, branch, weight, eps, dtype, group_size)
@@ -372,7 +368,7 @@ def dequantize(quantized, scale, *, group_size=None, dtype=torch.bfloat16,
                          "for each group of columns")
     if torch.is_grad_enabled() and scale.requires_grad:
         raise RuntimeError("dequantize records no gradient: call it under torch.no_grad()")
-    if _has_tangent(quantized, scale):
+    if has_tangent(quantized, scale):
         raise RuntimeError("dequantize has no forward-mode derivative: call it on tensors without "
                            "a tangent")
     args = (quantized, scale, group_size, dtype)
