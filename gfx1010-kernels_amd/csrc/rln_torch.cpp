@@ -729,6 +729,7 @@ PYBIND11_MODULE(_C, module) {
         pybind11::arg("parameter_groups"),
         pybind11::arg("compute_parameter_gradients"),
         pybind11::arg("branch_dtype") = pybind11::none());
+    module.def("graph_recorded", &graph_recorded);
     module.def("target_arch", []() { return std::string(rln_target_arch()); });
     module.def("library_version", []() { return std::string(rln_version()); });
 }

@@ -5,7 +5,9 @@
 
 #include <torch/extension.h>
 
+#include <ATen/TracerMode.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <functional>
 #include <initializer_list>
@@ -53,6 +55,25 @@ inline void refuse_tangents(
 // trace. Its dispatch key is then in the thread's included set.
 inline bool dispatch_watched() {
     return !(c10::impl::tls_local_dispatch_key_set().included_ - c10::default_included_set).empty();
+}
+
+// Whether the operators called on this thread are recorded into a graph
+// (torch.jit.trace, make_fx). Such a graph would hold the outputs' allocations
+// and no kernel, and return memory as it comes: the calls decline or raise, and
+// go through the registered operators (torch.ops.gfx1010_kernels) instead, which
+// a graph holds whole. A registered operator's own kernel runs outside of the
+// recording. PreDispatch stands for make_fx(pre_dispatch=True).
+inline bool graph_recorded() {
+    return dispatch_watched()
+        && (at::tracer::impl::is_dispatch_enabled()
+            || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch)
+            || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY)
+                   .has_value());
+}
+
+inline void refuse_recording(const char* what) {
+    TORCH_CHECK(!graph_recorded(), what, " is being recorded into a graph that cannot hold it; "
+                "torch.ops.gfx1010_kernels has the operators a graph can hold");
 }
 
 // Outputs and scratch, straight from the caching allocator. at::empty goes

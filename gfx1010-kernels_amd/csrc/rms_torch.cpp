@@ -73,6 +73,7 @@ void check_inputs(const at::Tensor& x, const at::Tensor& branch, const at::Tenso
                   double eps) {
     TORCH_CHECK(x.is_cuda(), "x must be a HIP tensor");
     refuse_tangents("residual RMSNorm", {x, branch, weight});
+    refuse_recording("residual RMSNorm");
     TORCH_CHECK((!branch.defined() || branch.is_cuda()) && weight.is_cuda(),
                 "branch and weight must be HIP tensors");
     TORCH_CHECK(
@@ -186,6 +187,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> backward_impl(
     bool weight_gradient) {
     TORCH_CHECK(grad_normalized_in.is_cuda(), "grad_normalized must be a HIP tensor");
     refuse_tangents("residual RMSNorm", {grad_updated_in, grad_normalized_in, updated, weight});
+    refuse_recording("residual RMSNorm's backward");
     const auto device = grad_normalized_in.device();
     TORCH_CHECK(
         (!grad_updated_in.defined() || grad_updated_in.device() == device)
@@ -426,7 +428,8 @@ std::optional<std::tuple<at::Tensor, at::Tensor>> residual_rms_norm_if_supported
     double eps,
     std::optional<at::ScalarType> normalized_dtype,
     bool checkpoint) {
-    if (!rms_inputs_supported(x, branch.value_or(at::Tensor()), weight, eps)) {
+    if (graph_recorded()
+        || !rms_inputs_supported(x, branch.value_or(at::Tensor()), weight, eps)) {
         return std::nullopt;
     }
     return residual_rms_norm(x, branch, weight, eps, normalized_dtype, checkpoint);
@@ -531,7 +534,8 @@ residual_rms_norm_quantized_if_supported(
     at::ScalarType dtype,
     int64_t group) {
     const at::Tensor branch = branch_in.value_or(at::Tensor());
-    if (!rms_inputs_supported(x, branch, weight, eps) || recorded(x, branch, weight)) {
+    if (graph_recorded() || !rms_inputs_supported(x, branch, weight, eps)
+        || recorded(x, branch, weight)) {
         return std::nullopt;
     }
     return residual_rms_norm_quantized(x, branch_in, weight, eps, dtype, group);
@@ -540,7 +544,8 @@ residual_rms_norm_quantized_if_supported(
 at::Tensor dequantize(const at::Tensor& quantized, const at::Tensor& scale, int64_t group,
                       at::ScalarType dtype) {
     TORCH_CHECK(quantized.is_cuda(), "quantized must be a HIP tensor");
-    refuse_tangents("residual RMSNorm", {quantized, scale});
+    refuse_tangents("dequantize", {quantized, scale});
+    refuse_recording("dequantize");
     TORCH_CHECK(scale.device() == quantized.device(),
                 "all tensors must be on the same HIP device");
     TORCH_CHECK(code_type(quantized.scalar_type()), "quantized must use int8 or float8_e4m3fn");
@@ -568,7 +573,8 @@ at::Tensor dequantize(const at::Tensor& quantized, const at::Tensor& scale, int6
 std::optional<at::Tensor> dequantize_if_supported(const at::Tensor& quantized,
                                                   const at::Tensor& scale, int64_t group,
                                                   at::ScalarType dtype) {
-    if (!quantized.is_cuda() || scale.device() != quantized.device() || quantized.dim() < 1
+    if (graph_recorded() || !quantized.is_cuda() || scale.device() != quantized.device()
+        || quantized.dim() < 1
         || !code_type(quantized.scalar_type()) || scale.scalar_type() != at::kFloat
         || quantized.size(-1) < 1
         || scale.sizes() != at::IntArrayRef(scale_sizes(quantized.sizes(), group))

@@ -62,6 +62,13 @@ def native_extension_status():
     return extension is not None, reason
 
 
+def graph_recorded():
+    """Whether ``torch.jit.trace`` or ``make_fx`` records this thread's operators:
+    the graph holds the registered ones, and nothing of the extension's calls."""
+    extension, _ = _extension()
+    return extension is not None and extension.graph_recorded()
+
+
 def native_residual_layer_norm(
     x,
     branch,
@@ -129,6 +136,7 @@ __all__ = [
     "launch_threads",
     "SPECIALIZED_HIDDEN_SIZES",
     "TARGET_ARCHITECTURE",
+    "graph_recorded",
     "native_extension_status",
     "native_residual_layer_norm",
     "native_residual_layer_norm_if_supported",

@@ -28,7 +28,7 @@ import warnings
 
 import torch
 
-from ._normalization_native import TARGET_ARCHITECTURE, _extension
+from ._normalization_native import TARGET_ARCHITECTURE, _extension, graph_recorded
 from ._ops import dequantize_op, residual_rms_norm_op, residual_rms_norm_quantized_op
 from .normalization import (
     IMPLEMENTATIONS,
@@ -164,6 +164,14 @@ def _input_reason(x, branch, weight, eps):
     return None
 
 
+def _traced_inputs_served(x, branch, weight, eps):
+    """Whether _input_reason finds none. From the extension's check while
+    torch.jit.trace runs, which hands out sizes that are tensors of its graph."""
+    if torch.jit.is_tracing():
+        return _extension()[0].rms_inputs_supported(x, branch, weight, float(eps))
+    return _input_reason(x, branch, weight, eps) is None
+
+
 def _check_implementation(implementation):
     if implementation not in IMPLEMENTATIONS:
         raise ValueError(
@@ -221,9 +229,10 @@ def residual_rms_norm(
     fp32, fp16 or bf16; tensors whose rows are evenly spaced are read in place,
     others are copied first.
 
-    Supports first-order autograd, HIP graph capture and ``torch.compile``; inputs
-    with a forward-mode tangent take the PyTorch path, which carries it (the native
-    modes raise). The
+    Supports first-order autograd, HIP graph capture, ``torch.compile``,
+    ``torch.jit.trace`` and ``make_fx`` (whose graphs hold the operators
+    ``torch.ops.gfx1010_kernels`` registers). Inputs with a forward-mode tangent
+    take the PyTorch path, which carries it (the native modes raise). The
     weight's gradient is summed in a fixed order (bitwise reproducible with and
     without ``torch.use_deterministic_algorithms``). The gradients of ``x`` and
     of a branch of the same type are one tensor, as those of ``x + branch`` are.
@@ -256,6 +265,10 @@ def residual_rms_norm(
             x, branch, weight, float(eps), normalized_dtype, checkpoint_dtype is not None)
         if result is not None:
             return result
+    if x.is_cuda and graph_recorded():
+        if implementation in _STRICT_NATIVE or _traced_inputs_served(x, branch, weight, eps):
+            return residual_rms_norm_op(*args)
+        return _torch_residual_rms_norm(*args)
     native, reason = _native_or_reason(x, _input_reason(x, branch, weight, eps), implementation)
     if native is None:
         _warn(reason)
@@ -325,6 +338,10 @@ def residual_rms_norm_quantized(
         if implementation in _STRICT_NATIVE or _input_reason(x, branch, weight, eps) is None:
             return residual_rms_norm_quantized_op(*args)
         return _torch_quantized(*args)
+    if x.is_cuda and graph_recorded():
+        if implementation in _STRICT_NATIVE or _traced_inputs_served(x, branch, weight, eps):
+            return residual_rms_norm_quantized_op(*args)
+        return _torch_quantized(*args)
     native, reason = _native_or_reason(x, _input_reason(x, branch, weight, eps), implementation)
     if native is None:
         _warn(reason)
@@ -375,6 +392,10 @@ def dequantize(quantized, scale, *, group_size=None, dtype=torch.bfloat16,
     if implementation == "torch":
         return _torch_dequantize(*args)
     if torch.compiler.is_compiling():
+        if implementation in _STRICT_NATIVE or _dequantize_reason(quantized, scale) is None:
+            return dequantize_op(*args)
+        return _torch_dequantize(*args)
+    if quantized.is_cuda and graph_recorded():
         if implementation in _STRICT_NATIVE or _dequantize_reason(quantized, scale) is None:
             return dequantize_op(*args)
         return _torch_dequantize(*args)
