@@ -182,13 +182,15 @@ def _check_implementation(implementation):
             "the Triton backend is not part of the MI355X build")
 
 
-def _native_or_reason(tensor, reason, implementation):
-    """The native extension, or None and why ``"auto"`` falls back; the strict
-    modes and a broken install on the target hardware raise."""
+def _native_or_reason(tensor, reason_of, implementation):
+    """The native extension, or None and why ``"auto"`` falls back (the answer of
+    ``reason_of()``, which the strict modes do not ask); the strict modes and a
+    broken install on the target hardware raise."""
     strict = implementation in _STRICT_NATIVE
+    reason = None if strict else reason_of()
     if strict and not tensor.is_cuda:
         raise RuntimeError(f"{_UNAVAILABLE}: the inputs must be HIP tensors")
-    if reason is None or strict:
+    if reason is None:
         if tensor.get_device() not in _READY_DEVICES:
             status = residual_layer_norm_status(tensor.device)
             if not status.available:
@@ -269,7 +271,8 @@ def residual_rms_norm(
         if implementation in _STRICT_NATIVE or _traced_inputs_served(x, branch, weight, eps):
             return residual_rms_norm_op(*args)
         return _torch_residual_rms_norm(*args)
-    native, reason = _native_or_reason(x, _input_reason(x, branch, weight, eps), implementation)
+    native, reason = _native_or_reason(
+        x, lambda: _input_reason(x, branch, weight, eps), implementation)
     if native is None:
         _warn(reason)
         return _torch_residual_rms_norm(*args)
@@ -342,7 +345,8 @@ def residual_rms_norm_quantized(
         if implementation in _STRICT_NATIVE or _traced_inputs_served(x, branch, weight, eps):
             return residual_rms_norm_quantized_op(*args)
         return _torch_quantized(*args)
-    native, reason = _native_or_reason(x, _input_reason(x, branch, weight, eps), implementation)
+    native, reason = _native_or_reason(
+        x, lambda: _input_reason(x, branch, weight, eps), implementation)
     if native is None:
         _warn(reason)
         return _torch_quantized(*args)
@@ -399,8 +403,8 @@ def dequantize(quantized, scale, *, group_size=None, dtype=torch.bfloat16,
         if implementation in _STRICT_NATIVE or _dequantize_reason(quantized, scale) is None:
             return dequantize_op(*args)
         return _torch_dequantize(*args)
-    native, reason = _native_or_reason(quantized, _dequantize_reason(quantized, scale),
-                                       implementation)
+    native, reason = _native_or_reason(
+        quantized, lambda: _dequantize_reason(quantized, scale), implementation)
     if native is None:
         _warn(reason)
         return _torch_dequantize(*args)
