@@ -57,6 +57,7 @@ void check_forward_inputs(
     double eps,
     int64_t threads) {
     refuse_tangents("residual LayerNorm", {x, branch, weight, bias});
+    refuse_recording("residual LayerNorm");
     TORCH_CHECK(x.is_cuda(), "x must be a HIP tensor");
     TORCH_CHECK(
         branch.is_cuda() && weight.is_cuda() && bias.is_cuda(),
@@ -110,6 +111,7 @@ void check_backward_inputs(
     refuse_tangents("residual LayerNorm",
                     {grad_updated ? *grad_updated : absent,
                      grad_normalized ? *grad_normalized : absent, updated, weight});
+    refuse_recording("residual LayerNorm's backward");
     TORCH_CHECK(updated.is_cuda(), "updated must be a HIP tensor");
     const auto device = updated.device();
     const bool same_device = (!grad_updated || grad_updated->device() == device)
@@ -652,7 +654,7 @@ std::optional<torch::autograd::variable_list> residual_layer_norm_if_supported(
     int64_t parameter_threads,
     int64_t parameter_groups,
     std::optional<at::ScalarType> normalized_dtype) {
-    if (!fused_inputs_supported(x, branch, weight, bias, dropout_p, eps)) {
+    if (graph_recorded() || !fused_inputs_supported(x, branch, weight, bias, dropout_p, eps)) {
         return std::nullopt;
     }
     return residual_layer_norm_autograd(x, branch, weight, bias, dropout_p, eps, training,

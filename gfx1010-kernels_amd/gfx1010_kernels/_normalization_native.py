@@ -116,6 +116,10 @@ def native_residual_layer_norm_if_supported(
     native hidden size), else None. For callers that already know the
     extension is loaded and the device ready; ``x`` has at least two
     dimensions."""
+    try:
+        threads = _THREADS.get(x.shape[-1], 128)
+    except TypeError:  # a size without a hash: traced symbolically, by no native call
+        return None
     result = _extension()[0].residual_layer_norm_if_supported(
         x,
         branch,
@@ -124,7 +128,7 @@ def native_residual_layer_norm_if_supported(
         float(dropout_p),
         float(eps),
         bool(training),
-        _THREADS.get(x.shape[-1], 128),
+        threads,
         *_LAUNCH_HINTS,
         normalized_dtype,
     )

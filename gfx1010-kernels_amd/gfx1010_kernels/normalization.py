@@ -41,6 +41,8 @@ from ._normalization_native import (
     NATIVE_HIDDEN_SIZES,
     NATIVE_HIDDEN_SIZES_TEXT,
     TARGET_ARCHITECTURE,
+    _extension,
+    graph_recorded,
     native_residual_layer_norm,
     native_residual_layer_norm_if_supported,
 )
@@ -244,6 +246,23 @@ def _traced(x, branch, weight, bias, dropout_p, eps, training, normalized_dtype,
     return _torch_residual_layer_norm(*args)
 
 
+def _recorded(x, branch, weight, bias, dropout_p, eps, training, normalized_dtype,
+              implementation):
+    """Dispatch of HIP tensors while ``torch.jit.trace`` or ``make_fx`` records:
+    the graph holds the registered operator, as a compiled one does. The sizes are
+    asked in C++ under ``torch.jit.trace``, whose own are tensors of its graph."""
+    args = (x, branch, weight, bias, dropout_p, eps, training, normalized_dtype)
+    if torch.jit.is_tracing():
+        served = _extension()[0].fused_inputs_supported(
+            x, branch, weight, bias, float(dropout_p), float(eps))
+    else:
+        served = (_input_reason(x, branch, weight, bias, dropout_p, eps) is None
+                  and int(x.shape[-1]) in _NATIVE_SIZES)
+    if served or implementation in _STRICT_NATIVE:
+        return residual_layer_norm_op(*args)
+    return _torch_residual_layer_norm(*args)
+
+
 def residual_layer_norm(
     x,
     branch,
@@ -263,8 +282,10 @@ def residual_layer_norm(
     is ``torch.float16`` / ``torch.bfloat16``, rounded to that type for a
     half-precision consumer (the reference always returns fp32). ``branch``
     may be fp32, fp16 or bf16. Supports first-order autograd, HIP graph
-    capture and ``torch.compile``; inputs with a forward-mode tangent take the
-    PyTorch path, which carries it (the native modes raise).
+    capture, ``torch.compile``, ``torch.jit.trace`` and ``make_fx`` (whose graphs
+    hold the operators ``torch.ops.gfx1010_kernels`` registers). Inputs with a
+    forward-mode tangent take the PyTorch path, which carries it (the native
+    modes raise).
     """
     if implementation not in IMPLEMENTATIONS:
         raise ValueError(
@@ -279,7 +300,14 @@ def residual_layer_norm(
     if torch.compiler.is_compiling():
         return _traced(*args, implementation)
     if implementation in _STRICT_NATIVE:
-        return _strict_native(*args)
+        try:
+            return _strict_native(*args)
+        except (RuntimeError, TypeError):
+            # The extension refuses to be recorded; asked here, so that other calls
+            # do not pay for the question (0.2 of 5.6 us).
+            if x.is_cuda and graph_recorded():
+                return _recorded(*args, implementation)
+            raise
     # Inputs the fused kernels serve, on a device whose backend is known to be
     # ready: one C++ check and call. The reasons below are only worked out
     # when it declines.
@@ -290,6 +318,8 @@ def residual_layer_norm(
         if result is not None:
             return result
 
+    if implementation == "auto" and x.is_cuda and graph_recorded():
+        return _recorded(*args, implementation)
     reason = _input_reason(x, branch, weight, bias, dropout_p, eps)
     if implementation == "triton":
         raise RuntimeError(
