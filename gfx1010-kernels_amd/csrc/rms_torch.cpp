@@ -20,6 +20,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/dynamo/compiled_autograd.h>
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -292,37 +293,128 @@ class ResidualRmsNormBackward : public torch::autograd::Node {
     // either may be undefined.
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
-        const at::Tensor grad_updated = branch_type ? grads[0] : at::Tensor();
-        const at::Tensor grad_normalized = branch_type ? grads[1] : grads[0];
+        if (!grads[branch_type ? 1 : 0].defined()) {
+            Held held;  // the addition's gradient needs nothing that is kept
+            held.branch_type = branch_type;
+            return gradients(grads, held);
+        }
+        return gradients(grads, unpack());
+    }
+
+    // Compiled autograd: what the node holds, and its gradients as one call that the
+    // compiled graph makes with its own tensors.
+    void compiled_args(torch::dynamo::autograd::CompiledNodeArgs& args) const override {
+        if (!checkpoint) {
+            args.collect(kept, branch_type.has_value());
+        }
+        args.collect(weight, false);
+        args.collect(state, false);
+        args.collect(x_type);
+        args.collect(branch_type);
+        args.collect(checkpoint);
+    }
+
+    torch::autograd::variable_list apply_with_saved(
+        const torch::autograd::variable_list& grads,
+        torch::dynamo::autograd::SwapSavedVariables& saved) override {
+        namespace compiled = torch::dynamo::autograd;
+        if (!checkpoint) {
+            saved.before(kept);
+        }
+        saved.before(weight);
+        saved.before(state);
+        const Held held = unpack();
+        compiled::PackedArgs packed;
+        packed.pack(held.kept.defined() ? std::optional(held.kept) : std::nullopt);
+        packed.pack(held.weight);
+        packed.pack(held.state);
+        packed.pack(held.x_type);
+        packed.pack(held.branch_type);
+        packed.pack(held.checkpoint);
+        packed.pack(held.weight_gradient);
+        const auto call = [](const torch::autograd::variable_list& grads,
+                             const std::vector<c10::IValue>& args) {
+            compiled::PackedArgs given(args);
+            Held held;
+            held.kept = given.unpack<std::optional<at::Tensor>>().value_or(at::Tensor());
+            held.weight = given.unpack<at::Tensor>();
+            held.state = given.unpack<at::Tensor>();
+            held.x_type = given.unpack<at::ScalarType>();
+            held.branch_type = given.unpack<std::optional<at::ScalarType>>();
+            held.checkpoint = given.unpack<bool>();
+            held.weight_gradient = given.unpack<bool>();
+            return gradients(grads, held);
+        };
+        const auto& compiler = compiled::getPyCompilerInterface();
+        const std::string function = compiler->bind_function(
+            saved.get_py_compiler(), name(), call,
+            {compiled::IValuePacker<std::optional<at::Tensor>>::packed_type(),
+             compiled::IValuePacker<at::Tensor>::packed_type(),
+             compiled::IValuePacker<at::Tensor>::packed_type(),
+             compiled::IValuePacker<at::ScalarType>::packed_type(),
+             compiled::IValuePacker<std::optional<at::ScalarType>>::packed_type(),
+             compiled::IValuePacker<bool>::packed_type(),
+             compiled::IValuePacker<bool>::packed_type()},
+            /*is_custom_function=*/true, /*is_traceable=*/false);
+        auto results = compiler->call_function(
+            saved.get_py_compiler(), "apply_functional", function, grads, packed.vec(),
+            compiled::IValuePacker<std::vector<std::optional<torch::autograd::InputMetadata>>>::
+                pack(compiled::get_input_metadata(next_edges())));
+        if (!checkpoint) {
+            saved.after(kept);
+        }
+        saved.after(weight);
+        saved.after(state);
+        return results;
+    }
+
+ private:
+    // What the gradients are computed from.
+    struct Held {
+        at::Tensor kept;
+        at::Tensor weight;
+        at::Tensor state;
+        at::ScalarType x_type = at::kFloat;
+        std::optional<at::ScalarType> branch_type;
+        bool checkpoint = false;
+        bool weight_gradient = false;
+    };
+
+    Held unpack() {
+        return Held{checkpoint ? at::Tensor() : kept.unpack(branch_type ? getptr() : nullptr),
+                    weight.unpack(), state.unpack(), x_type, branch_type, checkpoint,
+                    task_should_compute_output(2)};
+    }
+
+    static torch::autograd::variable_list gradients(const torch::autograd::variable_list& grads,
+                                                    const Held& held) {
+        const at::Tensor grad_updated = held.branch_type ? grads[0] : at::Tensor();
+        const at::Tensor grad_normalized = held.branch_type ? grads[1] : grads[0];
         at::Tensor grad_x;
         at::Tensor grad_branch;
         at::Tensor grad_weight;
         if (grad_normalized.defined()) {
-            const auto kept_rows =
-                checkpoint ? at::Tensor() : kept.unpack(branch_type ? getptr() : nullptr);
-            const auto weight_row = weight.unpack();
             std::tie(grad_x, grad_branch, grad_weight) = backward_impl(
-                grad_updated, grad_normalized, kept_rows, state.unpack(), weight_row, x_type,
-                branch_type, checkpoint, task_should_compute_output(2));
-            if (branch_type && !grad_branch.defined()) {
+                grad_updated, grad_normalized, held.kept, held.state, held.weight, held.x_type,
+                held.branch_type, held.checkpoint, held.weight_gradient);
+            if (held.branch_type && !grad_branch.defined()) {
                 grad_branch = grad_x;  // one tensor, as for any addition
             }
             if (at::GradMode::is_enabled()) {
                 // create_graph: the gradients are constants of a backward that
                 // has none of its own; differentiating them again raises.
                 refuse_second_order(
-                    {grad_updated, grad_normalized, kept_rows, weight_row},
+                    {grad_updated, grad_normalized, held.kept, held.weight},
                     {grad_x, grad_branch.is_same(grad_x) ? at::Tensor() : grad_branch,
                      grad_weight});
             }
         } else if (grad_updated.defined()) {
             grad_x = grad_updated;
-            grad_branch = grad_updated.to(*branch_type);
+            grad_branch = grad_updated.to(*held.branch_type);
         }
         return {grad_x, grad_branch, grad_weight};
     }
 
- private:
     static void refuse_second_order(const torch::autograd::variable_list& inputs,
                                     const torch::autograd::variable_list& outputs) {
         if (!torch::autograd::any_variable_requires_grad(inputs)) {
