@@ -22,6 +22,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/dynamo/compiled_autograd.h>
 
+#include <ATen/NamedTensorUtils.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
@@ -93,10 +94,17 @@ void check_inputs(const at::Tensor& x, const at::Tensor& branch, const at::Tenso
     TORCH_CHECK(eps >= 0.0, "eps must not be negative");
 }
 
-// Outputs in x's shape; what empty_device_like takes over from a contiguous x.
+// Dense outputs in x's shape, with its dimension names; of a contiguous x
+// whatever else empty_device_like takes over.
 at::Tensor output_like(const at::Tensor& x, at::ScalarType type) {
-    return x.is_contiguous() ? empty_device_like(x, type)
-                             : empty_device(x.sizes(), type, x.device());
+    if (x.is_contiguous()) {
+        return empty_device_like(x, type);
+    }
+    auto output = empty_device(x.sizes(), type, x.device());
+    if (x.has_names()) {
+        at::namedinference::propagate_names(output, x);
+    }
+    return output;
 }
 
 // What a recorded forward keeps beside (or, with the checkpoint, in the place

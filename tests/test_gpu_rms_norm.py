@@ -8,6 +8,7 @@ lane, a short last vector, groups of 32 to 256 columns that end inside a vector.
 
 import itertools
 import threading
+import warnings
 
 import pytest
 import torch
@@ -917,3 +918,29 @@ def test_serving_stack():
                 exact = residual_rms_norm(x, branch, norm, EPS)[1]
                 assert (wide - exact).float().norm() < 0.04 * exact.float().norm()
                 x, branch = ours[0], wide @ weight
+
+
+# What the calls take over from their inputs, and what they keep.
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("added", [True, False])
+@pytest.mark.parametrize("layout", ["dense", "part of wider rows", "transposed"])
+def test_outputs_keep_dimension_names(layout, added, grad):
+    x, branch, weight = (t.cuda() for t in make((3, 4, 96), F32, BF16, F32))
+    wide = {"dense": x, "part of wider rows": torch.cat([x, x], -1)[..., :96],
+            "transposed": x.transpose(0, 1).contiguous().transpose(0, 1)}[layout]
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        named = wide.refine_names("N", "T", "C")
+    leaf = named.requires_grad_(grad)
+    for implementation in ("gfx950", "auto"):
+        outputs = residual_rms_norm(leaf, branch if added else None, weight, EPS,
+                                    implementation=implementation)
+        assert [t.names for t in outputs] == [("N", "T", "C")] * 2
+        plain = residual_rms_norm(x, branch if added else None, weight, EPS)
+        for a, b in zip(outputs, plain):
+            assert reference.same_bits(a.detach().rename(None), b)
+    with torch.no_grad():
+        _, codes, scale = residual_rms_norm_quantized(leaf, branch, weight, EPS, dtype=torch.int8)
+        assert codes.names == ("N", "T", "C")
+        assert dequantize(codes, scale, dtype=F32).names == ("N", "T", "C")
