@@ -277,7 +277,12 @@ rms_forward.register_autograd(_rms_backward_formula, setup_context=_rms_setup_co
 
 
 def residual_rms_norm_op(x, branch, weight, eps, normalized_dtype=None, checkpoint=False):
-    """``(updated, normalized)`` through the registered custom op."""
+    """``(updated, normalized)`` through the registered custom op. A compiled call that
+    records no gradient writes no checkpoint (grad mode and what requires a gradient
+    are guarded by the compiler; other recorded graphs may run under any)."""
+    if checkpoint and torch.compiler.is_compiling():
+        checkpoint = torch.is_grad_enabled() and any(
+            tensor is not None and tensor.requires_grad for tensor in (x, branch, weight))
     updated, normalized, _ = rms_forward(x, branch, weight, float(eps), normalized_dtype,
                                          checkpoint)
     return (x if branch is None else updated), normalized

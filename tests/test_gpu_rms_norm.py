@@ -944,3 +944,32 @@ def test_outputs_keep_dimension_names(layout, added, grad):
         _, codes, scale = residual_rms_norm_quantized(leaf, branch, weight, EPS, dtype=torch.int8)
         assert codes.names == ("N", "T", "C")
         assert dequantize(codes, scale, dtype=F32).names == ("N", "T", "C")
+
+
+@pytest.mark.parametrize("grad,needs,expected", [(False, True, False), (True, False, False),
+                                                 (True, True, True)])
+def test_a_compiled_call_writes_a_checkpoint_only_where_a_gradient_is_recorded(grad, needs,
+                                                                               expected):
+    calls = []
+
+    def backend(module, _):
+        calls.extend(node.args[5] for node in module.graph.nodes
+                     if "rms_forward" in str(node.target))
+        return module.forward
+
+    def function(x, branch, weight):
+        updated, first = residual_rms_norm(x, branch, weight, EPS, checkpoint_dtype=torch.int8)
+        return residual_rms_norm(updated, first, weight, EPS, checkpoint_dtype=torch.int8)
+
+    x, branch, weight = (t.cuda() for t in make((6, 200), F32, BF16, F32))
+    weight.requires_grad_(needs)
+    torch._dynamo.reset()
+    with torch.set_grad_enabled(grad):
+        outputs = torch.compile(function, backend=backend, fullgraph=True)(x, branch, weight)
+        for a, b in zip(outputs, function(x, branch, weight)):
+            assert reference.same_bits(a, b) and a.requires_grad == b.requires_grad
+    assert calls == [expected, expected]
+    if expected:
+        grads = [torch.autograd.grad(o[1].square().sum() + o[0].sin().sum(), weight)[0]
+                 for o in (outputs, function(x, branch, weight))]
+        assert reference.same_bits(*grads)
