@@ -973,3 +973,57 @@ def test_a_compiled_call_writes_a_checkpoint_only_where_a_gradient_is_recorded(g
         grads = [torch.autograd.grad(o[1].square().sum() + o[0].sin().sum(), weight)[0]
                  for o in (outputs, function(x, branch, weight))]
         assert reference.same_bits(*grads)
+
+
+def test_two_threads_end():
+    """As test_two_threads_at_once, of threads that are known to have ended, with
+    backwards of both forms (slab blocks and the walk)."""
+    cases = [tuple(t.cuda() for t in make((rows, 1000), F32, BF16, F32, rows))
+             for rows in (300, 2500)]
+
+    def work(x, branch, weight):
+        leaves = [t.clone().requires_grad_() for t in (x, branch, weight)]
+        outputs = residual_rms_norm(*leaves, EPS, implementation="gfx950")
+        return [*outputs, *torch.autograd.grad(outputs, leaves, [x, x])]
+
+    expected = [work(*case) for case in cases]
+    torch.cuda.synchronize()
+    results = {}
+
+    def run(index):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                found = work(*cases[index])
+        stream.synchronize()
+        results[index] = all(reference.same_bits(a, b) for a, b in zip(found, expected[index]))
+
+    threads = [threading.Thread(target=run, args=(index,), daemon=True) for index in range(2)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join(timeout=60)
+        assert not thread.is_alive()
+    assert results == {0: True, 1: True}
+
+
+def test_what_transforms_and_fake_tensors_are_refused_for():
+    """The kernels ask for addresses, which a transform's tensor does not have and
+    a fake output's are null."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    x, branch, weight = (t.cuda() for t in make((3, 64), F32, F32, F32))
+    residual_rms_norm(x, branch, weight)
+    for implementation in ("auto", "gfx950"):
+        options = dict(implementation=implementation)
+        for call in (lambda t: residual_rms_norm(t, t, weight, **options)[1],
+                     lambda t: residual_rms_norm(t, None, weight, **options)[1],
+                     lambda t: residual_rms_norm_quantized(t, None, weight, **options)[2]):
+            with pytest.raises(RuntimeError, match="data pointer"):
+                torch.func.vmap(call)(x)
+            with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(
+                    RuntimeError, match="must not be null|data is not allocated"):
+                call(x)
+            assert call(x).isfinite().all()
+        with pytest.raises(RuntimeError, match="data pointer"):
+            torch.func.grad(lambda t: residual_rms_norm(t, branch, weight, **options)[1].sum())(x)
