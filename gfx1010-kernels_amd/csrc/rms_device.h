@@ -170,7 +170,9 @@ struct Raw {
 // through: measured against plain stores, [16384, 4096] bf16 forward 84.0 against
 // 90.3 us (write-through 85.5), [6001, 2880] 25.6 against 28.2 (26.3), [8192, 8192]
 // fp32 backward with the checkpoint 157.0 against 170.4 (non-temporal 159.8),
-// [16384, 2048] bf16 44.2 against 46.1 (45.6).
+// [16384, 2048] bf16 44.2 against 46.1 (45.6). All over buffers that pass the caches;
+// what a small launch's consumer pays for outputs it might have found there was not
+// measured.
 constexpr int kCached = 0;
 constexpr int kOnce = 2;
 constexpr int kForwardStores = 2;
@@ -1132,9 +1134,12 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 //    16-bit stream ([16384, 4096] bf16: 6.2 against 5.9 with two) and two of a
 //    32-bit one, whose half as many waves then store whole words of codes
 //    ([32768, 1024] e4m3 in fp32: 6.2 against 5.4 with one; without codes 6.2
-//    against 5.9), and doubles them until a row fits 8 waves: in blocks of 16
-//    waves a CU idles while they wait for each other ([8192, 8192] fp32 with the
-//    checkpoint: 5.6 with four slots and 8 waves, 5.2 with two and 16).
+//    against 5.9), and doubles them until a row fits 8 waves, a 32-bit stream's up
+//    to four: in blocks of 16 waves a CU idles while they wait for each other
+//    ([8192, 8192] fp32 with the checkpoint: 5.6 with four slots and 8 waves, 5.2
+//    with two and 16). A 16-bit stream's stop at two, so that its rows past 8192
+//    columns take 9 to 16 waves, at no loss ([8192, 16384] bf16: 6.0, [8192, 9216]
+//    6.0, [8192, 8192] in 8 waves 6.0).
 //  * Short rows share waves, 2, 4 or 8 in each ([262144, 128] bf16 forward 52 against
 //    83 us with a wave for each, with codes 44 against 110, backward 50 against 80;
 //    [524288, 64] 52 against 156, 71 with at least 16 lanes a row).

@@ -30,6 +30,8 @@ fused op instead of breaking around it (the reference does not support
 * ``gfx1010_kernels::rms_forward`` / ``rms_backward`` / ``rms_quantized`` /
   ``dequantize`` do the same for the root-mean-square norm
   (``_C.residual_rms_norm_*``). They draw nothing, so equal calls may be merged.
+
+``torch.jit.trace`` and ``make_fx`` record these operators as well.
 """
 
 from __future__ import annotations
