@@ -234,7 +234,8 @@ def residual_rms_norm(
     Supports first-order autograd, HIP graph capture, ``torch.compile``,
     ``torch.jit.trace`` and ``make_fx`` (whose graphs hold the operators
     ``torch.ops.gfx1010_kernels`` registers). Inputs with a forward-mode tangent
-    take the PyTorch path, which carries it (the native modes raise). The
+    take the PyTorch path, which carries it (the native modes raise, and so does
+    ``checkpoint_dtype``, whose norm has no forward-mode derivative). The
     weight's gradient is summed in a fixed order (bitwise reproducible with and
     without ``torch.use_deterministic_algorithms``). The gradients of ``x`` and
     of a branch of the same type are one tensor, as those of ``x + branch`` are.

@@ -93,3 +93,25 @@ def test_a_compiled_step():
         torch.compile(function, backend="aot_eager")(*inputs).backward()
     for a, b in zip(inputs, expected):
         assert reference.same_bits(a.grad, b)
+
+
+@pytest.mark.parametrize("checkpoint", [None, torch.int8])
+def test_other_row_counts_after_the_first(checkpoint):
+    """One compiler over calls of several sizes, whose graphs it may make dynamic."""
+    def function(x, branch, weight):
+        updated, normalized = residual_rms_norm(x, branch, weight, checkpoint_dtype=checkpoint)
+        return updated.float().sin().sum() + normalized.float().square().sum()
+
+    def inputs(rows, hidden):
+        generator = torch.Generator("cuda").manual_seed(rows)
+        return [torch.randn(shape, device="cuda", generator=generator).requires_grad_()
+                for shape in ((rows, hidden), (rows, hidden), (hidden,))]
+
+    torch._dynamo.reset()
+    compiler = torch.compile(backend="eager")
+    for rows, hidden in ((6, 200), (7, 200), (9, 200), (9, 96), (2000, 200)):
+        expected, found = inputs(rows, hidden), inputs(rows, hidden)
+        function(*expected).backward()
+        with compiled_autograd._enable(compiler):
+            function(*found).backward()
+        assert all(reference.same_bits(a.grad, b.grad) for a, b in zip(found, expected))

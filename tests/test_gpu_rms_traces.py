@@ -136,3 +136,19 @@ def test_the_extension_itself_refuses_to_be_recorded():
         with pytest.raises(RuntimeError, match="recorded into a graph"):
             make_fx(call)(x)
         call(x)
+
+
+@pytest.mark.parametrize("checkpoint", [None, torch.int8])
+@pytest.mark.parametrize("traced_with_grad", [False, True])
+def test_gradients_through_a_traced_call(checkpoint, traced_with_grad):
+    norm = functions("auto", checkpoint)[0]
+    with torch.set_grad_enabled(traced_with_grad):
+        traced = torch.jit.trace(norm, tuple(t.requires_grad_(traced_with_grad) for t in make()))
+    for seed, rows in ((1, 5), (2, 5), (3, 2000)):
+        results = []
+        for call in (traced, norm):
+            leaves = [t.requires_grad_() for t in make(seed, rows)]
+            outputs = call(*leaves)
+            loss = outputs[0].sin().sum() + outputs[1].square().sum()
+            results.append([*outputs, *torch.autograd.grad(loss, leaves)])
+        check_same(*([t.detach() for t in r] for r in results))
