@@ -32,7 +32,8 @@ ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = "gfx950"
 LIBRARY = PACKAGE / f"librln_{ARCH}.so"
 GLUE = PACKAGE / f"_C{sysconfig.get_config_var('EXT_SUFFIX')}"
-GLUE_SOURCES = (CSRC / "rln_torch.cpp", CSRC / "rms_torch.cpp")
+GLUE_SOURCES = (CSRC / "rln_torch.cpp", CSRC / "rms_torch.cpp", CSRC / "gated_torch.cpp",
+                CSRC / "rotary_torch.cpp")
 PROBE_SOURCE = REPO / "benchmarks" / "rln_probe.hip"
 PROBE = REPO / "benchmarks" / f"librln_probe_{ARCH}.so"
 
@@ -73,7 +74,8 @@ FIXED_BACKWARD = (128, 256, 384, 512, 768)
 WIDE_FORWARD = ((1, 1), (2, 1), (3, 1), (4, 1), (3, 2), (4, 2), (3, 4), (4, 4), (3, 8), (4, 8))
 WIDE_BACKWARD = ((1, 1), (2, 1), (3, 1), (1, 3), (1, 4), (3, 2), (2, 4), (3, 4), (2, 8), (3, 8),
                  (4, 8), (2, 16))
-# The root-mean-square norm: one translation unit per stream type and pass.
+# The root-mean-square norm and the gated residual norm: one translation unit each
+# per stream type and pass.
 RMS_STREAMS = ("float", "half_t", "bf16_t")
 RMS_PASSES = (("forward", 1), ("backward", 2))
 BUILD_DIR = ROOT / "_build"
@@ -119,11 +121,12 @@ def build_library(jobs: int | None = None, defines: tuple[str, ...] = (),
         for v, p in sorted(set(WIDE_FORWARD) | set(WIDE_BACKWARD))
     ]
     units += [
-        (CSRC / "rms_kernels.hip", build_dir / f"rms_{stream}_{name}.o",
+        (CSRC / f"{norm}_kernels.hip", build_dir / f"{norm}_{stream}_{name}.o",
          [*extra, f"-DRMS_STREAM={stream}", f"-DRMS_PASS={number}"])
-        for stream in RMS_STREAMS for name, number in RMS_PASSES
+        for norm in ("rms", "gated") for stream in RMS_STREAMS for name, number in RMS_PASSES
     ]
-    units += [(CSRC / "rms_api.hip", build_dir / "rms_api.o", extra)]
+    units += [(CSRC / f"{name}.hip", build_dir / f"{name}.o", extra)
+              for name in ("rms_api", "gated_api", "rotary")]
     workers = jobs or min(len(units), max(1, (os.cpu_count() or 1)))
     with ThreadPoolExecutor(max_workers=workers) as pool:
         objects = list(pool.map(lambda unit: _compile_object(*unit), units))

@@ -1,0 +1,683 @@
+// Kernels of the gated residual norm (include/rln.h, the rln_gated_* entry
+// points): a block's output, normed, gated and scaled, added to the stream,
+// and the norm in front of the next block.
+//
+// Per row of H values (rs, bs two constants; gate and the norms' weights rows of
+// H values, c = bs * gate * branch_weight):
+//
+//   rb = 1 / sqrt(sum(branch^2) / H + branch_eps), or 1 without a branch weight
+//   u  = rs * x + c * (branch * rb), rounded to x's type
+//   r  = 1 / sqrt(sum(u^2) / H + eps);    normalized = u * r * weight
+//
+// Backward, with v = u * r, a = branch * rb and p = gy * weight:
+//
+//   g           = gu + r * (p - v * sum(p * v) / H)        the gradient of u
+//   grad_x      = rs * g
+//   q           = c * g                                     the gradient of a
+//   grad_branch = rb * (q - a * sum(q * a) / H), or q without a branch weight
+//   S = g * a,  T = gy * v; their sums over the rows give, by products with rows
+//   that do not depend on the token, the gradients of gate, branch_weight, weight
+//
+// sum(q * a) would wait for sum(p * v). With g written out it is
+//
+//   sum(q * a) = sum(c * a * (gu + r * p)) - r * sum(p * v) / H * sum(c * a * v)
+//
+// so the row's three sums are taken together, and a row costs one exchange
+// between its waves instead of two.
+//
+// Every pass is bound by memory (about 15 fp32 operations per element forward, 40
+// backward, against 6-24 bytes). Rows, waves, vectors and accesses are those of the
+// root-mean-square norm (rms_device.h), whose helpers these kernels use.
+#ifndef GATED_DEVICE_H
+#define GATED_DEVICE_H
+
+#include "rms_device.h"
+
+namespace rln {
+namespace gated {
+
+using namespace rms;
+
+// A row of factors (gate, weight) that `rows` consecutive rows of the stream
+// share: all rows, those of a sample, or one.
+struct Factor {
+    const void* data;  // null: one
+    int64_t stride;    // between consecutive rows of factors, in elements
+    int64_t rows;
+    int dtype;
+};
+
+struct ForwardArgs {
+    const void* x;
+    const void* branch;
+    const void* branch_weight;  // null without a norm of the branch
+    Factor gate;
+    Factor weight;
+    void* updated;
+    void* normalized;
+    float* statistics;  // r, then rb, [rows] each; may be null
+    int64_t x_stride;
+    int64_t branch_stride;
+    int64_t rows;
+    int hidden;
+    int parts;
+    int row_lanes;
+    int words;
+    int branch_weight_dtype;
+    int output_dtype;
+    float residual_scale;
+    float branch_scale;
+    float eps;
+    float branch_eps;
+    float inv_hidden;
+};
+
+struct BackwardArgs {
+    const void* grad_updated;     // may be null, as grad_normalized
+    const void* grad_normalized;
+    const void* updated;
+    const void* branch;
+    const void* branch_weight;
+    Factor gate;
+    Factor weight;
+    const float* statistics;
+    void* grad_x;
+    void* grad_branch;
+    void* grad_gate;    // of a gate with a row for each token; else null
+    float* partials;    // [units][2][hidden]: sums of S and T, or null
+    int64_t branch_stride;
+    int64_t rows;
+    int64_t group_rows;  // rows that share their factors
+    int64_t units;       // runs of rows with sums of their own
+    int group_units;     // of a group
+    int hidden;
+    int parts;
+    int row_lanes;
+    int words;
+    int grad_dtype;      // grad_normalized's
+    int branch_weight_dtype;
+    float residual_scale;
+    float branch_scale;
+    float inv_hidden;
+};
+
+// N elements of a type known at run time, as raw words (16-bit ones in the
+// first half). Loaded and widened apart, so that a row's loads are all under way
+// before the first is waited for.
+template <int N>
+struct RawAny {
+    uint32_t words[N];
+};
+
+template <Access kAccess, int N, int Policy = kCached>
+__device__ __forceinline__ RawAny<N> load_any(const void* data, int dtype, int64_t first,
+                                              int column, int hidden) {
+    RawAny<N> out;
+    if (dtype == RLN_DTYPE_F32) {
+        const auto raw = load<kAccess, float, N, Policy>(static_cast<const float*>(data) + first,
+                                                         column, hidden);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            out.words[i] = raw.words[i];
+        }
+    } else {  // both 16-bit types are loaded alike
+        const auto raw = load<kAccess, half_t, N, Policy>(static_cast<const half_t*>(data) + first,
+                                                          column, hidden);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            out.words[i] = i < N / 2 ? raw.words[i] : 0;
+        }
+    }
+    return out;
+}
+
+template <Access kAccess, int N>
+__device__ __forceinline__ void widen_any(const RawAny<N>& any, int dtype, int column, int hidden,
+                                          float (&out)[N]) {
+    if (dtype == RLN_DTYPE_F32) {
+        Raw<float, N> raw;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            raw.words[i] = any.words[i];
+        }
+        settle<kAccess>(raw, column, hidden);
+        widen<float, N>(raw, out);
+    } else {
+        Raw<half_t, N> raw;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            raw.words[i] = any.words[i];
+        }
+        settle<kAccess>(raw, column, hidden);
+        if (dtype == RLN_DTYPE_F16) {
+            widen<half_t, N>(raw, out);
+        } else {
+            Raw<bf16_t, N> other;
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+                other.words[i] = raw.words[i];
+            }
+            widen<bf16_t, N>(other, out);
+        }
+    }
+}
+
+// Of a tensor that may be missing; `missing` is then every element's value.
+template <Access kAccess, int N, int Policy = kCached>
+__device__ __forceinline__ RawAny<N> load_optional(const void* data, int dtype, int64_t first,
+                                                   int column, int hidden) {
+    if (data != nullptr) {
+        return load_any<kAccess, N, Policy>(data, dtype, first, column, hidden);
+    }
+    return RawAny<N>{};
+}
+
+template <Access kAccess, int N>
+__device__ __forceinline__ void widen_optional(const RawAny<N>& raw, const void* data, int dtype,
+                                               int column, int hidden, float missing,
+                                               float (&out)[N]) {
+    if (data != nullptr) {
+        widen_any<kAccess, N>(raw, dtype, column, hidden, out);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            out[e] = missing;
+        }
+    }
+}
+
+// The first element of the factors' row for a row of the stream.
+__device__ __forceinline__ int64_t factor_row(const Factor& factor, int64_t row, int64_t rows) {
+    if (factor.rows >= rows) {
+        return 0;
+    }
+    if (factor.rows == 1) {
+        return row * factor.stride;
+    }
+    return (rows <= UINT32_MAX ? static_cast<int64_t>(static_cast<uint32_t>(row)
+                                                      / static_cast<uint32_t>(factor.rows))
+                               : row / factor.rows) * factor.stride;
+}
+
+// The factors from an element on.
+__device__ __forceinline__ const void* row_of(const Factor& factor, int64_t first) {
+    return static_cast<const char*>(factor.data) + first * (factor.dtype == RLN_DTYPE_F32 ? 4 : 2);
+}
+
+// N elements of a streamed tensor whose type is known at run time.
+template <Access kAccess, typename T, int N>
+__device__ __forceinline__ void load_widened(const void* data, int64_t first, int column,
+                                             int hidden, float (&out)[N]) {
+    auto raw = load<kAccess, T, N>(static_cast<const T*>(data) + first, column, hidden);
+    settle<kAccess>(raw, column, hidden);
+    widen<T, N>(raw, out);
+}
+
+template <Access kAccess, int N>
+__device__ __forceinline__ void load_upstream(const void* data, int dtype, int64_t first,
+                                              int column, int hidden, float (&out)[N]) {
+    if (dtype == RLN_DTYPE_F32) {
+        load_widened<kAccess, float, N>(data, first, column, hidden, out);
+    } else if (dtype == RLN_DTYPE_F16) {
+        load_widened<kAccess, half_t, N>(data, first, column, hidden, out);
+    } else {
+        load_widened<kAccess, bf16_t, N>(data, first, column, hidden, out);
+    }
+}
+
+template <Access kAccess>
+__device__ __forceinline__ float row_total(float value, int row_lanes) {
+    return kAccess == Access::kLanes ? lanes_sum(value, row_lanes) : wave_sum(value);
+}
+
+// ----------------------------------------------------------------------------
+// Forward: one row per team and turn, as rms_device.h's.
+
+template <typename X, typename B, int V, bool kPost, Access kAccess>
+__global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs a) {
+    constexpr int N = kColumns<X>;
+    __shared__ float sums[2][2][kMaxParts];
+    const Team team = team_of(a.parts);
+    const Place place = place_of<kAccess>(a.row_lanes);
+    const int block_rows = team.teams * place.rows;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * block_rows;
+    int turn = 0;
+    // The team's total of one value per wave; every team of the block makes the
+    // same number of calls. Two buffers: a wave that is ahead writes the one that
+    // the slower ones do not read.
+    const auto team_total = [&](float value, int which) {
+        if (a.parts > 1) {
+            sums[turn][which][team.wave] = value;
+            __syncthreads();
+            value = 0.0f;
+            for (int part = 0; part < a.parts; ++part) {
+                value += sums[turn][which][team.index * a.parts + part];
+            }
+        }
+        return value;
+    };
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * block_rows; base < a.rows;
+         base += step) {
+        const int64_t row = base + team.index * place.rows + place.row;
+        const bool live = row < a.rows;
+        const int hidden = live ? a.hidden : 0;
+        const int64_t first = row * a.hidden;
+        const X* x = static_cast<const X*>(a.x) + row * a.x_stride;
+        const B* branch = static_cast<const B*>(a.branch) + row * a.branch_stride;
+        const int64_t gate_row = live ? factor_row(a.gate, row, a.rows) : 0;
+        const int64_t weight_row = live ? factor_row(a.weight, row, a.rows) : 0;
+        int column[V];
+        Raw<X, N> raw_x[V];
+        Raw<B, N> raw_branch[V];
+        RawAny<N> raw_gate[V];
+        RawAny<N> raw_post[V];
+        RawAny<N> raw_weight[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            column[v] = ((v * a.parts + team.part) * kWave + place.lane) * N;
+            raw_branch[v] = load<kAccess, B, N>(branch, column[v], hidden);
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            raw_x[v] = load<kAccess, X, N>(x, column[v], hidden);
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            raw_gate[v] = load_optional<kAccess, N>(a.gate.data, a.gate.dtype, gate_row, column[v],
+                                                    hidden);
+            if constexpr (kPost) {
+                raw_post[v] = load_any<kAccess, N>(a.branch_weight, a.branch_weight_dtype, 0,
+                                                   column[v], hidden);
+            }
+            raw_weight[v] = load_any<kAccess, N>(a.weight.data, a.weight.dtype, weight_row,
+                                                 column[v], hidden);
+        }
+        float u[V][N];
+        float branch_rstd = 1.0f;
+        float sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            settle<kAccess>(raw_branch[v], column[v], hidden);
+            widen<B, N>(raw_branch[v], u[v]);
+            if constexpr (kPost) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    sum += u[v][e] * u[v][e];
+                }
+            }
+        }
+        if constexpr (kPost) {
+            sum = team_total(row_total<kAccess>(sum, a.row_lanes), 0);
+            branch_rstd = 1.0f / __builtin_sqrtf(sum * a.inv_hidden + a.branch_eps);
+        }
+        X* updated = static_cast<X*>(a.updated) + first;
+        sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float stream[N];
+            float gate[N];
+            settle<kAccess>(raw_x[v], column[v], hidden);
+            widen<X, N>(raw_x[v], stream);
+            widen_optional<kAccess, N>(raw_gate[v], a.gate.data, a.gate.dtype, column[v], hidden,
+                                       1.0f, gate);
+            float post[N];
+            if constexpr (kPost) {
+                widen_any<kAccess, N>(raw_post[v], a.branch_weight_dtype, column[v], hidden, post);
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                float factor = a.branch_scale * gate[e];
+                if constexpr (kPost) {
+                    factor *= post[e];
+                    u[v][e] *= branch_rstd;
+                }
+                u[v][e] = a.residual_scale * stream[e] + factor * u[v][e];
+            }
+            // The norm is taken of the rounded stream, which is what the
+            // backward and the next layer read.
+            const Raw<X, N> rounded = narrow<X, N>(u[v]);
+            store<kAccess, kForwardStores, X, N>(updated, column[v], hidden, rounded);
+            widen<X, N>(rounded, u[v]);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                // Past the row's end the scaled zeros are zeros: nothing is added.
+                sum += u[v][e] * u[v][e];
+            }
+        }
+        sum = team_total(row_total<kAccess>(sum, a.row_lanes), 1);
+        turn ^= 1;
+        const float rstd = 1.0f / __builtin_sqrtf(sum * a.inv_hidden + a.eps);
+        if (a.statistics != nullptr && live && team.part == 0 && place.lane == 0) {
+            a.statistics[row] = rstd;
+            if constexpr (kPost) {
+                a.statistics[a.rows + row] = branch_rstd;
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float weight[N];
+            widen_any<kAccess, N>(raw_weight[v], a.weight.dtype, column[v], hidden, weight);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                u[v][e] = u[v][e] * rstd * weight[e];
+            }
+            store_as<kAccess, kForwardStores, N>(a.normalized, a.output_dtype, first, column[v],
+                                                 hidden, u[v]);
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------
+// Backward: a block's teams walk the rows of a unit, a run of rows of one group;
+// each lane keeps its columns' share of the sums of S and T in registers, the block
+// adds its teams' shares through LDS and writes them to the unit's row of the
+// partials, which sum_units_kernel adds in a fixed order: no atomics, the same bits
+// on every run.
+
+// kToken: the gate has a row for each token, read beside the others; S then holds
+// it as a factor. Otherwise the factors do not depend on the row and stay in
+// registers over a unit's rows.
+
+template <typename X, typename B, int V, bool kPost, bool kToken, Access kAccess>
+__global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArgs a) {
+    constexpr int N = kColumns<X>;
+    extern __shared__ float shares[];  // [teams - 1][hidden], one sum at a time
+    __shared__ float sums[2][3][kMaxParts];
+    const Team team = team_of(a.parts);
+    const Place place = place_of<kAccess>(a.row_lanes);
+    const int block_rows = team.teams * place.rows;
+    int column[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        column[v] = ((v * a.parts + team.part) * kWave + place.lane) * N;
+    }
+    int turn = 0;
+    // Every team of the block makes the same number of turns (barriers inside).
+    for (int64_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+        const int64_t group = unit / a.group_units;
+        const int64_t begin = group * a.group_rows;
+        const int64_t end = begin + a.group_rows;
+        float weight[V][N];
+        float factor[V][N];  // branch_scale * branch_weight, and the gate unless kToken
+        float sum_s[V][N];
+        float sum_t[V][N];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            load_weight<kAccess, N>(
+                row_of(a.weight, factor_row(a.weight, begin, a.rows)), a.weight.dtype, column[v],
+                a.hidden, weight[v]);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                factor[v][e] = a.branch_scale;
+                sum_s[v][e] = 0.0f;
+                sum_t[v][e] = 0.0f;
+            }
+            if constexpr (kPost) {
+                float post[N];
+                load_weight<kAccess, N>(a.branch_weight, a.branch_weight_dtype, column[v],
+                                        a.hidden, post);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    factor[v][e] *= post[e];
+                }
+            }
+            if (!kToken && a.gate.data != nullptr) {
+                float gate[N];
+                load_weight<kAccess, N>(row_of(a.gate, factor_row(a.gate, begin, a.rows)),
+                                        a.gate.dtype, column[v], a.hidden, gate);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    factor[v][e] *= gate[e];
+                }
+            }
+        }
+        const int64_t step = static_cast<int64_t>(a.group_units) * block_rows;
+        for (int64_t base = begin + (unit - group * a.group_units) * block_rows; base < end;
+             base += step) {
+            const int64_t row = base + team.index * place.rows + place.row;
+            const bool live = row < end;
+            const int hidden = live ? a.hidden : 0;
+            const int64_t first = row * a.hidden;
+            Raw<B, N> raw_branch[V];
+            Raw<X, N> raw_u[V];
+            Raw<X, N> raw_grad[V];
+            RawAny<N> raw_gate[V];
+            float upstream[V][N];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                raw_u[v] = load<kAccess, X, N>(static_cast<const X*>(a.updated) + first,
+                                               column[v], hidden);
+                raw_branch[v] = load<kAccess, B, N>(
+                    static_cast<const B*>(a.branch) + row * a.branch_stride, column[v], hidden);
+                raw_grad[v] = Raw<X, N>{};
+                if (a.grad_updated != nullptr) {
+                    raw_grad[v] = load<kAccess, X, N>(static_cast<const X*>(a.grad_updated) + first,
+                                                      column[v], hidden);
+                }
+                if constexpr (kToken) {
+                    raw_gate[v] = load_any<kAccess, N, kOnce>(a.gate.data, a.gate.dtype,
+                                                              row * a.gate.stride, column[v],
+                                                              hidden);
+                }
+            }
+            const float rstd = live ? a.statistics[row] : 0.0f;
+            const float branch_rstd = kPost && live ? a.statistics[a.rows + row] : 1.0f;
+            // Last, since its type is known at run time only and it is waited for in
+            // the branch that loads it.
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (a.grad_normalized != nullptr) {
+                    load_upstream<kAccess, N>(a.grad_normalized, a.grad_dtype, first, column[v],
+                                              hidden, upstream[v]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        upstream[v][e] = 0.0f;
+                    }
+                }
+            }
+            float unit_u[V][N];
+            float unit_branch[V][N];
+            float gradient[V][N];
+            float total[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float gate[N];
+                settle<kAccess>(raw_u[v], column[v], hidden);
+                settle<kAccess>(raw_branch[v], column[v], hidden);
+                settle<kAccess>(raw_grad[v], column[v], hidden);
+                widen<X, N>(raw_u[v], unit_u[v]);
+                widen<B, N>(raw_branch[v], unit_branch[v]);
+                widen<X, N>(raw_grad[v], gradient[v]);
+                if constexpr (kToken && kPost) {
+                    widen_any<kAccess, N>(raw_gate[v], a.gate.dtype, column[v], hidden, gate);
+                }
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    unit_u[v][e] *= rstd;
+                    unit_branch[v][e] *= branch_rstd;
+                    const float product = upstream[v][e] * weight[v][e];
+                    sum_t[v][e] += upstream[v][e] * unit_u[v][e];
+                    gradient[v][e] += rstd * product;
+                    total[0] += product * unit_u[v][e];
+                    if constexpr (kPost) {
+                        float inner = factor[v][e] * unit_branch[v][e];
+                        if constexpr (kToken) {
+                            inner *= gate[e];
+                        }
+                        total[1] += inner * gradient[v][e];
+                        total[2] += inner * unit_u[v][e];
+                    }
+                }
+            }
+            constexpr int kTotals = kPost ? 3 : 1;
+#pragma unroll
+            for (int i = 0; i < kTotals; ++i) {
+                total[i] = row_total<kAccess>(total[i], a.row_lanes);
+            }
+            if (a.parts > 1) {
+                // Two buffers: a team's next turn writes the other one while
+                // slower waves still read this one.
+#pragma unroll
+                for (int i = 0; i < kTotals; ++i) {
+                    sums[turn][i][team.wave] = total[i];
+                }
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < kTotals; ++i) {
+                    total[i] = 0.0f;
+                    for (int part = 0; part < a.parts; ++part) {
+                        total[i] += sums[turn][i][team.index * a.parts + part];
+                    }
+                }
+                turn ^= 1;
+            }
+            const float shared = rstd * (total[0] * a.inv_hidden);
+            const float branch_shared = (total[1] - shared * total[2]) * a.inv_hidden;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float gate[N];
+                float grad_x[N];
+                float grad_branch[N];
+                if constexpr (kToken) {
+                    widen_any<kAccess, N>(raw_gate[v], a.gate.dtype, column[v], hidden, gate);
+                }
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const float g = gradient[v][e] - unit_u[v][e] * shared;
+                    grad_x[e] = a.residual_scale * g;
+                    grad_branch[e] = factor[v][e] * g;
+                    // A team without a row adds nothing, whatever the factors hold.
+                    const float each = live ? g * unit_branch[v][e] : 0.0f;
+                    if constexpr (kToken) {
+                        grad_branch[e] *= gate[e];
+                        sum_s[v][e] += each * gate[e];
+                        gate[e] = each * factor[v][e];  // from here on its gradient
+                    } else {
+                        sum_s[v][e] += each;
+                    }
+                    if constexpr (kPost) {
+                        grad_branch[e] =
+                            branch_rstd * (grad_branch[e] - unit_branch[v][e] * branch_shared);
+                    }
+                }
+                store<kAccess, kBackwardStores, X, N>(static_cast<X*>(a.grad_x) + first, column[v],
+                                                      hidden, narrow<X, N>(grad_x));
+                store<kAccess, kBackwardStores, B, N>(static_cast<B*>(a.grad_branch) + first,
+                                                      column[v], hidden, narrow<B, N>(grad_branch));
+                if (kToken && a.grad_gate != nullptr) {
+                    store_as<kAccess, kBackwardStores, N>(a.grad_gate, a.gate.dtype, first,
+                                                          column[v], hidden, gate);
+                }
+            }
+        }
+        if (a.partials == nullptr) {
+            continue;
+        }
+        int own[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            own[v] = column[v];
+        }
+        if constexpr (kAccess == Access::kLanes) {
+            // The wave's rows first; row 0's lanes stand for all of them.
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                for (int other = a.row_lanes; other < kWave; other *= 2) {
+                    sum_s[0][e] += __shfl_xor(sum_s[0][e], other);
+                    sum_t[0][e] += __shfl_xor(sum_t[0][e], other);
+                }
+            }
+            if (place.row > 0) {
+                own[0] = a.hidden;  // past the end: nothing to leave or to store
+            }
+        }
+        // Teams 1, 2, ... leave their shares; team 0 adds them in that order.
+        float* partial = a.partials + unit * 2 * a.hidden;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            if (team.teams > 1) {
+                __syncthreads();  // the shares left before are read
+            }
+            if (team.index > 0) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        if (own[v] + e < a.hidden) {
+                            shares[(team.index - 1) * a.hidden + own[v] + e] =
+                                which == 0 ? sum_s[v][e] : sum_t[v][e];
+                        }
+                    }
+                }
+            }
+            if (team.teams > 1) {
+                __syncthreads();
+            }
+            if (team.index == 0) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    float sum[N];
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        sum[e] = which == 0 ? sum_s[v][e] : sum_t[v][e];
+                    }
+                    for (int other = 0; other < team.teams - 1; ++other) {
+#pragma unroll
+                        for (int e = 0; e < N; ++e) {
+                            if (own[v] + e < a.hidden) {
+                                sum[e] += shares[other * a.hidden + own[v] + e];
+                            }
+                        }
+                    }
+                    store<kAccess, kBackwardStores, float, N>(
+                        partial + which * a.hidden, own[v], a.hidden, narrow<float, N>(sum));
+                }
+            }
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------
+// Launch shapes (host).
+
+// Units of a backward: runs of rows of one group, together at most as many as
+// the blocks of rms_device.h's walk, but at least one for each group.
+struct Units {
+    int64_t groups;
+    int64_t group_rows;
+    int64_t group_units;
+    int64_t count;
+};
+
+// The norm's shape (rms_device.h), but one slot as long as sixteen waves hold a
+// row: the sums and factors of two slots of a 16-bit stream do not fit the registers.
+inline Shape walk_shape(int64_t hidden, int x_dtype) {
+    const Shape shape = backward_shape(hidden, x_dtype);
+    const int64_t vectors = wave_vectors(hidden, x_dtype);
+    return shape.slots > 1 && vectors <= kMaxParts ? shape_of(vectors, 1, 8) : shape;
+}
+
+inline Units units_of(int64_t rows, int64_t group_rows, const Shape& shape) {
+    Units units;
+    units.group_rows = group_rows;
+    units.groups = rows / group_rows;
+    const int64_t most = shape.threads <= 10 * kWave ? 2 * kComputeUnits : kComputeUnits;
+    const int64_t wanted = blocks_of(group_rows, shape);
+    const int64_t each = most / units.groups > 0 ? most / units.groups : 1;
+    units.group_units = wanted < each ? wanted : each;
+    units.count = units.groups * units.group_units;
+    return units;
+}
+
+// Defined in gated_kernels.hip, one translation unit per stream type and pass.
+template <typename X>
+int launch_forward(const ForwardArgs& a, const Shape& shape, int branch_dtype, hipStream_t stream);
+template <typename X>
+int launch_backward(const BackwardArgs& a, const Shape& shape, int branch_dtype,
+                    hipStream_t stream);
+
+}  // namespace gated
+}  // namespace rln
+
+#endif  // GATED_DEVICE_H

@@ -667,6 +667,8 @@ std::optional<torch::autograd::variable_list> residual_layer_norm_if_supported(
 PYBIND11_MODULE(_C, module) {
     module.doc() = "MI355X (gfx950) fused residual + dropout + LayerNorm, residual + RMSNorm";
     bind_rms(module);
+    bind_gated(module);
+    bind_rotary(module);
     module.def(
         "residual_layer_norm",
         &residual_layer_norm_autograd,

@@ -1,5 +1,5 @@
-// Shared by the torch glue of the C ABI (rln_torch.cpp, rms_torch.cpp): status
-// to exception, element types, and allocation.
+// Shared by the torch glue of the C ABI (rln_torch.cpp, rms_torch.cpp, gated_torch.cpp,
+// rotary_torch.cpp): status to exception, element types, and allocation.
 #ifndef RLN_TORCH_H
 #define RLN_TORCH_H
 
@@ -111,7 +111,9 @@ inline at::Tensor empty_device_like(const at::Tensor& like, at::ScalarType type)
 
 }  // namespace rln_glue
 
-// The entry points of rms_torch.cpp.
+// The entry points of rms_torch.cpp, gated_torch.cpp and rotary_torch.cpp.
 void bind_rms(pybind11::module_& module);
+void bind_gated(pybind11::module_& module);
+void bind_rotary(pybind11::module_& module);
 
 #endif  // RLN_TORCH_H

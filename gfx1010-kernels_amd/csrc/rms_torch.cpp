@@ -15,16 +15,14 @@
 // the caller: tensor allocation, row strides, the device guard and the current
 // stream.
 
-#include "rln_torch.h"
+#include "rows_torch.h"
 
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/dynamo/compiled_autograd.h>
 
-#include <ATen/NamedTensorUtils.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
 #include <memory>
 #include <mutex>
@@ -38,38 +36,6 @@ using namespace rln_glue;
 namespace {
 
 constexpr int64_t kCheckpointGroup = 128;
-
-// The one step between consecutive rows of `tensor` seen as [rows, hidden], or
-// nullopt where its leading dimensions are no single run of rows or the elements
-// of a row are apart.
-std::optional<int64_t> row_stride(const at::Tensor& tensor) {
-    const int64_t dims = tensor.dim();
-    if (tensor.size(-1) != 1 && tensor.stride(-1) != 1) {
-        return std::nullopt;
-    }
-    int64_t stride = tensor.size(-1);
-    int64_t next = -1;  // the step that the dimension outside has to have
-    for (int64_t i = dims - 2; i >= 0; --i) {
-        if (tensor.size(i) == 1) {
-            continue;
-        }
-        if (next < 0) {
-            stride = tensor.stride(i);
-        } else if (tensor.stride(i) != next) {
-            return std::nullopt;
-        }
-        next = tensor.stride(i) * tensor.size(i);
-    }
-    return stride;
-}
-
-// `tensor` with rows of consecutive elements one stride apart, copied only
-// where it has none.
-at::Tensor as_rows(const at::Tensor& tensor, int64_t* stride) {
-    const auto found = row_stride(tensor);
-    *stride = found.value_or(tensor.size(-1));
-    return found ? tensor : tensor.contiguous();
-}
 
 void check_inputs(const at::Tensor& x, const at::Tensor& branch, const at::Tensor& weight,
                   double eps) {
@@ -94,19 +60,6 @@ void check_inputs(const at::Tensor& x, const at::Tensor& branch, const at::Tenso
     TORCH_CHECK(eps >= 0.0, "eps must not be negative");
 }
 
-// Dense outputs in x's shape, with its dimension names; of a contiguous x
-// whatever else empty_device_like takes over.
-at::Tensor output_like(const at::Tensor& x, at::ScalarType type) {
-    if (x.is_contiguous()) {
-        return empty_device_like(x, type);
-    }
-    auto output = empty_device(x.sizes(), type, x.device());
-    if (x.has_names()) {
-        at::namedinference::propagate_names(output, x);
-    }
-    return output;
-}
-
 // What a recorded forward keeps beside (or, with the checkpoint, in the place
 // of) `updated`, in one allocation of bytes: rstd, the checkpoint's scales and
 // its codes, each 256-byte aligned.
@@ -124,10 +77,6 @@ State state_layout(int64_t rows, int64_t hidden, bool checkpoint) {
     state.codes = state.scale + (checkpoint ? aligned(4 * rows * groups) : 0);
     state.bytes = checkpoint ? state.codes + rows * hidden : 4 * rows;
     return state;
-}
-
-hipStream_t stream_of(const at::Tensor& x) {
-    return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index()).stream();
 }
 
 // updated is undefined without a branch; state, when given, receives what the

@@ -43,6 +43,60 @@ class RlnPhilox(ctypes.Structure):
     ]
 
 
+class RlnFactor(ctypes.Structure):
+    """``rln_factor_t``: rows of factors, each shared by ``rows`` rows of the stream."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("stride", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+    ]
+
+
+class RlnHeads(ctypes.Structure):
+    """``rln_heads_t``: heads [outer, inner, heads, size] by strides in elements."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("outer_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class RlnRotary(ctypes.Structure):
+    """``rln_rotary_t``: positions and the pairs they turn."""
+
+    _fields_ = [
+        ("positions", ctypes.c_void_p),
+        ("positions_type", ctypes.c_int),
+        ("axis_stride", ctypes.c_int64),
+        ("outer_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("frequencies", ctypes.c_void_p),
+        ("wide_frequencies", ctypes.c_int),
+        ("axis_of_pair", ctypes.POINTER(ctypes.c_uint8)),
+        ("axes", ctypes.c_int64),
+        ("pairs", ctypes.c_int64),
+        ("interleaved", ctypes.c_int),
+    ]
+
+
+class RlnRotarySide(ctypes.Structure):
+    """``rln_rotary_side_t``: one of the two tensors of heads of a call."""
+
+    _fields_ = [
+        ("heads", RlnHeads),
+        ("grad", RlnHeads),
+        ("count", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("weight_dtype", ctypes.c_int),
+        ("output", ctypes.c_void_p),
+        ("grad_weight", ctypes.c_void_p),
+    ]
+
+
 class RlnError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(message)
@@ -51,6 +105,8 @@ class RlnError(RuntimeError):
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
+_FACTOR = ctypes.POINTER(RlnFactor)
+_SIDE = ctypes.POINTER(RlnRotarySide)
 
 # name -> (restype, argtypes), in declaration order of include/rln.h.
 SIGNATURES = {
@@ -95,6 +151,32 @@ SIGNATURES = {
         [_P, ctypes.c_int, _P, _I64, _P, ctypes.c_int, _I64, _I64, _P],
     ),
     "rln_rms_hidden_supported": (ctypes.c_int, [_I64]),
+    "rln_gated_forward": (
+        ctypes.c_int,
+        [_P, ctypes.c_int, _I64, _P, ctypes.c_int, _I64, _P, ctypes.c_int, _FACTOR, _FACTOR, _P,
+         _P, ctypes.c_int, _P, _I64, _I64, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+         ctypes.c_double, _P],
+    ),
+    "rln_gated_backward": (
+        ctypes.c_int,
+        [_P, _P, ctypes.c_int, _P, ctypes.c_int, _P, ctypes.c_int, _I64, _P, ctypes.c_int, _FACTOR,
+         _FACTOR, _P, _P, _P, _P, _P, _P, _I64, _I64, ctypes.c_double, ctypes.c_double, _P,
+         ctypes.c_size_t, _P],
+    ),
+    "rln_gated_backward_workspace_bytes": (
+        ctypes.c_size_t, [_I64, _I64, ctypes.c_int, _I64, _I64]),
+    "rln_rotary_forward": (
+        ctypes.c_int,
+        [_SIDE, _SIDE, ctypes.c_int, ctypes.POINTER(RlnRotary), _I64, _I64, _I64, ctypes.c_double,
+         _P],
+    ),
+    "rln_rotary_backward": (
+        ctypes.c_int,
+        [_SIDE, _SIDE, ctypes.c_int, ctypes.POINTER(RlnRotary), _I64, _I64, _I64, ctypes.c_double,
+         _P, ctypes.c_size_t, _P],
+    ),
+    "rln_rotary_backward_workspace_bytes": (
+        ctypes.c_size_t, [_I64, _I64, _I64, _I64, _I64, _I64, ctypes.c_int]),
     "rln_last_error": (ctypes.c_char_p, []),
     "rln_target_arch": (ctypes.c_char_p, []),
     "rln_version": (ctypes.c_char_p, []),

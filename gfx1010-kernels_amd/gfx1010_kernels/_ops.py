@@ -30,13 +30,18 @@ fused op instead of breaking around it (the reference does not support
 * ``gfx1010_kernels::rms_forward`` / ``rms_backward`` / ``rms_quantized`` /
   ``dequantize`` do the same for the root-mean-square norm
   (``_C.residual_rms_norm_*``). They draw nothing, so equal calls may be merged.
+* ``gfx1010_kernels::gated_forward`` / ``gated_backward`` and ``rotary_forward`` /
+  ``rotary_backward`` do so for the gated residual norm and the rotary norm of heads
+  (``_C.gated_residual_rms_norm_*``, ``_C.rms_norm_rotary_*``); ``needed`` has bit ``i``
+  set where the gradient of tensor input ``i`` is asked for, and an output that is
+  not asked for, or does not exist, is empty.
 
 ``torch.jit.trace`` and ``make_fx`` record these operators as well.
 """
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 from torch import Tensor
@@ -336,9 +341,219 @@ def dequantize_op(quantized, scale, group_size, dtype):
     return dequantize(quantized, scale, group_size or 0, dtype)
 
 
+def _or_empty(tensor, like):
+    """``tensor``, or an empty one: an operator returns every output."""
+    return like.new_empty((0,)) if tensor is None else tensor
+
+
+@torch.library.custom_op(f"{_NAMESPACE}::gated_forward", mutates_args=(), device_types="cuda")
+def gated_forward(
+    x: Tensor,
+    branch: Tensor,
+    weight: Tensor,
+    branch_weight: Optional[Tensor],
+    gate: Optional[Tensor],
+    eps: float,
+    branch_eps: float,
+    residual_scale: float,
+    branch_scale: float,
+    normalized_dtype: Optional[torch.dtype] = None,
+) -> tuple[Tensor, Tensor, Tensor]:
+    return _native().gated_residual_rms_norm_forward(
+        x, branch, weight, branch_weight, gate, float(eps), float(branch_eps),
+        float(residual_scale), float(branch_scale), normalized_dtype)
+
+
+@gated_forward.register_fake
+def _gated_forward_fake(x, branch, weight, branch_weight, gate, eps, branch_eps, residual_scale,
+                        branch_scale, normalized_dtype=None):
+    rows = x.numel() // x.shape[-1]
+    return (
+        x.new_empty(x.shape),
+        x.new_empty(x.shape, dtype=normalized_dtype or x.dtype),
+        x.new_empty((rows if branch_weight is None else 2 * rows,), dtype=torch.float32),
+    )
+
+
+@torch.library.custom_op(f"{_NAMESPACE}::gated_backward", mutates_args=(), device_types="cuda")
+def gated_backward(
+    grad_updated: Optional[Tensor],
+    grad_normalized: Optional[Tensor],
+    updated: Tensor,
+    branch: Tensor,
+    weight: Tensor,
+    branch_weight: Optional[Tensor],
+    gate: Optional[Tensor],
+    statistics: Tensor,
+    residual_scale: float,
+    branch_scale: float,
+    needed: int,
+) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    gradients = _native().gated_residual_rms_norm_backward(
+        grad_updated, grad_normalized, updated, branch, weight, branch_weight, gate, statistics,
+        float(residual_scale), float(branch_scale), needed)
+    return tuple(_or_empty(gradient, updated) for gradient in gradients)
+
+
+@gated_backward.register_fake
+def _gated_backward_fake(grad_updated, grad_normalized, updated, branch, weight, branch_weight,
+                         gate, statistics, residual_scale, branch_scale, needed):
+    def like(tensor, wanted):
+        if not wanted or tensor is None:
+            return updated.new_empty((0,))
+        return tensor.new_empty(tensor.shape)
+
+    return (
+        updated.new_empty(updated.shape),
+        branch.new_empty(branch.shape),
+        like(weight, needed >> 2 & 1 and grad_normalized is not None),
+        like(branch_weight, needed >> 3 & 1),
+        like(gate, needed >> 4 & 1),
+    )
+
+
+def _needed(flags):
+    return sum(1 << index for index, flag in enumerate(flags) if flag)
+
+
+def _gated_setup_context(ctx, inputs, output):
+    _, branch, weight, branch_weight, gate, _, _, ctx.residual_scale, ctx.branch_scale, _ = inputs
+    updated, _, statistics = output
+    ctx.save_for_backward(updated, branch, weight, branch_weight, gate, statistics)
+    ctx.mark_non_differentiable(statistics)
+    ctx.set_materialize_grads(False)
+
+
+def _gated_backward_formula(ctx, grad_updated, grad_normalized, _grad_statistics):
+    grads = [None] * 10
+    if grad_updated is None and grad_normalized is None:
+        return tuple(grads)
+    needed = _needed(ctx.needs_input_grad[:5])
+    if grad_normalized is None:
+        needed &= ~4
+    gradients = gated_backward(grad_updated, grad_normalized, *ctx.saved_tensors,
+                               ctx.residual_scale, ctx.branch_scale, needed)
+    for index in range(5):
+        if needed >> index & 1:
+            grads[index] = gradients[index]
+    return tuple(grads)
+
+
+gated_forward.register_autograd(_gated_backward_formula, setup_context=_gated_setup_context)
+
+
+def gated_residual_rms_norm_op(*args):
+    """``(updated, normalized)`` through the registered custom op."""
+    updated, normalized, _ = gated_forward(*args)
+    return updated, normalized
+
+
+@torch.library.custom_op(f"{_NAMESPACE}::rotary_forward", mutates_args=(), device_types="cuda")
+def rotary_forward(
+    q: Tensor,
+    k: Optional[Tensor],
+    positions: Tensor,
+    inverse_frequencies: Tensor,
+    sections: Sequence[int],
+    cyclic: bool,
+    interleaved: bool,
+    q_weight: Optional[Tensor],
+    k_weight: Optional[Tensor],
+    eps: float,
+) -> tuple[Tensor, Tensor]:
+    return _native().rms_norm_rotary_forward(
+        q, k, positions, inverse_frequencies, list(sections), cyclic, interleaved, q_weight,
+        k_weight, float(eps))
+
+
+@rotary_forward.register_fake
+def _rotary_forward_fake(q, k, positions, inverse_frequencies, sections, cyclic, interleaved,
+                         q_weight, k_weight, eps):
+    return q.new_empty(q.shape), q.new_empty((0,) if k is None else k.shape)
+
+
+@torch.library.custom_op(f"{_NAMESPACE}::rotary_backward", mutates_args=(), device_types="cuda")
+def rotary_backward(
+    grad_q: Optional[Tensor],
+    grad_k: Optional[Tensor],
+    q: Optional[Tensor],
+    k: Optional[Tensor],
+    positions: Tensor,
+    inverse_frequencies: Tensor,
+    sections: Sequence[int],
+    cyclic: bool,
+    interleaved: bool,
+    q_weight: Optional[Tensor],
+    k_weight: Optional[Tensor],
+    eps: float,
+    needed: int,
+) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    gradients = _native().rms_norm_rotary_backward(
+        grad_q, grad_k, q, k, positions, inverse_frequencies, list(sections), cyclic, interleaved,
+        q_weight, k_weight, float(eps), needed)
+    like = grad_k if grad_q is None else grad_q
+    return tuple(_or_empty(gradient, like) for gradient in gradients)
+
+
+@rotary_backward.register_fake
+def _rotary_backward_fake(grad_q, grad_k, q, k, positions, inverse_frequencies, sections, cyclic,
+                          interleaved, q_weight, k_weight, eps, needed):
+    base = grad_k if grad_q is None else grad_q
+
+    def like(tensor, wanted=True):
+        if tensor is None or not wanted:
+            return base.new_empty((0,))
+        return tensor.new_empty(tensor.shape)
+
+    return (like(grad_q), like(grad_k),
+            like(q_weight, grad_q is not None and needed >> 2 & 1),
+            like(k_weight, grad_k is not None and needed >> 3 & 1))
+
+
+def _rotary_setup_context(ctx, inputs, output):
+    (q, k, positions, frequencies, ctx.sections, ctx.cyclic, ctx.interleaved, q_weight, k_weight,
+     ctx.eps) = inputs
+    ctx.save_for_backward(None if q_weight is None else q, None if k_weight is None else k,
+                          positions, frequencies, q_weight, k_weight)
+    ctx.has_k = k is not None
+    if k is None:
+        ctx.mark_non_differentiable(output[1])
+    ctx.set_materialize_grads(False)
+
+
+def _rotary_backward_formula(ctx, grad_q, grad_k):
+    grads = [None] * 10
+    if not ctx.has_k:
+        grad_k = None
+    if grad_q is None and grad_k is None:
+        return tuple(grads)
+    q, k, positions, frequencies, q_weight, k_weight = ctx.saved_tensors
+    places = (0, 1, 7, 8)
+    needed = _needed(ctx.needs_input_grad[place] for place in places)
+    needed &= ~((0 if grad_q is not None else 5) | (0 if grad_k is not None else 10))
+    gradients = rotary_backward(grad_q, grad_k, q, k, positions, frequencies, ctx.sections,
+                                ctx.cyclic, ctx.interleaved, q_weight, k_weight, ctx.eps, needed)
+    for index, place in enumerate(places):
+        if needed >> index & 1:
+            grads[place] = gradients[index]
+    return tuple(grads)
+
+
+rotary_forward.register_autograd(_rotary_backward_formula, setup_context=_rotary_setup_context)
+
+
+def rms_norm_rotary_op(q, k, *args):
+    """``(q, k)`` through the registered custom op."""
+    q_out, k_out = rotary_forward(q, k, *args)
+    return q_out, None if k is None else k_out
+
+
 __all__ = [
     "dequantize",
     "dequantize_op",
+    "gated_backward",
+    "gated_forward",
+    "gated_residual_rms_norm_op",
     "residual_layer_norm_op",
     "residual_rms_norm_op",
     "residual_rms_norm_quantized_op",
@@ -346,5 +561,8 @@ __all__ = [
     "rln_forward",
     "rms_backward",
     "rms_forward",
+    "rms_norm_rotary_op",
     "rms_quantized",
+    "rotary_backward",
+    "rotary_forward",
 ]

@@ -17,7 +17,9 @@ This module is that recipe as code:
   block's ``ln_1`` after its MLP, and the final norm after the last MLP. Only
   the first ``ln_1`` (no residual add before it) runs as a plain LayerNorm.
 
-Both take ``nn.RMSNorm`` modules as well, through ``residual_rms_norm``.
+Both take ``nn.RMSNorm`` modules as well, through ``residual_rms_norm``, and then
+blocks that norm their sublayers' outputs too, gate them or scale the residual,
+through ``gated_residual_rms_norm``.
 
 Neither function owns parameters: they read the caller's modules, so a model
 that switches its ``forward`` to them keeps its ``state_dict`` unchanged.
@@ -25,12 +27,13 @@ that switches its ``forward`` to them keeps its ``state_dict`` unchanged.
 
 from __future__ import annotations
 
-from typing import Callable, Sequence, Union
+from typing import Callable, Optional, Sequence, Union
 
 import torch
 from torch import nn
 from torch.nn import functional as F
 
+from .gated_norm import gated_residual_rms_norm
 from .normalization import residual_layer_norm
 from .rms_norm import residual_rms_norm
 
@@ -75,18 +78,45 @@ def _refuse_checkpoint(checkpoint_dtype) -> None:
         raise ValueError("checkpoint_dtype needs torch.nn.RMSNorm modules")
 
 
+def _gated_norm(x, branch, norm, branch_norm, gate, residual_scale, branch_scale, dropout_p,
+                training, implementation, normalized_dtype, checkpoint_dtype):
+    if not isinstance(norm, nn.RMSNorm) or not isinstance(branch_norm, (nn.RMSNorm, type(None))):
+        raise TypeError("branch_norm, gate and scales need torch.nn.RMSNorm modules")
+    if checkpoint_dtype is not None:
+        raise ValueError("checkpoint_dtype does not go with branch_norm, gate or scales")
+    if branch_norm is not None:
+        _check_norm(branch_norm, x.shape[-1])
+    if training and dropout_p != 0.0:
+        branch = F.dropout(branch, dropout_p, True)
+    return gated_residual_rms_norm(
+        x, branch, norm.weight, _rms_eps(norm, x.dtype),
+        branch_weight=None if branch_norm is None else branch_norm.weight,
+        branch_eps=None if branch_norm is None else _rms_eps(branch_norm, branch.dtype),
+        gate=gate, residual_scale=residual_scale, branch_scale=branch_scale,
+        implementation=implementation, normalized_dtype=normalized_dtype)
+
+
 def residual_norm(x, branch, norm: Union[nn.LayerNorm, nn.RMSNorm], dropout_p: float = 0.0,
                   training: bool = True, *, implementation: str = "auto", normalized_dtype=None,
-                  checkpoint_dtype=None):
+                  checkpoint_dtype=None, branch_norm: Optional[nn.RMSNorm] = None, gate=None,
+                  residual_scale: float = 1.0, branch_scale: float = 1.0):
     """``x + dropout(branch)`` followed by ``norm``, as one fused operation.
 
     Returns ``(updated, normalized)`` like ``residual_layer_norm``, or like
     ``residual_rms_norm`` for an ``nn.RMSNorm`` (whose dropout, if any, is a
     separate ``F.dropout``); ``norm`` supplies weight, bias and eps and keeps its
     parameters (and their ``state_dict`` keys) in the caller's model.
-    ``checkpoint_dtype`` is ``residual_rms_norm``'s.
+    ``checkpoint_dtype`` is ``residual_rms_norm``'s. With an ``nn.RMSNorm``, ``branch_norm``
+    (another one, of the branch), ``gate`` and the scales are
+    ``gated_residual_rms_norm``'s: ``residual_scale * x + branch_scale * gate *
+    branch_norm(dropout(branch))`` and its norm.
     """
     _check_norm(norm, x.shape[-1])
+    if (branch_norm is not None or gate is not None or residual_scale != 1.0
+            or branch_scale != 1.0):
+        return _gated_norm(x, branch, norm, branch_norm, gate, residual_scale, branch_scale,
+                           dropout_p, training, implementation, normalized_dtype,
+                           checkpoint_dtype)
     if isinstance(norm, nn.RMSNorm):
         return _rms_norm(x, branch, norm, dropout_p, training, implementation, normalized_dtype,
                          checkpoint_dtype)
@@ -120,6 +150,12 @@ def prenorm_forward(
     implementation: str = "auto",
     normalized_dtype=None,
     checkpoint_dtype=None,
+    post_ln1: Optional[Accessor] = None,
+    post_ln2: Optional[Accessor] = None,
+    gate1: Optional[Accessor] = None,
+    gate2: Optional[Accessor] = None,
+    residual_scale: float = 1.0,
+    branch_scale: float = 1.0,
 ):
     """Run pre-norm blocks with fused residual LayerNorms; returns ``(x, out)``.
 
@@ -138,6 +174,12 @@ def prenorm_forward(
     outputs' without ``normalized_dtype``, and ``checkpoint_dtype=torch.int8``
     keeps each norm's input for the backward in 8 bits
     (``residual_rms_norm``), so that no norm keeps the stream itself alive.
+
+    Blocks of ``nn.RMSNorm`` modules may also norm what their sublayers return
+    (``post_ln1`` after the attention, ``post_ln2`` after the MLP), gate it (``gate1``,
+    ``gate2``: tensors that ``gated_residual_rms_norm`` takes, by name or function, such as
+    ``lambda block: block.gate.tanh()``) and scale the sum (``residual_scale``,
+    ``branch_scale``).
     """
     if len(blocks) == 0:
         raise ValueError("prenorm_forward needs at least one block")
@@ -153,12 +195,21 @@ def prenorm_forward(
         normalized = F.layer_norm(x, (hidden,), first.weight, first.bias, first.eps)
         if normalized_dtype is not None:
             normalized = normalized.to(normalized_dtype)
+    options.update(residual_scale=residual_scale, branch_scale=branch_scale)
+
+    def own(block, branch_norm, gate):
+        """The block's parts around one of its additions."""
+        return dict(branch_norm=None if branch_norm is None else _module(block, branch_norm),
+                    gate=None if gate is None else _module(block, gate))
+
     for index, block in enumerate(blocks):
         x, normalized = residual_norm(x, _sublayer(block, attention, normalized),
-                                      _module(block, ln2), dropout_p, training, **options)
+                                      _module(block, ln2), dropout_p, training,
+                                      **own(block, post_ln1, gate1), **options)
         following = _module(blocks[index + 1], ln1) if index + 1 < len(blocks) else final_norm
         x, normalized = residual_norm(x, _sublayer(block, mlp, normalized), following,
-                                      dropout_p, training, **options)
+                                      dropout_p, training, **own(block, post_ln2, gate2),
+                                      **options)
     return x, normalized
 
 

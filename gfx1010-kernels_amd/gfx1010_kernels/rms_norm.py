@@ -172,30 +172,31 @@ def _traced_inputs_served(x, branch, weight, eps):
     return _input_reason(x, branch, weight, eps) is None
 
 
-def _check_implementation(implementation):
+def _check_implementation(implementation, what="residual RMSNorm"):
     if implementation not in IMPLEMENTATIONS:
         raise ValueError(
             "implementation must be 'auto', 'gfx950', 'gfx1010', 'triton' or 'torch'")
     if implementation == "triton":
         raise RuntimeError(
-            f"{TARGET_ARCHITECTURE} residual RMSNorm is unavailable: "
+            f"{TARGET_ARCHITECTURE} {what} is unavailable: "
             "the Triton backend is not part of the MI355X build")
 
 
-def _native_or_reason(tensor, reason_of, implementation):
+def _native_or_reason(tensor, reason_of, implementation, what="residual RMSNorm"):
     """The native extension, or None and why ``"auto"`` falls back (the answer of
     ``reason_of()``, which the strict modes do not ask); the strict modes and a
     broken install on the target hardware raise."""
     strict = implementation in _STRICT_NATIVE
+    unavailable = f"{TARGET_ARCHITECTURE} native {what} is unavailable"
     reason = None if strict else reason_of()
     if strict and not tensor.is_cuda:
-        raise RuntimeError(f"{_UNAVAILABLE}: the inputs must be HIP tensors")
+        raise RuntimeError(f"{unavailable}: the inputs must be HIP tensors")
     if reason is None:
         if tensor.get_device() not in _READY_DEVICES:
             status = residual_layer_norm_status(tensor.device)
             if not status.available:
                 if strict or status.architecture == TARGET_ARCHITECTURE:
-                    raise RuntimeError(f"{_UNAVAILABLE}: {status.reason}")
+                    raise RuntimeError(f"{unavailable}: {status.reason}")
                 return None, status.reason
             _READY_DEVICES.add(tensor.get_device())
         # What the strict modes cannot serve raises in the extension.
@@ -203,9 +204,9 @@ def _native_or_reason(tensor, reason_of, implementation):
     return None, reason
 
 
-def _warn(reason):
+def _warn(reason, what="residual RMSNorm"):
     warnings.warn(
-        f"{TARGET_ARCHITECTURE} native residual RMSNorm was not used: {reason}",
+        f"{TARGET_ARCHITECTURE} native {what} was not used: {reason}",
         RuntimeWarning,
         stacklevel=3,
     )

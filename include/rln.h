@@ -411,6 +411,230 @@ int rln_dequantize(
  * else 0 (no counterpart in the reference). */
 int rln_rms_hidden_supported(int64_t hidden);
 
+/*
+ * Gated residual norm (rln_gated_*). It has no counterpart in the reference. Per
+ * row of `hidden` elements, with gate and weight rows of as many:
+ *
+ *   a          = branch * branch_rstd * branch_weight,
+ *                branch_rstd = 1 / sqrt(sum(branch^2) / hidden + branch_eps);
+ *                a = branch where branch_weight is NULL
+ *   updated    = residual_scale * x + branch_scale * gate * a
+ *   rstd       = 1 / sqrt(sum(updated^2) / hidden + eps)     (of the rounded stream)
+ *   normalized = updated * rstd * weight
+ *
+ * computed in fp32 and rounded once to the outputs' types. x, branch,
+ * branch_weight, gate, weight and normalized each use fp32, fp16 or bf16; updated
+ * has x's type.
+ */
+
+/* Rows of factors that repeat over the stream: row r of the stream takes row
+ * r / rows of `data`, whose rows of consecutive elements are `stride` elements
+ * apart. `rows` divides the number of the stream's rows: all of them for one row of
+ * factors, 1 for one each. data is NULL for factors of one (of a gate). */
+typedef struct rln_factor_t {
+    const void* data;
+    int dtype;
+    int64_t stride;
+    int64_t rows;
+} rln_factor_t;
+
+/*
+ * Forward (no counterpart in the reference). x and branch are rows of consecutive
+ * elements, `x_stride` and `branch_stride` elements apart (any value); branch_weight
+ * is one row; updated and normalized are dense. No output may overlap an input.
+ * Every address is aligned to its elements; more is not asked. gate may be NULL,
+ * weight may not. Where gate and weight both repeat over some of the rows, they
+ * repeat over the same. statistics: fp32 [2 * rows] for the backward (rstd, then
+ * branch_rstd with a branch_weight), or NULL. Any hidden from 1 to 16384.
+ */
+int rln_gated_forward(
+    const void* x,
+    int x_dtype,
+    int64_t x_stride,
+    const void* branch,
+    int branch_dtype,
+    int64_t branch_stride,
+    const void* branch_weight,
+    int branch_weight_dtype,
+    const rln_factor_t* gate,
+    const rln_factor_t* weight,
+    void* updated,
+    void* normalized,
+    int normalized_dtype,
+    float* statistics,
+    int64_t rows,
+    int64_t hidden,
+    double residual_scale,
+    double branch_scale,
+    double eps,
+    double branch_eps,
+    void* stream);
+
+/*
+ * Backward of rln_gated_forward (no counterpart in the reference). Per row, with
+ * c = branch_scale * gate * branch_weight, v = updated * rstd, b = branch * branch_rstd:
+ *
+ *   p           = grad_normalized * weight
+ *   g           = grad_updated + rstd * (p - v * sum(p * v) / hidden)
+ *   grad_x      = residual_scale * g
+ *   grad_branch = branch_rstd * (c * g - b * sum(c * g * b) / hidden), or c * g
+ *                 without a branch_weight
+ *   grad_gate   = branch_scale * branch_weight * g * b, grad_branch_weight =
+ *                 branch_scale * gate * g * b, grad_weight = grad_normalized * v,
+ *                 each summed in fp32 over the rows that share the factor, in a
+ *                 fixed order (bitwise reproducible)
+ *
+ * grad_updated (x's type) and grad_normalized may be NULL, meaning zero. Gradients
+ * are dense, in the types of what they belong to (grad_gate and grad_weight with a
+ * row for each row of factors); updated is dense. grad_gate, grad_branch_weight and
+ * grad_weight may each be NULL. No output may overlap an input. workspace: device
+ * scratch of rln_gated_backward_workspace_bytes bytes, aligned to 4 (unused, may be
+ * NULL, where none of the three is asked for, or grad_gate alone of a gate with a
+ * row each); nothing in it needs clearing, and calls that overlap need one each.
+ */
+int rln_gated_backward(
+    const void* grad_updated,
+    const void* grad_normalized,
+    int grad_normalized_dtype,
+    const void* updated,
+    int x_dtype,
+    const void* branch,
+    int branch_dtype,
+    int64_t branch_stride,
+    const void* branch_weight,
+    int branch_weight_dtype,
+    const rln_factor_t* gate,
+    const rln_factor_t* weight,
+    const float* statistics,
+    void* grad_x,
+    void* grad_branch,
+    void* grad_gate,
+    void* grad_branch_weight,
+    void* grad_weight,
+    int64_t rows,
+    int64_t hidden,
+    double residual_scale,
+    double branch_scale,
+    void* workspace,
+    size_t workspace_bytes,
+    void* stream);
+
+/* Workspace bytes rln_gated_backward needs for its sums (no counterpart in the
+ * reference). gate_rows and weight_rows are the factors' `rows`; without a gate,
+ * gate_rows is `rows`. */
+size_t rln_gated_backward_workspace_bytes(
+    int64_t rows,
+    int64_t hidden,
+    int x_dtype,
+    int64_t gate_rows,
+    int64_t weight_rows);
+
+/*
+ * Rotary positions of query and key heads, with the root-mean-square norm of each
+ * head in front (rln_rotary_*; no counterpart in the reference). Per head h of
+ * `size` elements of a token:
+ *
+ *   n = h * rstd * weight, rstd = 1 / sqrt(sum(h^2) / size + eps); n = h without a weight
+ *   pair i of n turns by positions[axis i] * frequencies[i], an angle taken in fp64:
+ *   (n1, n2) -> (n1 * cos - n2 * sin, n1 * sin + n2 * cos)
+ *
+ * where pair i is elements (i, i + pairs) of the head, or (2i, 2i + 1) with
+ * `interleaved`; elements from 2 * pairs on are not turned. Computed in fp32,
+ * rounded once to the heads' type (fp32, fp16 or bf16, that of all heads of a call).
+ */
+
+#define RLN_POSITIONS_I64 0
+#define RLN_POSITIONS_I32 1
+#define RLN_POSITIONS_F32 2
+
+/* Heads [outer, inner, heads, size] with consecutive elements, strides in elements
+ * (any values). data is NULL where there are none. */
+typedef struct rln_heads_t {
+    const void* data;
+    int64_t outer_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+} rln_heads_t;
+
+/* Positions [axes, outer, inner] by strides in elements, and the pairs they turn.
+ * `axis_of_pair`: host memory, `pairs` values below `axes`, or NULL for axis 0. */
+typedef struct rln_rotary_t {
+    const void* positions;
+    int positions_type;      /* RLN_POSITIONS_* */
+    int64_t axis_stride;
+    int64_t outer_stride;
+    int64_t token_stride;
+    const void* frequencies; /* fp32, or fp64 with wide_frequencies */
+    int wide_frequencies;
+    const uint8_t* axis_of_pair;
+    int64_t axes;            /* 1 to 4 */
+    int64_t pairs;           /* 2 * pairs <= size */
+    int interleaved;
+} rln_rotary_t;
+
+/* One of the two tensors of heads of a call, q or k. */
+typedef struct rln_rotary_side_t {
+    rln_heads_t heads;       /* the forward's input */
+    rln_heads_t grad;        /* backward: the gradient of its output */
+    int64_t count;           /* heads per token; 0 for no such tensor */
+    const void* weight;      /* [size], or NULL for heads without a norm */
+    int weight_dtype;
+    void* output;            /* dense: the turned heads, or the gradient of `heads` */
+    void* grad_weight;       /* backward: [size] in the weight's type, or NULL */
+} rln_rotary_side_t;
+
+/*
+ * Forward, of outer * inner tokens (no counterpart in the reference): q->output and
+ * k->output from q->heads and k->heads. size is 1 to 256, and outer * inner and the
+ * number of heads fit 31 bits. No output may overlap an input.
+ */
+int rln_rotary_forward(
+    const rln_rotary_side_t* q,
+    const rln_rotary_side_t* k,
+    int dtype,
+    const rln_rotary_t* rotary,
+    int64_t outer,
+    int64_t inner,
+    int64_t size,
+    double eps,
+    void* stream);
+
+/*
+ * Backward (no counterpart in the reference): q->output and k->output are the
+ * gradients of q->heads and k->heads, from q->grad and k->grad and, with a norm, the
+ * heads (heads.data is not read without one). With t the gradient turned back, n = h *
+ * rstd and p = t * weight:
+ *
+ *   gradient = rstd * (p - n * sum(p * n) / size), or t without a norm
+ *   grad_weight = t * n summed over tokens and heads in fp32, in a fixed order
+ *
+ * workspace: rln_rotary_backward_workspace_bytes of device scratch, aligned to 4
+ * (unused, may be NULL, without a grad_weight); calls that overlap need one each.
+ */
+int rln_rotary_backward(
+    const rln_rotary_side_t* q,
+    const rln_rotary_side_t* k,
+    int dtype,
+    const rln_rotary_t* rotary,
+    int64_t outer,
+    int64_t inner,
+    int64_t size,
+    double eps,
+    void* workspace,
+    size_t workspace_bytes,
+    void* stream);
+
+/* Workspace bytes rln_rotary_backward needs for its sums (no counterpart in the
+ * reference). */
+size_t rln_rotary_backward_workspace_bytes(
+    int64_t outer,
+    int64_t inner,
+    int64_t q_heads,
+    int64_t k_heads,
+    int64_t size,
+    int64_t pairs,
+    int dtype);
+
 /* Thread-local message for the last failed call on this thread (the text of
  * the reference's TORCH_CHECK messages, csrc/residual_layer_norm_kernel.hip:26-166). */
 const char* rln_last_error(void);
