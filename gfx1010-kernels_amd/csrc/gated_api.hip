@@ -55,7 +55,7 @@ int check_rows(const char* name, const void* data, int dtype, int64_t stride, in
 }
 
 int check_factor(const char* name, const rln_factor_t* given, int64_t rows, Factor* factor) {
-    *factor = Factor{nullptr, 0, rows, RLN_DTYPE_F32};
+    *factor = Factor{nullptr, 0, rows, RLN_DTYPE_F32, kShared, 0, 0};
     if (given == nullptr || given->data == nullptr) {
         return RLN_OK;
     }
@@ -63,7 +63,8 @@ int check_factor(const char* name, const rln_factor_t* given, int64_t rows, Fact
         return fail(RLN_ERR_INVALID, "%s: its rows must each serve a whole share of the rows",
                     name);
     }
-    *factor = Factor{given->data, given->stride, given->rows, given->dtype};
+    *factor = Factor{given->data, given->stride, given->rows, given->dtype, kShared, 0, 0};
+    set_repeat(factor, rows);
     return check_rows(name, given->data, given->dtype, given->stride, rows / given->rows);
 }
 
@@ -110,12 +111,14 @@ int check_common(const void* branch, int branch_dtype, int64_t branch_stride,
 
 // ----------------------------------------------------------------------------
 // The sums of S and T over the units (gated_device.h), in a fixed order, and the
-// factors' gradients from them. A block owns 16 columns of one of the two sums
-// (blockIdx.y): 16 lanes read one 64-byte line of a unit's row. Its 64 slots of
-// lanes take `concurrent` groups at a time, 64 / concurrent slots each, which add
-// every so manieth unit of their group in ascending order; the first slot of each
-// group adds the others' totals, writes the group's gradients and keeps the sum
-// over the groups it has seen, which are added last.
+// factors' gradients from them. A block owns 32 columns, a 128-byte line of a unit's
+// row, of one of the two sums (blockIdx.y). Its 32 slots of 32 lanes take `concurrent`
+// groups at a time, 32 / concurrent slots each, which add every so manieth unit of
+// their group in ascending order; the first slot of each group adds the others'
+// totals, writes the group's gradients and keeps the sum over the groups it has
+// seen, which are added last. Every thread's loads, and the additions' reads of LDS, are
+// under way together: one after another they took 6.5 us at [8192, 768] and 16.7 at
+// [4096, 8192], in blocks of 16 columns.
 
 struct SumArgs {
     const float* partials;
@@ -136,8 +139,8 @@ struct SumArgs {
     float branch_scale;
 };
 
-constexpr int kSumColumns = 16;
-constexpr int kSumSlots = 64;
+constexpr int kSumColumns = 32;
+constexpr int kSumSlots = 32;
 
 __device__ __forceinline__ float load_one(const void* tensor, int dtype, int64_t index) {
     if (dtype == RLN_DTYPE_F32) {
@@ -149,8 +152,24 @@ __device__ __forceinline__ float load_one(const void* tensor, int dtype, int64_t
     return static_cast<float>(static_cast<const bf16_t*>(tensor)[index]);
 }
 
+// The totals of slots slot, slot + step, ... below slot + count, in that order.
+__device__ __forceinline__ float add_slots(const float (&totals)[kSumSlots][kSumColumns], int slot,
+                                           int lane, int step, int count) {
+    float values[kSumSlots];
+#pragma unroll
+    for (int i = 0; i < kSumSlots; ++i) {
+        values[i] = i < count ? totals[slot + i * step][lane] : 0.0f;
+    }
+    float sum = values[0];
+#pragma unroll
+    for (int i = 1; i < kSumSlots; ++i) {
+        sum += values[i];
+    }
+    return sum;
+}
+
 __global__ __launch_bounds__(kSumColumns * kSumSlots) void sum_units_kernel(SumArgs a) {
-    __shared__ float totals[kSumSlots][kSumColumns + 1];
+    __shared__ float totals[kSumSlots][kSumColumns];
     const bool first_sum = blockIdx.y == 0;  // S; else T
     if (first_sum ? a.grad_gate == nullptr && a.grad_branch_weight == nullptr
                   : a.grad_weight == nullptr) {
@@ -165,31 +184,41 @@ __global__ __launch_bounds__(kSumColumns * kSumSlots) void sum_units_kernel(SumA
     const int part = slot - place * slots;
     const float* partials = a.partials + (first_sum ? 0 : a.hidden) + column;
     const int64_t unit_stride = int64_t{2} * a.hidden;
-    // The gate of token gates is in S already.
-    const bool gated = a.gate.data != nullptr && a.gate.rows > 1;
-    const float post =
-        a.branch_weight != nullptr && live
-            ? load_one(a.branch_weight, a.branch_weight_dtype, column) : 1.0f;
     float over_groups = 0.0f;
     for (int64_t base = 0; base < a.groups; base += a.concurrent) {
         const int64_t group = base + place;
         const bool own = group < a.groups && live;
         float total = 0.0f;
         if (own) {
-#pragma unroll 8
-            for (int64_t unit = part; unit < a.group_units; unit += slots) {
-                total += partials[(group * a.group_units + unit) * unit_stride];
+            const float* from = partials + (group * a.group_units + part) * unit_stride;
+            const int64_t step = slots * unit_stride;
+            constexpr int kBatch = 8;
+            int64_t unit = part;
+            for (; unit + (kBatch - 1) * slots < a.group_units; unit += kBatch * slots) {
+                float values[kBatch];
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    values[i] = from[i * step];
+                }
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    total += values[i];
+                }
+                from += kBatch * step;
+            }
+            for (; unit < a.group_units; unit += slots, from += step) {
+                total += *from;
             }
         }
         totals[slot][lane] = total;
         __syncthreads();
         if (own && part == 0) {
-            for (int other = 1; other < slots; ++other) {
-                total += totals[slot + other][lane];
-            }
+            total = add_slots(totals, slot, lane, 1, slots);
             if (first_sum) {
                 if (a.gate_groups) {
                     if (a.grad_gate != nullptr) {
+                        const float post = a.branch_weight != nullptr
+                            ? load_one(a.branch_weight, a.branch_weight_dtype, column) : 1.0f;
                         store_one(a.grad_gate, a.gate.dtype, group * a.hidden + column,
                                   a.branch_scale * post * total);
                     }
@@ -205,17 +234,18 @@ __global__ __launch_bounds__(kSumColumns * kSumSlots) void sum_units_kernel(SumA
     totals[slot][lane] = over_groups;
     __syncthreads();
     if (slot == 0 && live) {
-        for (int other = slots; other < kSumSlots; other += slots) {
-            over_groups += totals[other][lane];
-        }
+        over_groups = add_slots(totals, 0, lane, slots, a.concurrent);
         if (!first_sum) {
             if (!a.weight_groups) {
                 store_one(a.grad_weight, a.weight_dtype, column, over_groups);
             }
             return;
         }
-        const bool shared_gate = gated && !a.gate_groups;
+        // The gate of token gates is in S already.
+        const bool shared_gate = a.gate.data != nullptr && a.gate.rows > 1 && !a.gate_groups;
         if (a.grad_gate != nullptr && shared_gate) {
+            const float post = a.branch_weight != nullptr
+                ? load_one(a.branch_weight, a.branch_weight_dtype, column) : 1.0f;
             store_one(a.grad_gate, a.gate.dtype, column, a.branch_scale * post * over_groups);
         }
         if (a.grad_branch_weight != nullptr) {
@@ -265,7 +295,7 @@ int rln_gated_forward(
         || (status = check_stream(stream)) != RLN_OK) {
         return status;
     }
-    const Shape shape = forward_shape(rows, hidden, x_dtype);
+    const Shape shape = pass_shape(rows, hidden, x_dtype);
     a.x = x;
     a.branch = branch;
     a.branch_weight = branch_weight;
@@ -276,7 +306,7 @@ int rln_gated_forward(
     a.branch_stride = branch_stride;
     a.rows = rows;
     a.hidden = static_cast<int>(hidden);
-    a.parts = shape.parts;
+    a.split = split_of(shape);
     a.row_lanes = shape.row_lanes;
     a.branch_weight_dtype = branch_weight_dtype;
     a.output_dtype = normalized_dtype;
@@ -309,7 +339,9 @@ size_t rln_gated_backward_workspace_bytes(int64_t rows, int64_t hidden, int x_dt
         return 0;
     }
     const int64_t group = gate_rows > 1 && gate_rows < rows ? gate_rows : weight_rows;
-    return static_cast<size_t>(units_of(rows, group, walk_shape(hidden, x_dtype)).count)
+    const bool token_gate = gate_rows == 1 && rows > 1;
+    return static_cast<size_t>(
+               units_of(rows, group, token_gate, walk_shape(hidden, x_dtype)).count)
         * 2 * static_cast<size_t>(hidden) * sizeof(float);
 }
 
@@ -369,7 +401,7 @@ int rln_gated_backward(
         return status;
     }
     const Shape shape = walk_shape(hidden, x_dtype);
-    const Units units = units_of(rows, a.group_rows, shape);
+    const Units units = units_of(rows, a.group_rows, token_gate && rows > 1, shape);
     a.grad_updated = grad_updated;
     a.grad_normalized = grad_normalized;
     a.updated = updated;
@@ -385,7 +417,7 @@ int rln_gated_backward(
     a.units = units.count;
     a.group_units = static_cast<int>(units.group_units);
     a.hidden = static_cast<int>(hidden);
-    a.parts = shape.parts;
+    a.split = split_of(shape);
     a.row_lanes = shape.row_lanes;
     a.grad_dtype = grad_normalized_dtype;
     a.branch_weight_dtype = branch_weight_dtype;

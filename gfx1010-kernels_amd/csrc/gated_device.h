@@ -45,6 +45,19 @@ struct Factor {
     int64_t stride;    // between consecutive rows of factors, in elements
     int64_t rows;
     int dtype;
+    int kind;          // Repeat
+    uint32_t magic;    // of a 32-bit division by `rows`
+    int shift;
+};
+
+enum Repeat { kShared, kToken, kSample, kWideSample };
+
+// A block's waves as teams of `parts`. A wave finds its own by a product: a block of
+// one row would wait a good part of its time for the divisions.
+struct Split {
+    int parts;
+    int teams;
+    uint32_t inverse;  // 2^16 / parts, rounded up
 };
 
 struct ForwardArgs {
@@ -60,7 +73,7 @@ struct ForwardArgs {
     int64_t branch_stride;
     int64_t rows;
     int hidden;
-    int parts;
+    Split split;
     int row_lanes;
     int words;
     int branch_weight_dtype;
@@ -91,7 +104,7 @@ struct BackwardArgs {
     int64_t units;       // runs of rows with sums of their own
     int group_units;     // of a group
     int hidden;
-    int parts;
+    Split split;
     int row_lanes;
     int words;
     int grad_dtype;      // grad_normalized's
@@ -187,42 +200,33 @@ __device__ __forceinline__ void widen_optional(const RawAny<N>& raw, const void*
 }
 
 // The first element of the factors' row for a row of the stream.
-__device__ __forceinline__ int64_t factor_row(const Factor& factor, int64_t row, int64_t rows) {
-    if (factor.rows >= rows) {
+__device__ __forceinline__ int64_t factor_row(const Factor& factor, int64_t row) {
+    if (factor.kind == kShared) {
         return 0;
     }
-    if (factor.rows == 1) {
-        return row * factor.stride;
+    int64_t index = row;
+    if (factor.kind == kSample) {
+        const uint32_t narrow = static_cast<uint32_t>(row);
+        const uint32_t high = __umulhi(narrow, factor.magic);
+        index = (high + ((narrow - high) >> 1)) >> factor.shift;
+    } else if (factor.kind == kWideSample) {
+        index = row / factor.rows;
     }
-    return (rows <= UINT32_MAX ? static_cast<int64_t>(static_cast<uint32_t>(row)
-                                                      / static_cast<uint32_t>(factor.rows))
-                               : row / factor.rows) * factor.stride;
+    return index * factor.stride;
+}
+
+__device__ __forceinline__ Team team_of(const Split& split) {
+    Team team;
+    team.wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    team.index = static_cast<int>(static_cast<uint32_t>(team.wave) * split.inverse >> 16);
+    team.part = team.wave - team.index * split.parts;
+    team.teams = split.teams;
+    return team;
 }
 
 // The factors from an element on.
 __device__ __forceinline__ const void* row_of(const Factor& factor, int64_t first) {
     return static_cast<const char*>(factor.data) + first * (factor.dtype == RLN_DTYPE_F32 ? 4 : 2);
-}
-
-// N elements of a streamed tensor whose type is known at run time.
-template <Access kAccess, typename T, int N>
-__device__ __forceinline__ void load_widened(const void* data, int64_t first, int column,
-                                             int hidden, float (&out)[N]) {
-    auto raw = load<kAccess, T, N>(static_cast<const T*>(data) + first, column, hidden);
-    settle<kAccess>(raw, column, hidden);
-    widen<T, N>(raw, out);
-}
-
-template <Access kAccess, int N>
-__device__ __forceinline__ void load_upstream(const void* data, int dtype, int64_t first,
-                                              int column, int hidden, float (&out)[N]) {
-    if (dtype == RLN_DTYPE_F32) {
-        load_widened<kAccess, float, N>(data, first, column, hidden, out);
-    } else if (dtype == RLN_DTYPE_F16) {
-        load_widened<kAccess, half_t, N>(data, first, column, hidden, out);
-    } else {
-        load_widened<kAccess, bf16_t, N>(data, first, column, hidden, out);
-    }
 }
 
 template <Access kAccess>
@@ -237,7 +241,7 @@ template <typename X, typename B, int V, bool kPost, Access kAccess>
 __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs a) {
     constexpr int N = kColumns<X>;
     __shared__ float sums[2][2][kMaxParts];
-    const Team team = team_of(a.parts);
+    const Team team = team_of(a.split);
     const Place place = place_of<kAccess>(a.row_lanes);
     const int block_rows = team.teams * place.rows;
     const int64_t step = static_cast<int64_t>(gridDim.x) * block_rows;
@@ -246,12 +250,12 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
     // same number of calls. Two buffers: a wave that is ahead writes the one that
     // the slower ones do not read.
     const auto team_total = [&](float value, int which) {
-        if (a.parts > 1) {
+        if (a.split.parts > 1) {
             sums[turn][which][team.wave] = value;
             __syncthreads();
             value = 0.0f;
-            for (int part = 0; part < a.parts; ++part) {
-                value += sums[turn][which][team.index * a.parts + part];
+            for (int part = 0; part < a.split.parts; ++part) {
+                value += sums[turn][which][team.index * a.split.parts + part];
             }
         }
         return value;
@@ -264,8 +268,6 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
         const int64_t first = row * a.hidden;
         const X* x = static_cast<const X*>(a.x) + row * a.x_stride;
         const B* branch = static_cast<const B*>(a.branch) + row * a.branch_stride;
-        const int64_t gate_row = live ? factor_row(a.gate, row, a.rows) : 0;
-        const int64_t weight_row = live ? factor_row(a.weight, row, a.rows) : 0;
         int column[V];
         Raw<X, N> raw_x[V];
         Raw<B, N> raw_branch[V];
@@ -274,13 +276,15 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
         RawAny<N> raw_weight[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            column[v] = ((v * a.parts + team.part) * kWave + place.lane) * N;
+            column[v] = ((v * a.split.parts + team.part) * kWave + place.lane) * N;
             raw_branch[v] = load<kAccess, B, N>(branch, column[v], hidden);
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             raw_x[v] = load<kAccess, X, N>(x, column[v], hidden);
         }
+        const int64_t gate_row = factor_row(a.gate, live ? row : 0);
+        const int64_t weight_row = factor_row(a.weight, live ? row : 0);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             raw_gate[v] = load_optional<kAccess, N>(a.gate.data, a.gate.dtype, gate_row, column[v],
@@ -374,6 +378,63 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
 // partials, which sum_units_kernel adds in a fixed order: no atomics, the same bits
 // on every run.
 
+// What a lane reads of a row.
+template <typename X, typename B, int V, bool kToken>
+struct Row {
+    Raw<X, kColumns<X>> u[V];
+    Raw<B, kColumns<X>> branch[V];
+    Raw<X, kColumns<X>> grad[V];
+    RawAny<kColumns<X>> upstream[V];
+    RawAny<kColumns<X>> gate[kToken ? V : 1];
+    float rstd;
+    float branch_rstd;
+};
+
+template <typename X, typename B, int V, bool kPost, bool kToken, Access kAccess>
+__device__ __forceinline__ void load_row(const BackwardArgs& a, int64_t row, int64_t end,
+                                         const int (&column)[V], Row<X, B, V, kToken>* out) {
+    constexpr int N = kColumns<X>;
+    const bool live = row < end;
+    const int hidden = live ? a.hidden : 0;
+    const int64_t first = row * a.hidden;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        out->u[v] = load<kAccess, X, N>(static_cast<const X*>(a.updated) + first, column[v],
+                                        hidden);
+        out->branch[v] = load<kAccess, B, N>(
+            static_cast<const B*>(a.branch) + row * a.branch_stride, column[v], hidden);
+        out->grad[v] = Raw<X, N>{};
+        if (a.grad_updated != nullptr) {
+            out->grad[v] = load<kAccess, X, N>(static_cast<const X*>(a.grad_updated) + first,
+                                               column[v], hidden);
+        }
+        out->upstream[v] = load_optional<kAccess, N, kOnce>(a.grad_normalized, a.grad_dtype, first,
+                                                            column[v], hidden);
+        if constexpr (kToken) {
+            out->gate[v] = load_any<kAccess, N, kOnce>(a.gate.data, a.gate.dtype,
+                                                       row * a.gate.stride, column[v], hidden);
+        }
+    }
+    out->rstd = live ? a.statistics[row] : 0.0f;
+    out->branch_rstd = kPost && live ? a.statistics[a.rows + row] : 1.0f;
+}
+
+// sums += a * b, of a lane's own N sums in LDS.
+template <int N>
+__device__ __forceinline__ void add_products(float* sums, const float (&a)[N],
+                                             const float (&b)[N]) {
+    typedef float Four __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        Four four = *reinterpret_cast<Four*>(sums + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            four[k] = __builtin_fmaf(a[i + k], b[i + k], four[k]);
+        }
+        *reinterpret_cast<Four*>(sums + i) = four;
+    }
+}
+
 // kToken: the gate has a row for each token, read beside the others; S then holds
 // it as a factor. Otherwise the factors do not depend on the row and stay in
 // registers over a unit's rows.
@@ -381,15 +442,21 @@ __global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs 
 template <typename X, typename B, int V, bool kPost, bool kToken, Access kAccess>
 __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArgs a) {
     constexpr int N = kColumns<X>;
-    extern __shared__ float shares[];  // [teams - 1][hidden], one sum at a time
+    // As far as the registers go.
+    constexpr bool kAhead = kAccess != Access::kLanes && V * N <= (kToken ? 4 : 8);
+    // Lanes of more than 8 columns, of which a block is one row, keep the sums in LDS,
+    // each its own, since they do not fit the registers.
+    constexpr bool kLdsSums = V * N > 8;
+    // [teams - 1][hidden], one sum at a time; or the sums [2][block's columns].
+    extern __shared__ __attribute__((aligned(16))) float shares[];
     __shared__ float sums[2][3][kMaxParts];
-    const Team team = team_of(a.parts);
+    const Team team = team_of(a.split);
     const Place place = place_of<kAccess>(a.row_lanes);
     const int block_rows = team.teams * place.rows;
     int column[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        column[v] = ((v * a.parts + team.part) * kWave + place.lane) * N;
+        column[v] = ((v * a.split.parts + team.part) * kWave + place.lane) * N;
     }
     int turn = 0;
     // Every team of the block makes the same number of turns (barriers inside).
@@ -397,15 +464,30 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
         const int64_t group = unit / a.group_units;
         const int64_t begin = group * a.group_rows;
         const int64_t end = begin + a.group_rows;
+        // The next row's loads are under way while a row is reduced and written.
+        const int64_t step = static_cast<int64_t>(a.group_units) * block_rows;
+        int64_t base = begin + (unit - group * a.group_units) * block_rows;
+        Row<X, B, V, kToken> next;
+        if constexpr (kAhead) {
+            load_row<X, B, V, kPost, kToken, kAccess>(a, base + team.index * place.rows + place.row,
+                                                      end, column, &next);
+        }
         float weight[V][N];
         float factor[V][N];  // branch_scale * branch_weight, and the gate unless kToken
         float sum_s[V][N];
         float sum_t[V][N];
+        float* lds_t = shares + V * N * static_cast<int>(blockDim.x);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            load_weight<kAccess, N>(
-                row_of(a.weight, factor_row(a.weight, begin, a.rows)), a.weight.dtype, column[v],
-                a.hidden, weight[v]);
+            if constexpr (kLdsSums) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    shares[column[v] + e] = 0.0f;
+                    lds_t[column[v] + e] = 0.0f;
+                }
+            }
+            load_weight<kAccess, N>(row_of(a.weight, factor_row(a.weight, begin)), a.weight.dtype,
+                                    column[v], a.hidden, weight[v]);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 factor[v][e] = a.branch_scale;
@@ -423,59 +505,30 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
             }
             if (!kToken && a.gate.data != nullptr) {
                 float gate[N];
-                load_weight<kAccess, N>(row_of(a.gate, factor_row(a.gate, begin, a.rows)),
-                                        a.gate.dtype, column[v], a.hidden, gate);
+                load_weight<kAccess, N>(row_of(a.gate, factor_row(a.gate, begin)), a.gate.dtype,
+                                        column[v], a.hidden, gate);
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
                     factor[v][e] *= gate[e];
                 }
             }
         }
-        const int64_t step = static_cast<int64_t>(a.group_units) * block_rows;
-        for (int64_t base = begin + (unit - group * a.group_units) * block_rows; base < end;
-             base += step) {
+        for (; base < end; base += step) {
             const int64_t row = base + team.index * place.rows + place.row;
+            if constexpr (!kAhead) {
+                load_row<X, B, V, kPost, kToken, kAccess>(a, row, end, column, &next);
+            }
+            Row<X, B, V, kToken> now = next;
+            if constexpr (kAhead) {
+                if (base + step < end) {
+                    load_row<X, B, V, kPost, kToken, kAccess>(a, row + step, end, column, &next);
+                }
+            }
             const bool live = row < end;
             const int hidden = live ? a.hidden : 0;
             const int64_t first = row * a.hidden;
-            Raw<B, N> raw_branch[V];
-            Raw<X, N> raw_u[V];
-            Raw<X, N> raw_grad[V];
-            RawAny<N> raw_gate[V];
-            float upstream[V][N];
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                raw_u[v] = load<kAccess, X, N>(static_cast<const X*>(a.updated) + first,
-                                               column[v], hidden);
-                raw_branch[v] = load<kAccess, B, N>(
-                    static_cast<const B*>(a.branch) + row * a.branch_stride, column[v], hidden);
-                raw_grad[v] = Raw<X, N>{};
-                if (a.grad_updated != nullptr) {
-                    raw_grad[v] = load<kAccess, X, N>(static_cast<const X*>(a.grad_updated) + first,
-                                                      column[v], hidden);
-                }
-                if constexpr (kToken) {
-                    raw_gate[v] = load_any<kAccess, N, kOnce>(a.gate.data, a.gate.dtype,
-                                                              row * a.gate.stride, column[v],
-                                                              hidden);
-                }
-            }
-            const float rstd = live ? a.statistics[row] : 0.0f;
-            const float branch_rstd = kPost && live ? a.statistics[a.rows + row] : 1.0f;
-            // Last, since its type is known at run time only and it is waited for in
-            // the branch that loads it.
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                if (a.grad_normalized != nullptr) {
-                    load_upstream<kAccess, N>(a.grad_normalized, a.grad_dtype, first, column[v],
-                                              hidden, upstream[v]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        upstream[v][e] = 0.0f;
-                    }
-                }
-            }
+            const float rstd = now.rstd;
+            const float branch_rstd = now.branch_rstd;
             float unit_u[V][N];
             float unit_branch[V][N];
             float gradient[V][N];
@@ -483,31 +536,39 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 float gate[N];
-                settle<kAccess>(raw_u[v], column[v], hidden);
-                settle<kAccess>(raw_branch[v], column[v], hidden);
-                settle<kAccess>(raw_grad[v], column[v], hidden);
-                widen<X, N>(raw_u[v], unit_u[v]);
-                widen<B, N>(raw_branch[v], unit_branch[v]);
-                widen<X, N>(raw_grad[v], gradient[v]);
+                float upstream[N];
+                settle<kAccess>(now.u[v], column[v], hidden);
+                settle<kAccess>(now.branch[v], column[v], hidden);
+                settle<kAccess>(now.grad[v], column[v], hidden);
+                widen<X, N>(now.u[v], unit_u[v]);
+                widen<B, N>(now.branch[v], unit_branch[v]);
+                widen<X, N>(now.grad[v], gradient[v]);
+                widen_optional<kAccess, N>(now.upstream[v], a.grad_normalized, a.grad_dtype,
+                                           column[v], hidden, 0.0f, upstream);
                 if constexpr (kToken && kPost) {
-                    widen_any<kAccess, N>(raw_gate[v], a.gate.dtype, column[v], hidden, gate);
+                    widen_any<kAccess, N>(now.gate[v], a.gate.dtype, column[v], hidden, gate);
                 }
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
                     unit_u[v][e] *= rstd;
                     unit_branch[v][e] *= branch_rstd;
-                    const float product = upstream[v][e] * weight[v][e];
-                    sum_t[v][e] += upstream[v][e] * unit_u[v][e];
-                    gradient[v][e] += rstd * product;
-                    total[0] += product * unit_u[v][e];
+                    const float product = upstream[e] * weight[v][e];
+                    if constexpr (!kLdsSums) {
+                        sum_t[v][e] = __builtin_fmaf(upstream[e], unit_u[v][e], sum_t[v][e]);
+                    }
+                    gradient[v][e] = __builtin_fmaf(rstd, product, gradient[v][e]);
+                    total[0] = __builtin_fmaf(product, unit_u[v][e], total[0]);
                     if constexpr (kPost) {
                         float inner = factor[v][e] * unit_branch[v][e];
                         if constexpr (kToken) {
                             inner *= gate[e];
                         }
-                        total[1] += inner * gradient[v][e];
-                        total[2] += inner * unit_u[v][e];
+                        total[1] = __builtin_fmaf(inner, gradient[v][e], total[1]);
+                        total[2] = __builtin_fmaf(inner, unit_u[v][e], total[2]);
                     }
+                }
+                if constexpr (kLdsSums) {
+                    add_products<N>(lds_t + column[v], upstream, unit_u[v]);
                 }
             }
             constexpr int kTotals = kPost ? 3 : 1;
@@ -515,7 +576,7 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
             for (int i = 0; i < kTotals; ++i) {
                 total[i] = row_total<kAccess>(total[i], a.row_lanes);
             }
-            if (a.parts > 1) {
+            if (a.split.parts > 1) {
                 // Two buffers: a team's next turn writes the other one while
                 // slower waves still read this one.
 #pragma unroll
@@ -526,8 +587,8 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 #pragma unroll
                 for (int i = 0; i < kTotals; ++i) {
                     total[i] = 0.0f;
-                    for (int part = 0; part < a.parts; ++part) {
-                        total[i] += sums[turn][i][team.index * a.parts + part];
+                    for (int part = 0; part < a.split.parts; ++part) {
+                        total[i] += sums[turn][i][team.index * a.split.parts + part];
                     }
                 }
                 turn ^= 1;
@@ -539,26 +600,38 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
                 float gate[N];
                 float grad_x[N];
                 float grad_branch[N];
+                float each[N];
                 if constexpr (kToken) {
-                    widen_any<kAccess, N>(raw_gate[v], a.gate.dtype, column[v], hidden, gate);
+                    widen_any<kAccess, N>(now.gate[v], a.gate.dtype, column[v], hidden, gate);
                 }
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    const float g = gradient[v][e] - unit_u[v][e] * shared;
+                    const float g = __builtin_fmaf(-unit_u[v][e], shared, gradient[v][e]);
                     grad_x[e] = a.residual_scale * g;
                     grad_branch[e] = factor[v][e] * g;
                     // A team without a row adds nothing, whatever the factors hold.
-                    const float each = live ? g * unit_branch[v][e] : 0.0f;
+                    each[e] = live ? g * unit_branch[v][e] : 0.0f;
                     if constexpr (kToken) {
                         grad_branch[e] *= gate[e];
-                        sum_s[v][e] += each * gate[e];
-                        gate[e] = each * factor[v][e];  // from here on its gradient
-                    } else {
-                        sum_s[v][e] += each;
                     }
                     if constexpr (kPost) {
-                        grad_branch[e] =
-                            branch_rstd * (grad_branch[e] - unit_branch[v][e] * branch_shared);
+                        grad_branch[e] = branch_rstd
+                            * __builtin_fmaf(-unit_branch[v][e], branch_shared, grad_branch[e]);
+                    }
+                }
+                if constexpr (!kToken) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        gate[e] = 1.0f;
+                    }
+                }
+                if constexpr (kLdsSums) {
+                    add_products<N>(shares + column[v], each, gate);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        sum_s[v][e] = kToken ? __builtin_fmaf(each[e], gate[e], sum_s[v][e])
+                                             : sum_s[v][e] + each[e];
                     }
                 }
                 store<kAccess, kBackwardStores, X, N>(static_cast<X*>(a.grad_x) + first, column[v],
@@ -566,12 +639,32 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
                 store<kAccess, kBackwardStores, B, N>(static_cast<B*>(a.grad_branch) + first,
                                                       column[v], hidden, narrow<B, N>(grad_branch));
                 if (kToken && a.grad_gate != nullptr) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        gate[e] = each[e] * factor[v][e];  // from here on its gradient
+                    }
                     store_as<kAccess, kBackwardStores, N>(a.grad_gate, a.gate.dtype, first,
                                                           column[v], hidden, gate);
                 }
             }
         }
         if (a.partials == nullptr) {
+            continue;
+        }
+        float* partial = a.partials + unit * 2 * a.hidden;
+        if constexpr (kLdsSums) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    sum_s[v][e] = shares[column[v] + e];
+                    sum_t[v][e] = lds_t[column[v] + e];
+                }
+                store<kAccess, kBackwardStores, float, N>(partial, column[v], a.hidden,
+                                                          narrow<float, N>(sum_s[v]));
+                store<kAccess, kBackwardStores, float, N>(partial + a.hidden, column[v], a.hidden,
+                                                          narrow<float, N>(sum_t[v]));
+            }
             continue;
         }
         int own[V];
@@ -593,7 +686,6 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
             }
         }
         // Teams 1, 2, ... leave their shares; team 0 adds them in that order.
-        float* partial = a.partials + unit * 2 * a.hidden;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             if (team.teams > 1) {
@@ -639,10 +731,80 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 }
 
 // ----------------------------------------------------------------------------
-// Launch shapes (host).
+// Launch shapes (host). Measured on MI355X, graphs of launches over buffers that pass
+// the caches (a large copy reaches 5.1 TB/s there):
+//
+//  * Forward: two slots of a 16-bit stream, four of a 32-bit one, so that a row has
+//    half or a quarter of the waves, which wait for one another twice a row ([6001,
+//    2880] bf16 29.7 against 37.8 us with one slot, [16384, 4096] 96 against 101;
+//    [8192, 4096] fp32 72.8 against 75.0 with two slots, 116.7 with one). Launches whose
+//    waves of one slot are at most half of those that the chip holds take one slot up to
+//    8 waves a row, two beyond: their time is one row's ([512, 4096] bf16 6.0 against
+//    6.5 us, [256, 512] fp32 3.7 against 4.5 with four).
+//  * Backward: one slot up to 16 waves a row of a 16-bit stream ([16384, 4096] bf16 155
+//    against 192 us with two: the next row's words no longer fit the registers), two
+//    from 5 vectors on of a 32-bit one ([4096, 4096] fp32 64 against 74 us, [8192, 1024]
+//    37.4 and 37.9).
+//  * One block of about 8 waves for each CU, of 12 to 16 where a row has 5 waves or more
+//    ([16384, 4096] bf16 148 against 162 us, [8192, 2048] 46.7 and 47.8): each block
+//    leaves two rows of partial sums, and more blocks cost more in those than they gain
+//    ([8192, 4096] fp32 111 against 114 us with two blocks). Two where a block has fewer
+//    than 8 waves, and of token gates up to 10, whose next row is not read ahead
+//    ([8192, 2048] bf16 62 against 73 us).
+//  * Rows of more columns than 16 waves of 8 hold keep their sums in LDS ([2048, 16384]
+//    bf16 113 us, 154 with sums that left the registers for memory).
 
-// Units of a backward: runs of rows of one group, together at most as many as
-// the blocks of rms_device.h's walk, but at least one for each group.
+inline Split split_of(const Shape& shape) {
+    const uint32_t parts = static_cast<uint32_t>(shape.parts);
+    return Split{shape.parts, teams_of(shape), ((1u << 16) + parts - 1) / parts};
+}
+
+// How a factor's row is found from the stream's: rows / `factor.rows` by a product
+// with ceil(2^(32 + s) / rows) - 2^32, s = ceil(log2(rows)), for 32-bit row numbers.
+inline void set_repeat(Factor* factor, int64_t rows) {
+    factor->kind = factor->rows >= rows ? kShared
+        : factor->rows == 1 ? kToken : rows <= INT32_MAX ? kSample : kWideSample;
+    if (factor->kind == kSample) {
+        int bits = 1;
+        while (int64_t{1} << bits < factor->rows) {
+            ++bits;
+        }
+        const uint64_t divisor = static_cast<uint64_t>(factor->rows);
+        factor->magic = static_cast<uint32_t>(
+            ((uint64_t{1} << 32) * ((uint64_t{1} << bits) - divisor)) / divisor + 1);
+        factor->shift = bits - 1;
+    }
+}
+
+inline Shape pass_shape(int64_t rows, int64_t hidden, int x_dtype) {
+    if (hidden <= 32 * columns_of(x_dtype)) {
+        return short_shape(hidden, x_dtype, 4);
+    }
+    const int64_t vectors = wave_vectors(hidden, x_dtype);
+    const bool resident = rows <= 16 * kComputeUnits && rows * vectors <= 16 * kComputeUnits;
+    const int wanted = resident ? (vectors <= 8 ? 1 : 2) : x_dtype == RLN_DTYPE_F32 ? 4 : 2;
+    int slots = 1;
+    while ((slots < wanted && slots < vectors) || slots * kMaxParts < vectors) {
+        slots *= 2;
+    }
+    return shape_of(vectors, slots, 4);
+}
+
+inline Shape walk_shape(int64_t hidden, int x_dtype) {
+    if (hidden <= 32 * columns_of(x_dtype)) {
+        return short_shape(hidden, x_dtype, 8);
+    }
+    const int64_t vectors = wave_vectors(hidden, x_dtype);
+    int slots = x_dtype == RLN_DTYPE_F32 && vectors > 4 ? 2 : 1;
+    while (slots * kMaxParts < vectors) {
+        slots *= 2;
+    }
+    const int waves = x_dtype != RLN_DTYPE_F32 && vectors > 4 && vectors <= kMaxParts ? 12 : 8;
+    return shape_of(vectors, slots, waves);
+}
+
+// Units of a backward: runs of rows of one group, together at most as many as the
+// launch has blocks, but at least one for each group.
 struct Units {
     int64_t groups;
     int64_t group_rows;
@@ -650,19 +812,12 @@ struct Units {
     int64_t count;
 };
 
-// The norm's shape (rms_device.h), but one slot as long as sixteen waves hold a
-// row: the sums and factors of two slots of a 16-bit stream do not fit the registers.
-inline Shape walk_shape(int64_t hidden, int x_dtype) {
-    const Shape shape = backward_shape(hidden, x_dtype);
-    const int64_t vectors = wave_vectors(hidden, x_dtype);
-    return shape.slots > 1 && vectors <= kMaxParts ? shape_of(vectors, 1, 8) : shape;
-}
-
-inline Units units_of(int64_t rows, int64_t group_rows, const Shape& shape) {
+inline Units units_of(int64_t rows, int64_t group_rows, bool token_gate, const Shape& shape) {
     Units units;
     units.group_rows = group_rows;
     units.groups = rows / group_rows;
-    const int64_t most = shape.threads <= 10 * kWave ? 2 * kComputeUnits : kComputeUnits;
+    const bool two = shape.threads < 8 * kWave || (token_gate && shape.threads <= 10 * kWave);
+    const int64_t most = (two ? 2 : 1) * kComputeUnits;
     const int64_t wanted = blocks_of(group_rows, shape);
     const int64_t each = most / units.groups > 0 ? most / units.groups : 1;
     units.group_units = wanted < each ? wanted : each;

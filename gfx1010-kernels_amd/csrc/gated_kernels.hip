@@ -32,13 +32,24 @@ using Args = ForwardArgs;
 #else
 template <typename X, typename B, int V, bool kPost, bool kToken>
 int run_token(const BackwardArgs& a, const Shape& shape, hipStream_t stream) {
-    const size_t lds = a.partials == nullptr
+    constexpr int kLaneColumns = V * kColumns<X>;
+    const size_t lds = kLaneColumns > 8
+        ? 2 * static_cast<size_t>(shape.threads) * kLaneColumns * sizeof(float)
+        : a.partials == nullptr
         ? 0 : static_cast<size_t>(teams_of(shape) - 1) * a.hidden * sizeof(float);
     auto kernel = a.words ? backward_kernel<X, B, V, kPost, kToken, Access::kWords>
                           : backward_kernel<X, B, V, kPost, kToken, Access::kElements>;
     if constexpr (V == 1) {
         if (shape.row_lanes < kWave) {
             kernel = backward_kernel<X, B, 1, kPost, kToken, Access::kLanes>;
+        }
+    }
+    if (lds > 1 << 16) {
+        const hipError_t status = hipFuncSetAttribute(
+            reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+            static_cast<int>(lds));
+        if (status != hipSuccess) {
+            return fail(RLN_ERR_HIP, "gated backward_kernel: %s", hipGetErrorString(status));
         }
     }
     const int64_t blocks = a.units < kMaxBlocks ? a.units : kMaxBlocks;
