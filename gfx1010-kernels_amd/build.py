@@ -177,17 +177,15 @@ def _torch_paths() -> tuple[list[str], Path, bool]:
     )
 
 
-def build_glue() -> Path:
+def build_glue(build_dir: Path = BUILD_DIR) -> Path:
     """Compile the torch glue module linked against librln_gfx950.so."""
     includes, torch_lib, cxx11_abi = _torch_paths()
     python_include = sysconfig.get_paths()["include"]
-    temporary = GLUE.with_name(GLUE.name + ".tmp")
-    command = [
-        "g++",
+    build_dir.mkdir(parents=True, exist_ok=True)
+    compile_flags = [
         "-O2",
         "-std=c++17",
         "-fPIC",
-        "-shared",
         "-Wall",
         "-Wno-unused-function",
         "-D__HIP_PLATFORM_AMD__=1",
@@ -199,7 +197,21 @@ def build_glue() -> Path:
         *[f"-I{path}" for path in includes],
         f"-I{python_include}",
         f"-I{ROCM / 'include'}",
-        *map(str, GLUE_SOURCES),
+    ]
+
+    # Named .glue: not among the library's objects, which are taken by pattern elsewhere.
+    def compile_one(source: Path) -> Path:
+        output = build_dir / f"{source.stem}.glue"
+        _run(["g++", *compile_flags, "-c", str(source), "-o", str(output)])
+        return output
+
+    with ThreadPoolExecutor(max_workers=len(GLUE_SOURCES)) as pool:
+        objects = list(pool.map(compile_one, GLUE_SOURCES))
+    temporary = GLUE.with_name(GLUE.name + ".tmp")
+    _run([
+        "g++",
+        "-shared",
+        *map(str, objects),
         f"-L{torch_lib}",
         f"-L{PACKAGE}",
         "-lc10",
@@ -212,8 +224,7 @@ def build_glue() -> Path:
         "-Wl,-rpath,$ORIGIN",
         "-o",
         str(temporary),
-    ]
-    _run(command)
+    ])
     os.replace(temporary, GLUE)
     return GLUE
 

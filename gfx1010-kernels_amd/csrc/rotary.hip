@@ -14,14 +14,16 @@
 // Bound by memory (4-16 bytes per value against 10-25 operations), as long as the
 // angles are not: each is a product in fp64, a reduction to an eighth of a turn and two
 // polynomials, about 45 operations, and all heads of a token share them. So a
-// block first makes the cosines and sines of a tile of tokens, one pair per thread,
-// in LDS, and its lanes then walk the heads of those tokens.
+// block first makes the cosines and sines of a tile of tokens in LDS, and its lanes then
+// walk the heads of those tokens, those of q or those of k: one side's weight and sums
+// fit the registers beside a head that is read ahead.
 //
 // A head belongs to the fewest lanes, a power of two, that hold it: a lane takes two
 // vectors of 16 bytes, eight pairs of a 16-bit type (four of fp32): from each half of
 // the turned part, or neighbouring ones where pairs are neighbours. Values that are
 // not turned follow in vectors of their own, with cosine 1 and sine 0. A wave holds
-// 64 / lanes heads, 8 of 128 16-bit values; a sum over a head stays in its lanes.
+// 64 / lanes heads, 8 of 128 16-bit values; a sum over a head stays in its lanes, and
+// a lane's columns, hence its weights, are the same for every head it walks.
 
 #include "rms_device.h"
 
@@ -34,7 +36,9 @@ using namespace rms;
 constexpr int kThreads = 256;
 constexpr int64_t kMaxSize = 256;
 constexpr int kMaxAxes = 4;
+constexpr int64_t kMaxHeads = 1 << 16;
 constexpr int kMaxPairs = kMaxSize / 2;
+constexpr int kTilePairs = 2048;  // 16 KB of LDS
 
 enum class Pass { kTurn, kNorm, kNormBackward };
 
@@ -43,28 +47,37 @@ struct Side {
     const void* grad;   // the backward's
     const void* weight;
     void* output;
+    float* partials;    // [blocks][size], or null
     int64_t heads_outer, heads_token, heads_head;
     int64_t grad_outer, grad_token, grad_head;
+    // From a head to the one that a lane takes next, row_step heads on: tokens and heads,
+    // and elements of both tensors, the latter for a token more and `count` heads less.
+    int step_tokens, step_heads;
+    int64_t heads_step, heads_wrap;
+    int64_t grad_step, grad_wrap;
+    int row_step;
     int count;
     float inverse_count;
     int weight_dtype;
+    int tile;           // tokens
+    int parts;          // blocks that share a tile's heads
+    int items;          // tiles * parts
+    int blocks;         // which walk the items
 };
 
 struct Args {
-    Side side[2];
+    Side side[2];             // the launch's first side[0].blocks are q's
     const void* positions;
     const void* frequencies;
-    float* partials;          // [blocks][2][size], or null
     int64_t position_axis, position_outer, position_token;
     int tokens;
     int inner;
-    int tile;                 // tokens
-    int tiles;
     int size;
     int pairs;
     int row_pairs;            // of a token in LDS: pairs in whole vectors
     float inverse_row_pairs;
     int lanes;                // of a head
+    int lanes_shift;
     int turned_lanes;         // those of turned values
     int positions_type;
     int wide_frequencies;
@@ -156,34 +169,51 @@ __device__ __forceinline__ Place place_of(const Args& a, int chunk) {
 // kWhole: every run is whole vectors, so that one is read or not at all.
 template <bool kWhole, typename T, int N>
 __device__ __forceinline__ Raw<T, N> load_vector(const T* head, const Place& place, int half,
-                                                 bool live) {
+                                                 int extent) {
     const T* run = head + place.base[half];
-    const int extent = live ? place.extent : 0;
     if constexpr (kWhole) {
-        using W = WordVector<4, static_cast<int>(sizeof(T))>;
+        constexpr int kWords = Raw<T, N>::kWords;
+        using W = WordVector<kWords, static_cast<int>(sizeof(T))>;
         typename W::plain words{};
         if (place.column[half] < extent) {
-            words = __builtin_nontemporal_load(
-                reinterpret_cast<const typename W::type*>(run + place.column[half]));
+            words = *reinterpret_cast<const typename W::type*>(run + place.column[half]);
         }
         Raw<T, N> raw;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kWords; ++i) {
             raw.words[i] = words[i];
         }
         return raw;
     } else {
-        return load<Access::kLanes, T, N>(run, place.column[half], extent);
+        return load<Access::kLanes, T, N, kCached>(run, place.column[half], extent);
     }
 }
 
 template <bool kWhole, typename T, int N>
 __device__ __forceinline__ void widen_vector(Raw<T, N>& raw, const Place& place, int half,
-                                             bool live, float (&out)[N]) {
+                                             int extent, float (&out)[N]) {
     if constexpr (!kWhole) {
-        settle<Access::kLanes>(raw, place.column[half], live ? place.extent : 0);
+        settle<Access::kLanes>(raw, place.column[half], extent);
     }
     widen<T, N>(raw, out);
+}
+
+// Each value rounded once to T, to nearest even, two with one instruction.
+template <typename T, int N>
+__device__ __forceinline__ Raw<T, N> narrow_pairs(const float (&values)[N]) {
+    if constexpr (sizeof(T) == 4) {
+        return narrow<T, N>(values);
+    } else {
+        typedef float Two __attribute__((ext_vector_type(2)));
+        typedef T Narrow __attribute__((ext_vector_type(2)));
+        Raw<T, N> raw;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const Two two = {values[2 * i], values[2 * i + 1]};
+            raw.words[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(two, Narrow));
+        }
+        return raw;
+    }
 }
 
 template <bool kWhole, typename T, int N>
@@ -192,16 +222,40 @@ __device__ __forceinline__ void store_vector(T* head, const Place& place, int ha
     T* run = head + place.base[half];
     if constexpr (kWhole) {
         if (place.column[half] < place.extent) {
-            const Raw<T, N> raw = narrow<T, N>(values);
-            using W = WordVector<4, static_cast<int>(sizeof(T))>;
-            const typename W::plain words = {raw.words[0], raw.words[1], raw.words[2],
-                                             raw.words[3]};
+            const Raw<T, N> raw = narrow_pairs<T, N>(values);
+            constexpr int kWords = Raw<T, N>::kWords;
+            using W = WordVector<kWords, static_cast<int>(sizeof(T))>;
+            typename W::plain words;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                words[i] = raw.words[i];
+            }
             __builtin_nontemporal_store(
                 words, reinterpret_cast<typename W::type*>(run + place.column[half]));
         }
     } else {
         store<Access::kLanes, kForwardStores, T, N>(run, place.column[half], place.extent,
-                                                    narrow<T, N>(values));
+                                                    narrow_pairs<T, N>(values));
+    }
+}
+
+// A lane's part of a norm's weight; zeros where it has no columns.
+template <bool kWhole, typename W, int N>
+__device__ __forceinline__ void load_weight(const void* weight, const Place& place,
+                                            float (&out)[2][N]) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const W* run = static_cast<const W*>(weight) + place.base[half];
+        Raw<W, N> raw{};
+        if constexpr (kWhole) {
+            if (place.column[half] < place.extent) {
+                __builtin_memcpy(&raw, run + place.column[half], sizeof(raw));
+            }
+        } else {
+            raw = load<Access::kLanes, W, N, kCached>(run, place.column[half], place.extent);
+            settle<Access::kLanes>(raw, place.column[half], place.extent);
+        }
+        widen<W, N>(raw, out[half]);
     }
 }
 
@@ -223,8 +277,8 @@ __device__ __forceinline__ void turn(float (&first)[N], float (&second)[N],
                                      const float (&cosine)[N], const float (&sine)[N],
                                      bool interleaved) {
     const auto pair = [](float& x, float& y, float c, float s) {
-        const float turned = x * c - y * s;
-        y = x * s + y * c;
+        const float turned = __builtin_fmaf(x, c, -(y * s));
+        y = __builtin_fmaf(x, s, y * c);
         x = turned;
     };
     if (interleaved) {
@@ -241,83 +295,162 @@ __device__ __forceinline__ void turn(float (&first)[N], float (&second)[N],
     }
 }
 
-// Sum over each aligned run of `lanes` lanes, a power of two.
+// Sum over each aligned run of `lanes` lanes, a power of two; kLanes: the number where
+// it is known at compile time, else 0.
+template <int kLanes>
 __device__ __forceinline__ float head_sum(float value, int lanes) {
+    const int own = kLanes > 0 ? kLanes : lanes;
 #define ROTARY_ADD(control) \
     value += __builtin_bit_cast(float, RMS_DPP(__builtin_bit_cast(uint32_t, value), control))
-    if (lanes > 1) {
+    if (own > 1) {
         ROTARY_ADD(kXor1);
     }
-    if (lanes > 2) {
+    if (own > 2) {
         ROTARY_ADD(kXor2);
     }
-    if (lanes > 4) {
+    if (own > 4) {
         ROTARY_ADD(kHalfMirror);
     }
-    if (lanes > 8) {
+    if (own > 8) {
         ROTARY_ADD(kMirror);
     }
 #undef ROTARY_ADD
-    if (lanes > 16) {
+    if (own > 16) {
         value += __shfl_xor(value, 16);
     }
-    if (lanes > 32) {
+    if (own > 32) {
         value += __shfl_xor(value, 32);
     }
     return value;
 }
 
+// 1 / sqrt(value), within two units in the last place: the hardware's reciprocal root
+// (one unit) where it takes the value whole, the exact operations under that.
+__device__ __forceinline__ float inverse_root(float value) {
+    return value >= 0x1p-120f ? __builtin_amdgcn_rsqf(value) : 1.0f / __builtin_sqrtf(value);
+}
+
 // ----------------------------------------------------------------------------
-// One block per tile of tokens and share of their heads (blockIdx.y); in the
-// backward with a norm the blocks walk the tiles, so that a block leaves one row of
+// One block per item, a tile of tokens and a share of their heads on one side; in the
+// backward with a norm the blocks walk the items, so that each leaves one row of
 // partial sums, which reduce_kernel adds in a fixed order.
 
-template <typename T, Pass kPass, bool kWhole>
-__global__ __launch_bounds__(kThreads) void heads_kernel(Args a) {
-    constexpr int N = kColumns<T>;
+// What a lane reads of a head: what is turned, and the backward's heads.
+template <typename T, int N, bool kSums>
+struct Head {
+    Raw<T, N> turned[2];
+    Raw<T, N> heads[kSums ? 2 : 1];
+    int local;  // its token in the tile
+};
+
+// Waves for each SIMD. The backward of eight pairs a lane needs 140 registers: held to
+// 128 it left 23 of them for memory, and wrote and read more there than its tensors have
+// ([8192, 24 heads of 64] fp16 41 against 33 us).
+constexpr int waves_of(Pass pass, int columns) {
+    return columns == 8 ? (pass == Pass::kNormBackward ? 3 : 4)
+                        : pass == Pass::kNormBackward ? 4 : 5;
+}
+
+template <typename T, int N, Pass kPass, bool kWhole, int kLanes>
+__global__ __launch_bounds__(kThreads, waves_of(kPass, N)) void heads_kernel(Args a) {
     constexpr bool kNormed = kPass != Pass::kTurn;
     constexpr bool kSums = kPass == Pass::kNormBackward;
-    // Cosines and sines [tile][row_pairs] each, then the weights [2][lanes][2][N].
+    // Ones and zeros [N] for values that are not turned, cosines and sines
+    // [tile][row_pairs] each; at the end the sums.
     extern __shared__ __attribute__((aligned(16))) float lds[];
-    const int angles = a.tile * a.row_pairs;
-    float* cosines = lds;
-    float* sines = lds + angles;
-    float* weights = lds + 2 * angles;
-    const int chunk = static_cast<int>(threadIdx.x) % a.lanes;
-    const int slot = static_cast<int>(threadIdx.x) / a.lanes;
-    const int slots = kThreads / a.lanes;
+    const int which = static_cast<int>(blockIdx.x) < a.side[0].blocks ? 0 : 1;
+    const Side& side = a.side[which];
+    const int block = static_cast<int>(blockIdx.x) - (which == 0 ? 0 : a.side[0].blocks);
+    const int half_lds = N + side.tile * a.row_pairs;
+    float* cosines = lds + N;
+    float* sines = cosines + half_lds;
+    const int lanes = kLanes > 0 ? kLanes : a.lanes;
+    const int shift = kLanes > 0 ? __builtin_ctz(kLanes > 0 ? kLanes : 1) : a.lanes_shift;
+    const int chunk = static_cast<int>(threadIdx.x) & (lanes - 1);
+    const int slot = static_cast<int>(threadIdx.x) >> shift;
+    const int slots = kThreads >> shift;
     const Place place = place_of<N>(a, chunk);
-    if constexpr (kNormed) {
-        for (int i = static_cast<int>(threadIdx.x); i < 4 * a.lanes; i += kThreads) {
-            const int half = i & 1;
-            const Place at = place_of<N>(a, (i >> 1) % a.lanes);
-            const Side& side = a.side[(i >> 1) / a.lanes];
-            float values[N];
+    const bool turns = place.pair >= 0;
+    const bool normed = kNormed && side.weight != nullptr;
+    const bool one_run = a.inner >= a.tokens;
+    if (threadIdx.x < N) {
+        lds[threadIdx.x] = 1.0f;
+        lds[half_lds + threadIdx.x] = 0.0f;
+    }
+    // A lane's head: its token in the tile, and where it is.
+    int local = 0;
+    int head = 0;
+    const T* heads = nullptr;
+    const T* grad = nullptr;
+    const auto find_head = [&](int begin, int row) {
+        local = static_cast<int>((static_cast<float>(row) + 0.5f) * side.inverse_count);
+        head = row - local * side.count;
+        int outer = 0;
+        int within = begin + local;
+        if (!one_run) {
+            outer = within / a.inner;
+            within -= outer * a.inner;
+        }
+        heads = static_cast<const T*>(side.heads) + outer * side.heads_outer
+            + within * side.heads_token + head * side.heads_head;
+        grad = static_cast<const T*>(side.grad) + outer * side.grad_outer
+            + within * side.grad_token + head * side.grad_head;
+    };
+    const auto next_head = [&](int begin, int row) {
+        if (!one_run) {
+            find_head(begin, row);
+            return;
+        }
+        local += side.step_tokens;
+        head += side.step_heads;
+        const bool wraps = head >= side.count;
+        local += wraps ? 1 : 0;
+        head -= wraps ? side.count : 0;
+        heads += side.heads_step + (wraps ? side.heads_wrap : 0);
+        if (a.backward) {
+            grad += side.grad_step + (wraps ? side.grad_wrap : 0);
+        }
+    };
+    const auto load_head = [&](Head<T, N, kSums>* out) {
+        const T* turned = a.backward ? grad : heads;
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const int column = at.column[half] + e;
-                const int64_t index = at.base[half] + column;
-                values[e] = 0.0f;
-                if (side.weight != nullptr && column < at.extent) {
-                    values[e] = side.weight_dtype == RLN_DTYPE_F32
-                        ? static_cast<const float*>(side.weight)[index]
-                        : side.weight_dtype == RLN_DTYPE_F16
-                        ? static_cast<float>(static_cast<const half_t*>(side.weight)[index])
-                        : static_cast<float>(static_cast<const bf16_t*>(side.weight)[index]);
-                }
-                weights[i * N + e] = values[e];
+        for (int half = 0; half < 2; ++half) {
+            out->turned[half] = load_vector<kWhole, T, N>(turned, place, half, place.extent);
+            if constexpr (kSums) {
+                out->heads[half] =
+                    load_vector<kWhole, T, N>(heads, place, half, normed ? place.extent : 0);
             }
         }
-    }
-    float sums[2][2][N];
+        out->local = local;
+    };
+    float weight[2][N];
+    float sums[2][N];
 #pragma unroll
-    for (int i = 0; i < 4 * N; ++i) {
-        (&sums[0][0][0])[i] = 0.0f;
+    for (int i = 0; i < 2 * N; ++i) {
+        (&sums[0][0])[i] = 0.0f;
+        (&weight[0][0])[i] = 1.0f;
     }
-    for (int tile = static_cast<int>(blockIdx.x); tile < a.tiles;
-         tile += static_cast<int>(gridDim.x)) {
-        const int begin = tile * a.tile;
-        const int tokens = a.tokens - begin < a.tile ? a.tokens - begin : a.tile;
+    Head<T, N, kSums> ahead;
+    for (int item = block; item < side.items; item += side.blocks) {
+        const int tile = side.parts == 1 ? item : item / side.parts;
+        const int first_row = slot + (item - tile * side.parts) * slots;
+        const int begin = tile * side.tile;
+        const int tokens = a.tokens - begin < side.tile ? a.tokens - begin : side.tile;
+        const int rows = tokens * side.count;
+        // A tile's first heads are read while its angles are made.
+        if (first_row < rows) {
+            find_head(begin, first_row);
+            load_head(&ahead);
+        }
+        if (normed && item == block) {
+            if (side.weight_dtype == RLN_DTYPE_F32) {
+                load_weight<kWhole, float, N>(side.weight, place, weight);
+            } else if (side.weight_dtype == RLN_DTYPE_F16) {
+                load_weight<kWhole, half_t, N>(side.weight, place, weight);
+            } else {
+                load_weight<kWhole, bf16_t, N>(side.weight, place, weight);
+            }
+        }
         for (int i = static_cast<int>(threadIdx.x); i < tokens * a.row_pairs; i += kThreads) {
             const int token =
                 static_cast<int>((static_cast<float>(i) + 0.5f) * a.inverse_row_pairs);
@@ -335,194 +468,146 @@ __global__ __launch_bounds__(kThreads) void heads_kernel(Args a) {
             sines[i] = a.backward ? -sine : sine;
         }
         __syncthreads();
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            const Side& side = a.side[which];
-            const bool normed = kNormed && side.weight != nullptr;
-            float weight[2][N];
-            if constexpr (kNormed) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    read_lds<N>(weights + ((which * a.lanes + chunk) * 2 + half) * N,
-                                weight[half]);
-                }
+        for (int row = first_row; row < rows; row += side.row_step) {
+            Head<T, N, kSums> now = ahead;
+            if (row + side.row_step < rows) {
+                next_head(begin, row + side.row_step);
+                load_head(&ahead);
             }
-            const int rows = tokens * side.count;
-            for (int row = slot + static_cast<int>(blockIdx.y) * slots; row < rows;
-                 row += slots * static_cast<int>(gridDim.y)) {
-                const int local =
-                    static_cast<int>((static_cast<float>(row) + 0.5f) * side.inverse_count);
-                const int head = row - local * side.count;
-                const int token = begin + local;
-                int outer = 0;
-                int within = token;
-                if (a.inner < a.tokens) {
-                    outer = token / a.inner;
-                    within = token - outer * a.inner;
-                }
-                // What is turned: the heads, or the backward's gradient.
-                const bool back = a.backward != 0;
-                const T* from = back
-                    ? static_cast<const T*>(side.grad) + outer * side.grad_outer
-                        + within * side.grad_token + head * side.grad_head
-                    : static_cast<const T*>(side.heads) + outer * side.heads_outer
-                        + within * side.heads_token + head * side.heads_head;
-                Raw<T, N> raw[2];
-                Raw<T, N> raw_heads[2];
+            const int angle = turns ? now.local * a.row_pairs + place.pair : -N;
+            float values[2][N];
+            float cosine[N];
+            float sine[N];
+            read_lds<N>(cosines + angle, cosine);
+            read_lds<N>(sines + angle, sine);
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    raw[half] = load_vector<kWhole, T, N>(from, place, half, true);
-                }
-                if constexpr (kSums) {
-                    const T* heads = static_cast<const T*>(side.heads)
-                        + outer * side.heads_outer + within * side.heads_token
-                        + head * side.heads_head;
+            for (int half = 0; half < 2; ++half) {
+                widen_vector<kWhole, T, N>(now.turned[half], place, half, place.extent,
+                                           values[half]);
+            }
+            if constexpr (kPass == Pass::kNorm) {
+                if (normed) {
+                    float sum = 0.0f;
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        raw_heads[half] = load_vector<kWhole, T, N>(heads, place, half, normed);
-                    }
-                }
-                float values[2][N];
-                float cosine[N];
-                float sine[N];
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    cosine[e] = 1.0f;
-                    sine[e] = 0.0f;
-                }
-                if (place.pair >= 0) {
-                    read_lds<N>(cosines + local * a.row_pairs + place.pair, cosine);
-                    read_lds<N>(sines + local * a.row_pairs + place.pair, sine);
-                }
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    widen_vector<kWhole, T, N>(raw[half], place, half, true, values[half]);
-                }
-                if constexpr (kPass == Pass::kNorm) {
-                    if (normed) {
-                        float sum = 0.0f;
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                            for (int e = 0; e < N; ++e) {
-                                sum += values[half][e] * values[half][e];
-                            }
-                        }
-                        sum = head_sum(sum, a.lanes);
-                        const float rstd =
-                            1.0f / __builtin_sqrtf(sum * a.inverse_size + a.eps);
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                            for (int e = 0; e < N; ++e) {
-                                values[half][e] *= rstd * weight[half][e];
-                            }
+                        for (int e = 0; e < N; ++e) {
+                            sum = __builtin_fmaf(values[half][e], values[half][e], sum);
                         }
                     }
-                }
-                turn<N>(values[0], values[1], cosine, sine, a.interleaved != 0);
-                if constexpr (kSums) {
-                    if (normed) {
-                        float unit[2][N];
-                        float square = 0.0f;
-                        float shared = 0.0f;
+                    sum = head_sum<kLanes>(sum, lanes);
+                    const float rstd =
+                        inverse_root(sum * a.inverse_size + a.eps);
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            widen_vector<kWhole, T, N>(raw_heads[half], place, half, normed,
-                                                       unit[half]);
+                    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                            for (int e = 0; e < N; ++e) {
-                                square += unit[half][e] * unit[half][e];
-                                shared += values[half][e] * weight[half][e] * unit[half][e];
-                            }
-                        }
-                        square = head_sum(square, a.lanes);
-                        shared = head_sum(shared, a.lanes);
-                        const float rstd =
-                            1.0f / __builtin_sqrtf(square * a.inverse_size + a.eps);
-                        shared *= rstd * a.inverse_size;
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                            for (int e = 0; e < N; ++e) {
-                                const float normal = unit[half][e] * rstd;
-                                sums[which][half][e] += values[half][e] * normal;
-                                values[half][e] = rstd
-                                    * (values[half][e] * weight[half][e] - normal * shared);
-                            }
+                        for (int e = 0; e < N; ++e) {
+                            values[half][e] *= rstd * weight[half][e];
                         }
                     }
-                }
-                T* to = static_cast<T*>(side.output)
-                    + (static_cast<int64_t>(token) * side.count + head) * a.size;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    store_vector<kWhole, T, N>(to, place, half, values[half]);
                 }
             }
-        }
+            turn<N>(values[0], values[1], cosine, sine, a.interleaved != 0);
+            if constexpr (kSums) {
+                if (normed) {
+                    float unit[2][N];
+                    float square = 0.0f;
+                    float shared = 0.0f;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        widen_vector<kWhole, T, N>(now.heads[half], place, half, place.extent,
+                                                   unit[half]);
+#pragma unroll
+                        for (int e = 0; e < N; ++e) {
+                            square = __builtin_fmaf(unit[half][e], unit[half][e], square);
+                            shared = __builtin_fmaf(values[half][e] * weight[half][e],
+                                                    unit[half][e], shared);
+                        }
+                    }
+                    square = head_sum<kLanes>(square, lanes);
+                    shared = head_sum<kLanes>(shared, lanes);
+                    const float rstd =
+                        inverse_root(square * a.inverse_size + a.eps);
+                    shared *= rstd * a.inverse_size;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                        for (int e = 0; e < N; ++e) {
+                            const float normal = unit[half][e] * rstd;
+                            sums[half][e] =
+                                __builtin_fmaf(values[half][e], normal, sums[half][e]);
+                            values[half][e] = rstd
+                                * __builtin_fmaf(-normal, shared,
+                                                 values[half][e] * weight[half][e]);
+                        }
+                    }
+                }
+            }
+            T* to = static_cast<T*>(side.output)
+                + (static_cast<int64_t>(begin) * side.count + row) * a.size;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                store_vector<kWhole, T, N>(to, place, half, values[half]);
+            }
+            }
         __syncthreads();  // the tile's angles are read before the next one's are written
     }
     if constexpr (kSums) {
-        if (a.partials == nullptr) {
+        if (side.partials == nullptr) {
             return;
         }
         // The wave's heads by exchanges, the block's waves through LDS, in their order.
         constexpr int kWaves = kThreads / kWave;
         const int wave = static_cast<int>(threadIdx.x) / kWave;
         const int lane = static_cast<int>(threadIdx.x) % kWave;
-        const int vectors = 4 * a.lanes;  // [2][lanes][2] of N
+        const int vectors = 2 * a.lanes;  // [lanes][2] of N
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
+        for (int half = 0; half < 2; ++half) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    float sum = sums[which][half][e];
-                    for (int other = a.lanes; other < kWave; other *= 2) {
-                        sum += __shfl_xor(sum, other);
-                    }
-                    if (lane < a.lanes) {
-                        lds[(wave * vectors + (which * a.lanes + chunk) * 2 + half) * N + e] = sum;
-                    }
+            for (int e = 0; e < N; ++e) {
+                float sum = sums[half][e];
+                for (int other = a.lanes; other < kWave; other *= 2) {
+                    sum += __shfl_xor(sum, other);
+                }
+                if (lane < a.lanes) {
+                    lds[(wave * vectors + chunk * 2 + half) * N + e] = sum;
                 }
             }
         }
         __syncthreads();
-        float* partial = a.partials
-            + (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * 2 * a.size;
+        float* partial = side.partials + static_cast<int64_t>(block) * a.size;
         for (int i = static_cast<int>(threadIdx.x); i < vectors * N; i += kThreads) {
             const int e = i % N;
-            const int vector = i / N;
-            const int half = vector & 1;
-            const Place at = place_of<N>(a, (vector >> 1) % a.lanes);
-            const int which = (vector >> 1) / a.lanes;
+            const int half = i / N & 1;
+            const Place at = place_of<N>(a, i / N >> 1);
             if (at.column[half] + e < at.extent) {
                 float sum = lds[i];
+#pragma unroll
                 for (int other = 1; other < kWaves; ++other) {
                     sum += lds[other * vectors * N + i];
                 }
-                partial[which * a.size + at.base[half] + at.column[half] + e] = sum;
+                partial[at.base[half] + at.column[half] + e] = sum;
             }
         }
     }
 }
 
-// Fixed-order sums of the partials [blocks][2][size], rounded once to the weights'
-// types. A block owns 16 columns; its 64 groups of 16 lanes take every 64th row.
+// Fixed-order sums of the partials [blocks][size], rounded once to the weights'
+// types. A block owns 16 columns of one side; its 64 groups of 16 lanes take every 64th
+// row, all reads of eight rows and of the groups' totals under way together.
 constexpr int kReduceColumns = 16;
 constexpr int kReduceGroups = 64;
 
 struct ReduceArgs {
-    const float* partials;
+    const float* partials[2];
     void* grad_weight[2];
     int dtype[2];
-    int blocks;
+    int blocks[2];
     int size;
 };
 
 __global__ __launch_bounds__(kReduceColumns * kReduceGroups) void reduce_kernel(ReduceArgs a) {
-    __shared__ float totals[kReduceGroups][kReduceColumns + 1];
+    __shared__ float totals[kReduceGroups][kReduceColumns];
     const int which = blockIdx.y;
     if (a.grad_weight[which] == nullptr) {
         return;
@@ -532,18 +617,32 @@ __global__ __launch_bounds__(kReduceColumns * kReduceGroups) void reduce_kernel(
     const int column = blockIdx.x * kReduceColumns + lane;
     float total = 0.0f;
     if (column < a.size) {
-#pragma unroll 8
-        for (int block = group; block < a.blocks; block += kReduceGroups) {
-            total += a.partials[(static_cast<int64_t>(block) * 2 + which) * a.size + column];
+        constexpr int kBatch = 8;
+        const int blocks = a.blocks[which];
+        const float* from = a.partials[which] + static_cast<int64_t>(group) * a.size + column;
+        const int64_t step = static_cast<int64_t>(kReduceGroups) * a.size;
+        for (int block = group; block < blocks; block += kBatch * kReduceGroups) {
+            float values[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                values[i] = block + i * kReduceGroups < blocks ? from[i * step] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                total += values[i];
+            }
+            from += kBatch * step;
         }
     }
     totals[group][lane] = total;
     __syncthreads();
     if (group == 0 && column < a.size) {
-        for (int other = 1; other < kReduceGroups; ++other) {
-            total += totals[other][lane];
+        float sum = 0.0f;
+#pragma unroll
+        for (int other = 0; other < kReduceGroups; ++other) {
+            sum += totals[other][lane];
         }
-        store_one(a.grad_weight[which], a.dtype[which], column, total);
+        store_one(a.grad_weight[which], a.dtype[which], column, sum);
     }
 }
 
@@ -551,44 +650,94 @@ __global__ __launch_bounds__(kReduceColumns * kReduceGroups) void reduce_kernel(
 // Launch shapes and checks (host).
 
 struct Grid {
+    int columns;   // of a lane's vector
     int lanes;
+    int lanes_shift;
     int turned_lanes;
-    int tile;
-    int tiles;
     int row_pairs;
-    unsigned x;
-    unsigned y;
     bool whole;
+    struct {
+        int tile;
+        int parts;
+        int items;
+        int blocks;
+    } side[2];
 };
 
-// A tile has about as many pairs as the block has threads, so that each makes one
-// angle, and a launch of few tokens spreads their heads over more blocks. A backward
-// with sums walks its tiles with at most four blocks for each CU.
-Grid grid_of(int64_t tokens, int64_t most_heads, int64_t size, int64_t pairs, int dtype,
-             bool sums) {
-    Grid grid;
-    const int columns = columns_of(dtype);
+// Tiles: the blocks that a CU holds at once make `resident` of the launch; each costs
+// its passes, the turns of its lanes over the tile's heads, and about one and a half more
+// for its start and its angles. The tiles (powers of two, both sides with about the same
+// passes) are those of the least time by that count, rounds of blocks times a block's cost:
+// ([16384, 32 + 8 heads of 128] bf16 69 us in tiles of 4 passes, 79 of 8, 89 of 2; [8858, 16
+// + 16 of 72] fp16 29 of 4, 23 of 16). Where even tiles of one token are too few blocks, several
+// share a tile's heads. A backward with sums walks its items with the resident blocks.
+Grid grid_of(int64_t tokens, const int64_t (&counts)[2], int64_t size, int64_t pairs, int dtype,
+             Pass pass) {
+    Grid grid{};
     const int left = static_cast<int>(size - 2 * pairs);
+    const auto whole = [&](int columns) {
+        return pairs % columns == 0 && left % (2 * columns) == 0;
+    };
+    grid.columns = columns_of(dtype);
+    if (!whole(grid.columns) && whole(4)) {
+        grid.columns = 4;
+    }
+    const int columns = grid.columns;
+    grid.whole = whole(columns);
     grid.turned_lanes = static_cast<int>((pairs + columns - 1) / columns);
     const int vectors = grid.turned_lanes + (left + 2 * columns - 1) / (2 * columns);
     grid.lanes = 1;
     while (grid.lanes < vectors) {
         grid.lanes *= 2;
+        ++grid.lanes_shift;
     }
     grid.row_pairs = grid.turned_lanes * columns;
-    grid.whole = pairs % columns == 0 && left % (2 * columns) == 0;
-    const int full = kThreads / (grid.row_pairs > 0 ? grid.row_pairs : 1);
-    grid.tile = full < 1 ? 1 : full > 16 ? 16 : full;
-    while (grid.tile > 1 && tokens / grid.tile < 4 * kComputeUnits) {
-        grid.tile /= 2;
+    const int64_t slots = kThreads / grid.lanes;
+    const int64_t resident = waves_of(pass, columns) * kComputeUnits;
+    const auto divided = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    int64_t least = INT64_MAX;
+    for (int64_t goal = 1; goal <= 32; goal *= 2) {
+        int64_t tile[2] = {0, 0};
+        int64_t blocks = 0;
+        int64_t passes = 0;
+        for (int i = 0; i < 2; ++i) {
+            if (counts[i] > 0) {
+                tile[i] = 1;
+                while (tile[i] * counts[i] < goal * slots
+                       && 2 * tile[i] * grid.row_pairs <= kTilePairs) {
+                    tile[i] *= 2;
+                }
+                blocks += divided(tokens, tile[i]);
+                const int64_t own = divided(tile[i] * counts[i], slots);
+                passes = own > passes ? own : passes;
+            }
+        }
+        const int64_t start = pass == Pass::kNormBackward ? 1 : 3;
+        const int64_t cost = divided(blocks, resident) * (start + 2 * passes);
+        if (cost < least) {
+            least = cost;
+            grid.side[0].tile = static_cast<int>(tile[0]);
+            grid.side[1].tile = static_cast<int>(tile[1]);
+        }
     }
-    grid.tiles = static_cast<int>((tokens + grid.tile - 1) / grid.tile);
-    const int slots = kThreads / grid.lanes;
-    const int64_t passes = (grid.tile * most_heads + slots - 1) / slots;
-    const int64_t wanted = 4 * kComputeUnits;
-    const int64_t share = wanted / grid.tiles > 1 ? wanted / grid.tiles : 1;
-    grid.y = static_cast<unsigned>(passes < share ? passes : share);
-    grid.x = static_cast<unsigned>(sums && grid.tiles > wanted ? wanted : grid.tiles);
+    for (int i = 0; i < 2; ++i) {
+        if (counts[i] == 0) {
+            continue;
+        }
+        auto& side = grid.side[i];
+        const int64_t share = resident * counts[i] / (counts[0] + counts[1]);
+        const int64_t tiles = divided(tokens, side.tile);
+        const int64_t passes = divided(side.tile * counts[i], slots);
+        const int64_t parts = share / tiles > 1 ? share / tiles : 1;
+        side.parts = static_cast<int>(passes < parts ? passes : parts);
+        side.items = static_cast<int>(tiles * side.parts);
+        // A launch holds fewer than 2^32 threads.
+        int64_t most = int64_t{1} << 22;
+        if (pass == Pass::kNormBackward) {
+            most = share > 0 ? share : 1;
+        }
+        side.blocks = static_cast<int>(side.items < most ? side.items : most);
+    }
     return grid;
 }
 
@@ -635,8 +784,8 @@ int check_side(const char* name, const rln_rotary_side_t* given, int dtype, int6
     if (given == nullptr || given->count == 0) {
         return RLN_OK;
     }
-    // The rows of a tile of 16 tokens are divided by the count in fp32.
-    if (given->count < 0 || given->count > 1 << 16) {
+    // The rows of a tile are divided by the count in fp32.
+    if (given->count < 0 || given->count > kMaxHeads) {
         return fail(RLN_ERR_UNSUPPORTED, "%s: unsupported number of heads: %lld", name,
                     static_cast<long long>(given->count));
     }
@@ -769,23 +918,41 @@ int arguments(const rln_rotary_side_t* q, const rln_rotary_side_t* k, int dtype,
             != RLN_OK) {
         return status;
     }
-    const int most = a->side[0].count > a->side[1].count ? a->side[0].count : a->side[1].count;
-    if (most == 0) {
+    const int64_t counts[2] = {a->side[0].count, a->side[1].count};
+    if (counts[0] == 0 && counts[1] == 0) {
         return fail(RLN_ERR_INVALID, "empty tensors are unsupported");
     }
     if ((status = check_stream(stream)) != RLN_OK) {
         return status;
     }
     *normed = a->side[0].weight != nullptr || a->side[1].weight != nullptr;
-    *grid = grid_of(outer * inner, most, size, a->pairs, dtype, backward && *normed);
+    *grid = grid_of(outer * inner, counts, size, a->pairs, dtype,
+                    !*normed ? Pass::kTurn : backward ? Pass::kNormBackward : Pass::kNorm);
+    for (int i = 0; i < 2; ++i) {
+        a->side[i].tile = grid->side[i].tile;
+        a->side[i].parts = grid->side[i].parts;
+        a->side[i].items = grid->side[i].items;
+        a->side[i].blocks = grid->side[i].blocks;
+        Side& side = a->side[i];
+        if (side.count > 0) {
+            side.row_step = kThreads / grid->lanes * side.parts;
+            side.step_tokens = side.row_step / side.count;
+            side.step_heads = side.row_step % side.count;
+            side.heads_step =
+                side.step_tokens * side.heads_token + side.step_heads * side.heads_head;
+            side.heads_wrap = side.heads_token - side.count * side.heads_head;
+            side.grad_step =
+                side.step_tokens * side.grad_token + side.step_heads * side.grad_head;
+            side.grad_wrap = side.grad_token - side.count * side.grad_head;
+        }
+    }
     a->tokens = static_cast<int>(outer * inner);
     a->inner = static_cast<int>(inner);
-    a->tile = grid->tile;
-    a->tiles = grid->tiles;
     a->size = static_cast<int>(size);
     a->row_pairs = grid->row_pairs;
     a->inverse_row_pairs = 1.0f / static_cast<float>(grid->row_pairs);
     a->lanes = grid->lanes;
+    a->lanes_shift = grid->lanes_shift;
     a->turned_lanes = grid->turned_lanes;
     a->backward = backward;
     a->eps = static_cast<float>(eps);
@@ -793,37 +960,56 @@ int arguments(const rln_rotary_side_t* q, const rln_rotary_side_t* k, int dtype,
     return RLN_OK;
 }
 
-template <typename T, Pass kPass>
+template <typename T, int N, Pass kPass>
 int launch(const Args& a, const Grid& grid, hipStream_t stream) {
-    const size_t weights = kPass == Pass::kTurn ? 0 : 4 * a.lanes * kColumns<T>;
-    size_t floats = 2 * static_cast<size_t>(a.tile) * a.row_pairs + weights;
-    if (kPass == Pass::kNormBackward && floats < kThreads / kWave * weights) {
-        floats = kThreads / kWave * weights;  // the block's sums, in the same place
+    const int tile = a.side[0].tile > a.side[1].tile ? a.side[0].tile : a.side[1].tile;
+    size_t floats = 2 * (N + static_cast<size_t>(tile) * a.row_pairs);
+    const size_t sums = static_cast<size_t>(kThreads / kWave) * 2 * a.lanes * N;
+    if (kPass == Pass::kNormBackward && floats < sums) {
+        floats = sums;  // in the place of the angles
     }
-    const auto kernel =
-        grid.whole ? heads_kernel<T, kPass, true> : heads_kernel<T, kPass, false>;
-    kernel<<<dim3(grid.x, grid.y), kThreads, floats * sizeof(float), stream>>>(a);
+    // Sums over the lanes of the usual head sizes without a choice at run time.
+    auto kernel =
+        grid.whole ? heads_kernel<T, N, kPass, true, 0> : heads_kernel<T, N, kPass, false, 0>;
+    if constexpr (kPass != Pass::kTurn) {
+        if (grid.whole) {
+            kernel = a.lanes == 4 ? heads_kernel<T, N, kPass, true, 4>
+                : a.lanes == 8    ? heads_kernel<T, N, kPass, true, 8>
+                : a.lanes == 16   ? heads_kernel<T, N, kPass, true, 16>
+                                  : kernel;
+        }
+    }
+    const unsigned blocks = static_cast<unsigned>(a.side[0].blocks + a.side[1].blocks);
+    kernel<<<dim3(blocks), kThreads, floats * sizeof(float), stream>>>(a);
     return check_launch("rotary heads_kernel");
 }
 
-template <typename T>
+template <typename T, int N>
 int launch_pass(const Args& a, const Grid& grid, bool normed, hipStream_t stream) {
     if (!normed) {
-        return launch<T, Pass::kTurn>(a, grid, stream);
+        return launch<T, N, Pass::kTurn>(a, grid, stream);
     }
-    return a.backward ? launch<T, Pass::kNormBackward>(a, grid, stream)
-                      : launch<T, Pass::kNorm>(a, grid, stream);
+    return a.backward ? launch<T, N, Pass::kNormBackward>(a, grid, stream)
+                      : launch<T, N, Pass::kNorm>(a, grid, stream);
+}
+
+template <typename T>
+int launch_columns(const Args& a, const Grid& grid, bool normed, hipStream_t stream) {
+    if (grid.columns == kColumns<T>) {
+        return launch_pass<T, kColumns<T>>(a, grid, normed, stream);
+    }
+    return launch_pass<T, 4>(a, grid, normed, stream);
 }
 
 int launch_dtype(const Args& a, const Grid& grid, int dtype, bool normed, void* stream) {
     const hipStream_t queue = static_cast<hipStream_t>(stream);
     switch (dtype) {
         case RLN_DTYPE_F32:
-            return launch_pass<float>(a, grid, normed, queue);
+            return launch_columns<float>(a, grid, normed, queue);
         case RLN_DTYPE_F16:
-            return launch_pass<half_t>(a, grid, normed, queue);
+            return launch_columns<half_t>(a, grid, normed, queue);
         default:
-            return launch_pass<bf16_t>(a, grid, normed, queue);
+            return launch_columns<bf16_t>(a, grid, normed, queue);
     }
 }
 
@@ -852,14 +1038,16 @@ int rln_rotary_forward(
 size_t rln_rotary_backward_workspace_bytes(
     int64_t outer, int64_t inner, int64_t q_heads, int64_t k_heads, int64_t size, int64_t pairs,
     int dtype) {
-    const int64_t most = q_heads > k_heads ? q_heads : k_heads;
     if (!float_dtype(dtype) || outer < 1 || inner < 1 || inner > INT32_MAX / 2
         || outer > INT32_MAX / 2 / inner || size < 1 || size > kMaxSize || pairs < 1
-        || 2 * pairs > size || most < 1 || most > 1 << 16) {
+        || 2 * pairs > size || q_heads < 0 || k_heads < 0 || q_heads > kMaxHeads
+        || k_heads > kMaxHeads) {
         return 0;
     }
-    const Grid grid = grid_of(outer * inner, most, size, pairs, dtype, true);
-    return static_cast<size_t>(grid.x) * grid.y * 2 * static_cast<size_t>(size) * sizeof(float);
+    const int64_t counts[2] = {q_heads, k_heads};
+    const Grid grid = grid_of(outer * inner, counts, size, pairs, dtype, Pass::kNormBackward);
+    return (static_cast<size_t>(grid.side[0].blocks) + grid.side[1].blocks)
+        * static_cast<size_t>(size) * sizeof(float);
 }
 
 int rln_rotary_backward(
@@ -881,7 +1069,8 @@ int rln_rotary_backward(
     const bool sums = reduce.grad_weight[0] != nullptr || reduce.grad_weight[1] != nullptr;
     if (sums) {
         const size_t needed =
-            static_cast<size_t>(grid.x) * grid.y * 2 * static_cast<size_t>(size) * sizeof(float);
+            (static_cast<size_t>(a.side[0].blocks) + a.side[1].blocks)
+            * static_cast<size_t>(size) * sizeof(float);
         if (workspace == nullptr || workspace_bytes < needed) {
             return fail(RLN_ERR_INVALID, "workspace too small: need %zu bytes, got %zu", needed,
                         workspace == nullptr ? static_cast<size_t>(0) : workspace_bytes);
@@ -889,16 +1078,19 @@ int rln_rotary_backward(
         if ((status = check_address("workspace", workspace, 4)) != RLN_OK) {
             return status;
         }
-        a.partials = static_cast<float*>(workspace);
+        a.side[0].partials = static_cast<float*>(workspace);
+        a.side[1].partials =
+            a.side[0].partials + static_cast<int64_t>(a.side[0].blocks) * a.size;
     }
     status = launch_dtype(a, grid, dtype, normed, stream);
     if (status != RLN_OK || !sums) {
         return status;
     }
-    reduce.partials = a.partials;
-    reduce.dtype[0] = a.side[0].weight_dtype;
-    reduce.dtype[1] = a.side[1].weight_dtype;
-    reduce.blocks = static_cast<int>(grid.x * grid.y);
+    for (int i = 0; i < 2; ++i) {
+        reduce.partials[i] = a.side[i].partials;
+        reduce.dtype[i] = a.side[i].weight_dtype;
+        reduce.blocks[i] = a.side[i].blocks;
+    }
     reduce.size = a.size;
     const unsigned blocks = static_cast<unsigned>((size + kReduceColumns - 1) / kReduceColumns);
     reduce_kernel<<<dim3(blocks, 2), kReduceColumns * kReduceGroups, 0,

@@ -261,8 +261,8 @@ def test_workspace_sizes():
             for dtype in (F32, F16, BF16):
                 shared = size(rows, hidden, dtype, rows, rows)
                 assert 8 * hidden <= shared <= 512 * 8 * hidden
-                # a sum of its own for every group, however many there are
-                assert size(rows, hidden, dtype, 1, rows) == shared
+                # token gates have more units, and other groups a sum each at least
+                assert shared <= size(rows, hidden, dtype, 1, rows) <= 512 * 8 * hidden
                 if rows % 2 == 0:
                     assert size(rows, hidden, dtype, 2, rows) >= rows // 2 * 8 * hidden
                     assert size(rows, hidden, dtype, rows // 2, rows) >= 16 * hidden
