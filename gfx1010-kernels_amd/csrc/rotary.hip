@@ -43,8 +43,8 @@ constexpr int kTilePairs = 2048;  // 16 KB of LDS
 enum class Pass { kTurn, kNorm, kNormBackward };
 
 struct Side {
-    const void* heads;
-    const void* grad;   // the backward's
+    const void* heads;  // what is turned; in a backward with a norm, its heads
+    const void* grad;   // and what is turned there
     const void* weight;
     void* output;
     float* partials;    // [blocks][size], or null
@@ -166,7 +166,11 @@ __device__ __forceinline__ Place place_of(const Args& a, int chunk) {
     return place;
 }
 
-// kWhole: every run is whole vectors, so that one is read or not at all.
+// kWhole: every run is whole vectors, so that one is read or not at all. Cached loads:
+// a head's half is less than a line where heads are short, and its line is read twice
+// ([8192, 24 heads of 64] fp16 13.9 us, 16.5 with loads that do not stay; longer heads the
+// same); the outputs are not read here and do not stay ([16384, 40 of 128] bf16 69
+// against 73 us with plain stores).
 template <bool kWhole, typename T, int N>
 __device__ __forceinline__ Raw<T, N> load_vector(const T* head, const Place& place, int half,
                                                  int extent) {
@@ -347,6 +351,9 @@ struct Head {
 // 128 it left 23 of them for memory, and wrote and read more there than its tensors have
 // ([8192, 24 heads of 64] fp16 41 against 33 us).
 constexpr int waves_of(Pass pass, int columns) {
+    if (pass == Pass::kTurn) {
+        return columns == 8 ? 5 : 6;
+    }
     return columns == 8 ? (pass == Pass::kNormBackward ? 3 : 4)
                         : pass == Pass::kNormBackward ? 4 : 5;
 }
@@ -355,6 +362,9 @@ template <typename T, int N, Pass kPass, bool kWhole, int kLanes>
 __global__ __launch_bounds__(kThreads, waves_of(kPass, N)) void heads_kernel(Args a) {
     constexpr bool kNormed = kPass != Pass::kTurn;
     constexpr bool kSums = kPass == Pass::kNormBackward;
+    // Without a norm there is little to do while the next head comes, and more waves
+    // fit instead ([3711, 20 heads of 80] fp32 11.7 against 12.9 us).
+    constexpr bool kAhead = kPass != Pass::kTurn;
     // Ones and zeros [N] for values that are not turned, cosines and sines
     // [tile][row_pairs] each; at the end the sums.
     extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -393,8 +403,10 @@ __global__ __launch_bounds__(kThreads, waves_of(kPass, N)) void heads_kernel(Arg
         }
         heads = static_cast<const T*>(side.heads) + outer * side.heads_outer
             + within * side.heads_token + head * side.heads_head;
-        grad = static_cast<const T*>(side.grad) + outer * side.grad_outer
-            + within * side.grad_token + head * side.grad_head;
+        if constexpr (kSums) {
+            grad = static_cast<const T*>(side.grad) + outer * side.grad_outer
+                + within * side.grad_token + head * side.grad_head;
+        }
     };
     const auto next_head = [&](int begin, int row) {
         if (!one_run) {
@@ -407,12 +419,12 @@ __global__ __launch_bounds__(kThreads, waves_of(kPass, N)) void heads_kernel(Arg
         local += wraps ? 1 : 0;
         head -= wraps ? side.count : 0;
         heads += side.heads_step + (wraps ? side.heads_wrap : 0);
-        if (a.backward) {
+        if constexpr (kSums) {
             grad += side.grad_step + (wraps ? side.grad_wrap : 0);
         }
     };
     const auto load_head = [&](Head<T, N, kSums>* out) {
-        const T* turned = a.backward ? grad : heads;
+        const T* turned = kSums ? grad : heads;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             out->turned[half] = load_vector<kWhole, T, N>(turned, place, half, place.extent);
@@ -469,8 +481,12 @@ __global__ __launch_bounds__(kThreads, waves_of(kPass, N)) void heads_kernel(Arg
         }
         __syncthreads();
         for (int row = first_row; row < rows; row += side.row_step) {
+            if (!kAhead && row > first_row) {
+                next_head(begin, row);
+                load_head(&ahead);
+            }
             Head<T, N, kSums> now = ahead;
-            if (row + side.row_step < rows) {
+            if (kAhead && row + side.row_step < rows) {
                 next_head(begin, row + side.row_step);
                 load_head(&ahead);
             }
@@ -665,10 +681,10 @@ struct Grid {
 };
 
 // Tiles: the blocks that a CU holds at once make `resident` of the launch; each costs
-// its passes, the turns of its lanes over the tile's heads, and about one and a half more
-// for its start and its angles. The tiles (powers of two, both sides with about the same
-// passes) are those of the least time by that count, rounds of blocks times a block's cost:
-// ([16384, 32 + 8 heads of 128] bf16 69 us in tiles of 4 passes, 79 of 8, 89 of 2; [8858, 16
+// its passes, the turns of its lanes over the tile's heads, and half of one more for its
+// start and its angles, one and a half in a forward with a norm. The tiles (powers of two,
+// both sides with about the same passes) are those of the least time by that count,
+// rounds of blocks times a block's cost ([16384, 32 + 8 heads of 128] bf16 69 us in tiles of 4 passes, 79 of 8, 89 of 2; [8858, 16
 // + 16 of 72] fp16 29 of 4, 23 of 16). Where even tiles of one token are too few blocks, several
 // share a tile's heads. A backward with sums walks its items with the resident blocks.
 Grid grid_of(int64_t tokens, const int64_t (&counts)[2], int64_t size, int64_t pairs, int dtype,
@@ -712,7 +728,7 @@ Grid grid_of(int64_t tokens, const int64_t (&counts)[2], int64_t size, int64_t p
                 passes = own > passes ? own : passes;
             }
         }
-        const int64_t start = pass == Pass::kNormBackward ? 1 : 3;
+        const int64_t start = pass == Pass::kNorm ? 3 : 1;
         const int64_t cost = divided(blocks, resident) * (start + 2 * passes);
         if (cost < least) {
             least = cost;
@@ -926,6 +942,14 @@ int arguments(const rln_rotary_side_t* q, const rln_rotary_side_t* k, int dtype,
         return status;
     }
     *normed = a->side[0].weight != nullptr || a->side[1].weight != nullptr;
+    if (backward && !*normed) {
+        for (Side& side : a->side) {
+            side.heads = side.grad;
+            side.heads_outer = side.grad_outer;
+            side.heads_token = side.grad_token;
+            side.heads_head = side.grad_head;
+        }
+    }
     *grid = grid_of(outer * inner, counts, size, a->pairs, dtype,
                     !*normed ? Pass::kTurn : backward ? Pass::kNormBackward : Pass::kNorm);
     for (int i = 0; i < 2; ++i) {
