@@ -21,7 +21,7 @@
 // A head belongs to the fewest lanes, a power of two, that hold it: a lane takes two
 // vectors of 16 bytes, eight pairs of a 16-bit type (four of fp32): from each half of
 // the turned part, or neighbouring ones where pairs are neighbours. Values that are
-// not turned follow in vectors of their own, with cosine 1 and sine 0. A wave holds
+// not turned follow in vectors of their own, in lanes that turn nothing. A wave holds
 // 64 / lanes heads, 8 of 128 16-bit values; a sum over a head stays in its lanes, and
 // a lane's columns, hence its weights, are the same for every head it walks.
 
@@ -365,15 +365,13 @@ __global__ __launch_bounds__(kThreads, waves_of(kPass, N)) void heads_kernel(Arg
     // Without a norm there is little to do while the next head comes, and more waves
     // fit instead ([3711, 20 heads of 80] fp32 11.7 against 12.9 us).
     constexpr bool kAhead = kPass != Pass::kTurn;
-    // Ones and zeros [N] for values that are not turned, cosines and sines
-    // [tile][row_pairs] each; at the end the sums.
+    // Cosines and sines [tile][row_pairs] each; at the end the sums.
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int which = static_cast<int>(blockIdx.x) < a.side[0].blocks ? 0 : 1;
     const Side& side = a.side[which];
     const int block = static_cast<int>(blockIdx.x) - (which == 0 ? 0 : a.side[0].blocks);
-    const int half_lds = N + side.tile * a.row_pairs;
-    float* cosines = lds + N;
-    float* sines = cosines + half_lds;
+    float* cosines = lds;
+    float* sines = lds + side.tile * a.row_pairs;
     const int lanes = kLanes > 0 ? kLanes : a.lanes;
     const int shift = kLanes > 0 ? __builtin_ctz(kLanes > 0 ? kLanes : 1) : a.lanes_shift;
     const int chunk = static_cast<int>(threadIdx.x) & (lanes - 1);
@@ -383,10 +381,6 @@ __global__ __launch_bounds__(kThreads, waves_of(kPass, N)) void heads_kernel(Arg
     const bool turns = place.pair >= 0;
     const bool normed = kNormed && side.weight != nullptr;
     const bool one_run = a.inner >= a.tokens;
-    if (threadIdx.x < N) {
-        lds[threadIdx.x] = 1.0f;
-        lds[half_lds + threadIdx.x] = 0.0f;
-    }
     // A lane's head: its token in the tile, and where it is.
     int local = 0;
     int head = 0;
@@ -490,7 +484,7 @@ __global__ __launch_bounds__(kThreads, waves_of(kPass, N)) void heads_kernel(Arg
                 next_head(begin, row + side.row_step);
                 load_head(&ahead);
             }
-            const int angle = turns ? now.local * a.row_pairs + place.pair : -N;
+            const int angle = now.local * a.row_pairs + (turns ? place.pair : 0);
             float values[2][N];
             float cosine[N];
             float sine[N];
@@ -523,7 +517,11 @@ __global__ __launch_bounds__(kThreads, waves_of(kPass, N)) void heads_kernel(Arg
                     }
                 }
             }
-            turn<N>(values[0], values[1], cosine, sine, a.interleaved != 0);
+            // Not by a cosine of 1 and a sine of 0: each of the other values stays, also
+            // beside one that is not finite.
+            if (turns) {
+                turn<N>(values[0], values[1], cosine, sine, a.interleaved != 0);
+            }
             if constexpr (kSums) {
                 if (normed) {
                     float unit[2][N];
@@ -962,11 +960,15 @@ int arguments(const rln_rotary_side_t* q, const rln_rotary_side_t* k, int dtype,
             side.row_step = kThreads / grid->lanes * side.parts;
             side.step_tokens = side.row_step / side.count;
             side.step_heads = side.row_step % side.count;
-            side.heads_step =
-                side.step_tokens * side.heads_token + side.step_heads * side.heads_head;
+            // Unsigned: a step past the last token may not fit, and is not taken.
+            const auto step = [&](int64_t token, int64_t head) {
+                return static_cast<int64_t>(
+                    static_cast<uint64_t>(side.step_tokens) * static_cast<uint64_t>(token)
+                    + static_cast<uint64_t>(side.step_heads) * static_cast<uint64_t>(head));
+            };
+            side.heads_step = step(side.heads_token, side.heads_head);
             side.heads_wrap = side.heads_token - side.count * side.heads_head;
-            side.grad_step =
-                side.step_tokens * side.grad_token + side.step_heads * side.grad_head;
+            side.grad_step = step(side.grad_token, side.grad_head);
             side.grad_wrap = side.grad_token - side.count * side.grad_head;
         }
     }
@@ -987,7 +989,7 @@ int arguments(const rln_rotary_side_t* q, const rln_rotary_side_t* k, int dtype,
 template <typename T, int N, Pass kPass>
 int launch(const Args& a, const Grid& grid, hipStream_t stream) {
     const int tile = a.side[0].tile > a.side[1].tile ? a.side[0].tile : a.side[1].tile;
-    size_t floats = 2 * (N + static_cast<size_t>(tile) * a.row_pairs);
+    size_t floats = 2 * static_cast<size_t>(tile) * a.row_pairs;
     const size_t sums = static_cast<size_t>(kThreads / kWave) * 2 * a.lanes * N;
     if (kPass == Pass::kNormBackward && floats < sums) {
         floats = sums;  // in the place of the angles

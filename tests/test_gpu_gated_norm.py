@@ -573,6 +573,29 @@ def test_captured_steps_replay():
             assert all(same_bits(a, b) for a, b in zip(found, expected)), turn
 
 
+@pytest.mark.parametrize("hidden", [8200, 16384])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_captured_steps_of_long_rows(hidden, dtype):
+    """Rows whose sums are in LDS, more of it than a launch has by default."""
+    parts = to_gpu(reference.make((3, 5, hidden), [dtype] * 5, seed=23))
+    upstream = [t.cuda() for t in upstream_of(parts, dtype)]
+    static = [t.clone().requires_grad_() for t in parts]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outputs = call(static, implementation="auto")
+        found = [*outputs, *torch.autograd.grad(outputs, static, upstream)]
+    for turn in range(3):
+        with torch.no_grad():
+            for leaf, value in zip(static, parts):
+                leaf.copy_(value + 0.25 * turn)
+        leaves = [(t + 0.25 * turn).requires_grad_() for t in parts]
+        outputs = call(leaves)
+        expected = [*outputs, *torch.autograd.grad(outputs, leaves, upstream)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(same_bits(a, b) for a, b in zip(found, expected)), turn
+
+
 @pytest.mark.parametrize("post,gate", [(True, "sample"), (False, "token"), (True, "none")])
 def test_compiled_step_equals_the_eager_one(post, gate):
     parts = to_gpu(reference.make((2, 9, 260), [BF16, F32, F32, F32, F32], post=post, gate=gate,

@@ -354,6 +354,24 @@ def test_heads_that_are_not_finite_stay_alone(bad, norm):
             assert same_bits(found[1][3], clean[1][3])
 
 
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("size,pairs", [(48, 8), (80, 16), (41, 5), (128, 32)])
+def test_values_that_are_not_turned_stay_alone(bad, size, pairs):
+    """Without a norm, a value behind the turned ones is copied, whatever is beside it;
+    so is its gradient."""
+    for dtype in (F32, BF16):
+        parts = to_gpu(reference.make((5,), 3, 1, size, dtype, pairs=pairs, norm=False, seed=28))
+        parts[2] = parts[2][0]
+        for column in {2 * pairs, size - 1, (2 * pairs + size) // 2}:
+            q = parts[0].clone()
+            q[1, 2, column] = bad
+            for interleaved in (False, True):
+                (out, _), grads = step([q, *parts[1:]], [q, parts[1]], interleaved=interleaved)
+                for found in (out, grads[0]):
+                    assert same_bits(found[..., 2 * pairs:], q[..., 2 * pairs:])
+                    assert found[..., :2 * pairs].isfinite().all()
+
+
 def test_positions_that_are_not_finite_stay_in_their_token():
     parts = to_gpu(reference.make((6,), 3, 1, 32, F32, seed=14, position_dtype=torch.float32))
     positions = parts[2][0].clone()
