@@ -860,7 +860,7 @@ int check_rotary(const rln_rotary_t* given, int64_t outer, int64_t inner, int64_
     if (given == nullptr || given->positions == nullptr || given->frequencies == nullptr) {
         return fail(RLN_ERR_INVALID, "positions and frequencies must not be null");
     }
-    if (given->pairs < 1 || 2 * given->pairs > size) {
+    if (given->pairs < 1 || given->pairs > size / 2) {
         return fail(RLN_ERR_INVALID, "the pairs must be 1 to half of the head's size");
     }
     if (given->axes < 1 || given->axes > kMaxAxes) {
@@ -1066,7 +1066,7 @@ size_t rln_rotary_backward_workspace_bytes(
     int dtype) {
     if (!float_dtype(dtype) || outer < 1 || inner < 1 || inner > INT32_MAX / 2
         || outer > INT32_MAX / 2 / inner || size < 1 || size > kMaxSize || pairs < 1
-        || 2 * pairs > size || q_heads < 0 || k_heads < 0 || q_heads > kMaxHeads
+        || pairs > size / 2 || q_heads < 0 || k_heads < 0 || q_heads > kMaxHeads
         || k_heads > kMaxHeads) {
         return 0;
     }
