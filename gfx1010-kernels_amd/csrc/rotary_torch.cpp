@@ -15,6 +15,7 @@
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 
+#include <algorithm>
 #include <optional>
 #include <tuple>
 
@@ -121,7 +122,8 @@ const char* refusal(const Inputs& in) {
             if (section < 0) {
                 return "sections must not be negative";
             }
-            total += section;
+            // One that is too many alone counts as that, so that no sum wraps round.
+            total += std::min(section, in.frequencies.size(0) + 1);
         }
         if (in.sections.size() > 4 || total != in.frequencies.size(0)) {
             return "sections must be 1 to 4 numbers of pairs that add up to inverse_frequencies";

@@ -255,6 +255,18 @@ def test_dispatch_reaches_the_kernels(recwarn):
                 call(given, implementation=implementation, **bad)
 
 
+def test_sections_whose_sum_wraps_round():
+    """Four sections that add up to the pairs in 64 bits alone are refused."""
+    parts = to_gpu(reference.make((5,), 3, 2, 40, F32, axes=4, seed=9))
+    pairs = parts[3].shape[0]
+    sections = (1 << 62, 1 << 62, 1 << 62, (1 << 62) + pairs)
+    for implementation in ("auto", "gfx950", "torch"):
+        with pytest.raises(ValueError, match="sections must add up"):
+            call(parts, sections=sections, implementation=implementation)
+    with pytest.raises(RuntimeError, match="that add up to"):
+        _C.rms_norm_rotary(*parts[:4], sections, False, False, *parts[4:], EPS)
+
+
 @pytest.mark.parametrize("shape", [(0, 4, 32), (2, 0, 4, 32), (2, 3, 0, 32)])
 def test_empty(shape):
     q = torch.zeros(shape, device="cuda", requires_grad=True)
