@@ -5,7 +5,7 @@
 //                           residual_scale, branch_scale, normalized_dtype)
 //       autograd op returning (updated, normalized)
 //   gated_residual_rms_norm_if_supported(...)   the same, or None
-//   gated_inputs_supported(...)                 the check alone
+//   gated_inputs_refusal(...)                   why the kernels refuse the inputs, or None
 //   gated_residual_rms_norm_forward(...)        (updated, normalized, statistics)
 //   gated_residual_rms_norm_backward(...)       the five gradients, None where not asked
 //

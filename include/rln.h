@@ -521,7 +521,8 @@ int rln_gated_backward(
 
 /* Workspace bytes rln_gated_backward needs for its sums (no counterpart in the
  * reference). gate_rows and weight_rows are the factors' `rows`; without a gate,
- * gate_rows is `rows`. */
+ * gate_rows is `rows`. Every group of rows that shares its factors has sums of its
+ * own, 8 bytes a column and more: a weight with a row each takes 8 bytes an element. */
 size_t rln_gated_backward_workspace_bytes(
     int64_t rows,
     int64_t hidden,
