@@ -295,7 +295,7 @@ int rln_gated_forward(
         || (status = check_stream(stream)) != RLN_OK) {
         return status;
     }
-    const Shape shape = pass_shape(rows, hidden, x_dtype);
+    const Shape shape = pass_shape(rows, hidden, x_dtype, branch_weight != nullptr);
     a.x = x;
     a.branch = branch;
     a.branch_weight = branch_weight;

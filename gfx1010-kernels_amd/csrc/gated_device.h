@@ -242,8 +242,16 @@ __device__ __forceinline__ float row_total(float value, int row_lanes) {
 // ----------------------------------------------------------------------------
 // Forward: one row per team and turn, as rms_device.h's.
 
+// Waves of a block: three slots are taken for rows of at most 8 (pass_shape). The
+// registers are those of four waves for each SIMD either way: a few of three slots go
+// to memory, and three waves without that are slower where it matters ([1820, 9216]
+// bf16 44 against 37 us).
+constexpr int forward_threads(int slots) {
+    return (slots == 3 ? 8 : kMaxParts) * kWave;
+}
+
 template <typename X, typename B, int V, bool kPost, Access kAccess>
-__global__ __launch_bounds__(kMaxParts * kWave) void forward_kernel(ForwardArgs a) {
+__global__ __launch_bounds__(forward_threads(V), 4) void forward_kernel(ForwardArgs a) {
     constexpr int N = kColumns<X>;
     __shared__ float sums[2][2][kMaxParts];
     const Team team = team_of(a.split);
@@ -742,10 +750,16 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 //  * Forward: two slots of a 16-bit stream, four of a 32-bit one, so that a row has
 //    half or a quarter of the waves, which wait for one another twice a row ([6001,
 //    2880] bf16 29.7 against 37.8 us with one slot, [16384, 4096] 96 against 101;
-//    [8192, 4096] fp32 72.8 against 75.0 with two slots, 116.7 with one). Launches whose
-//    waves of one slot are at most half of those that the chip holds take one slot up to
-//    8 waves a row, two beyond: their time is one row's ([512, 4096] bf16 6.0 against
-//    6.5 us, [256, 512] fp32 3.7 against 4.5 with four).
+//    [8192, 4096] fp32 72.8 against 75.0 with two slots, 116.7 with one). As many blocks
+//    of p waves fit a CU as of the next power of two, as measured: 16-bit rows of a
+//    normed branch take three slots where that power is less with them ([3640, 4608]
+//    29.0 against 41.8 us, [10922, 1536] 27.3 and 29.6, [1364, 12288] 30.4 and 37.7),
+//    and not where it is the same ([2340, 7168] 38.9 against 34.1, [2048, 8192] 36.4
+//    and 29.4). Branches without a norm wait once a row and show no difference (26.1
+//    and 26.3 at 4608); 32-bit rows of six slots are slower ([1820, 4608] 36.1 against
+//    31.1). Launches whose waves of one slot are at most half of those that the chip
+//    holds take one slot up to 8 waves a row, two beyond: their time is one row's
+//    ([512, 4096] bf16 6.0 against 6.5 us, [256, 512] fp32 3.7 against 4.5 with four).
 //  * Backward: one slot up to 16 waves a row of a 16-bit stream ([16384, 4096] bf16 155
 //    against 192 us with two: the next row's words no longer fit the registers), two
 //    from 5 vectors on of a 32-bit one ([4096, 4096] fp32 64 against 74 us, [8192, 1024]
@@ -781,7 +795,8 @@ inline void set_repeat(Factor* factor, int64_t rows) {
     }
 }
 
-inline Shape pass_shape(int64_t rows, int64_t hidden, int x_dtype) {
+// `normed`: with a branch weight.
+inline Shape pass_shape(int64_t rows, int64_t hidden, int x_dtype, bool normed) {
     if (hidden <= 32 * columns_of(x_dtype)) {
         return short_shape(hidden, x_dtype, 4);
     }
@@ -791,6 +806,16 @@ inline Shape pass_shape(int64_t rows, int64_t hidden, int x_dtype) {
     int slots = 1;
     while ((slots < wanted && slots < vectors) || slots * kMaxParts < vectors) {
         slots *= 2;
+    }
+    const auto held = [&](int of) {  // the next power of two of a row's waves
+        int waves = 1;
+        while (waves * of < vectors) {
+            waves *= 2;
+        }
+        return waves;
+    };
+    if (normed && x_dtype != RLN_DTYPE_F32 && slots == 2 && !resident && held(3) < held(2)) {
+        slots = 3;  // at most 8 waves: held(2) is at most 16
     }
     return shape_of(vectors, slots, 4);
 }

@@ -73,6 +73,11 @@ int slots(const Args& a, const Shape& shape, hipStream_t stream) {
         case 2:
             return run<X, B, 2, kPost>(a, shape, stream);
         default:
+#if RMS_PASS == 1
+            if constexpr (kColumns<X> == 8 && kPost) {
+                return run<X, B, 3, kPost>(a, shape, stream);
+            }
+#endif
             if constexpr (kColumns<X> == 4) {
                 return run<X, B, 4, kPost>(a, shape, stream);
             }

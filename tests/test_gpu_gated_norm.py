@@ -124,6 +124,18 @@ def test_shapes_of_factors(shape, gate, weight):
     check(parts, upstream_of(parts, F32), (shape, gate, weight))
 
 
+@pytest.mark.parametrize("hidden", [1025, 1288, 1535, 1536, 2048, 2303, 2304, 2880, 4607, 4608, 5120,
+                                    6143, 6144, 7168, 8190, 9215, 9216, 12287, 12288])
+@pytest.mark.parametrize("x_dtype,branch_dtype", [(BF16, BF16), (F16, F32), (F32, F16)])
+def test_launches_past_the_chip(hidden, x_dtype, branch_dtype):
+    """More rows than the chip's waves take at once, where a row has fewer waves."""
+    rows = 4096 // -(-hidden // 512) + 5
+    for post, gate in ((True, "shared"), (hidden % 2 == 0, "token")):
+        parts = reference.make((rows, hidden), [x_dtype, branch_dtype, x_dtype, F32, BF16], post=post,
+                               gate=gate, seed=hidden)
+        check(parts, upstream_of(parts, x_dtype), (hidden, x_dtype, gate))
+
+
 @pytest.mark.parametrize("rows", [1, 2, 3, 63, 64, 65, 513, 2049])
 @pytest.mark.parametrize("hidden", [24, 96, 513, 1024, 4097])
 def test_rows(rows, hidden):
