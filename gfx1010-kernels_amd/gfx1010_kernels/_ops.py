@@ -511,6 +511,9 @@ def _rotary_backward_fake(grad_q, grad_k, q, k, positions, inverse_frequencies, 
 
 
 def _rotary_setup_context(ctx, inputs, output):
+    # The operator's own kernel runs without grad mode and cannot tell.
+    if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
+        raise RuntimeError("rotary RMSNorm: positions and inverse_frequencies have no gradient")
     (q, k, positions, frequencies, ctx.sections, ctx.cyclic, ctx.interleaved, q_weight, k_weight,
      ctx.eps) = inputs
     ctx.save_for_backward(None if q_weight is None else q, None if k_weight is None else k,

@@ -34,6 +34,7 @@ MAX_TOKENS = (1 << 30) - 1
 POSITION_DTYPES = (torch.int64, torch.int32, torch.float32)
 FREQUENCY_DTYPES = (torch.float32, torch.float64)
 ARRANGEMENTS = ("blocks", "cyclic")
+_NO_TABLE_GRADIENTS = "positions and inverse_frequencies have no gradient"
 _WHAT = "rotary RMSNorm"
 
 
@@ -140,6 +141,10 @@ def _check_shapes(q, k, positions, frequencies, sections, arrangement, q_weight,
         raise ValueError("positions must broadcast over the tokens")
 
 
+def _tables_have_gradients(positions, frequencies):
+    return torch.is_grad_enabled() and (positions.requires_grad or frequencies.requires_grad)
+
+
 def _input_reason(q, k, positions, frequencies, sections, q_weight, k_weight, eps):
     """Why the native kernels cannot serve inputs that fit one another, or None."""
     heads = [tensor for tensor in (q, k) if tensor is not None]
@@ -163,8 +168,8 @@ def _input_reason(q, k, positions, frequencies, sections, q_weight, k_weight, ep
         return "positions must use int64, int32 or float32"
     if sections is not None and len(sections) > MAX_AXES:
         return f"at most {MAX_AXES} axes are supported"
-    if torch.is_grad_enabled() and (positions.requires_grad or frequencies.requires_grad):
-        return "positions and inverse_frequencies have no gradient"
+    if _tables_have_gradients(positions, frequencies):
+        return _NO_TABLE_GRADIENTS
     if q.shape[:-2].numel() > MAX_TOKENS:
         return "too many tokens"
     if not eps >= 0.0:
@@ -205,9 +210,10 @@ def rms_norm_rotary(
     Supports first-order autograd for the heads and their weights (summed in fp32 in a
     fixed order: bitwise reproducible), HIP graph capture, ``torch.compile``,
     ``torch.jit.trace`` and ``make_fx``; inputs with a forward-mode tangent, and positions or
-    frequencies that require a gradient, take the PyTorch path. The kernels serve heads of
-    1 to 256 values in fp32, fp16 and bf16. The graph keeps the heads only where they are
-    normed, and nothing else of their size.
+    frequencies that require a gradient, take the PyTorch path (the native modes raise, in
+    every kind of graph too). The kernels serve heads of up to 256 values in fp32, fp16 and
+    bf16. The graph keeps the heads only where they are normed, and nothing else of their
+    size.
     """
     ready = q.is_cuda and q.get_device() in _READY_DEVICES
     if (implementation == "auto" and ready and arrangement in ARRANGEMENTS
@@ -237,10 +243,13 @@ def rms_norm_rotary(
         return _torch_rotary(*plain)
     if torch.compiler.is_compiling():
         reason = reason_of()
-        if strict and reason == NO_TANGENTS:
+        if strict and reason in (NO_TANGENTS, _NO_TABLE_GRADIENTS):
             raise RuntimeError(f"{TARGET_ARCHITECTURE} native {_WHAT} is unavailable: {reason}")
         return rms_norm_rotary_op(*given) if strict or reason is None else _torch_rotary(*plain)
     if q.is_cuda and graph_recorded():
+        if strict and _tables_have_gradients(positions, inverse_frequencies):
+            raise RuntimeError(
+                f"{TARGET_ARCHITECTURE} native {_WHAT} is unavailable: {_NO_TABLE_GRADIENTS}")
         if not strict:
             reason = (_extension()[0].rotary_inputs_refusal(*given) if torch.jit.is_tracing()
                       else reason_of())

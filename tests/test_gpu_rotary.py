@@ -833,3 +833,75 @@ def test_the_norms_of_a_block_agree():
     first = residual_rms_norm(x, None, weight, EPS)[1]
     second = gated_residual_rms_norm(x, torch.zeros_like(x), weight, EPS, branch_weight=weight)[1]
     assert same_bits(first, second)
+
+
+# Tables that require a gradient.
+
+@pytest.mark.parametrize("table", [2, 3])
+@pytest.mark.parametrize("implementation", ["gfx950", "gfx1010"])
+def test_graphs_drop_no_gradient_of_the_tables(table, implementation):
+    """Positions or frequencies that require a gradient are refused where they would lose it, in
+    every way to the registered operator."""
+    parts = to_gpu(reference.make((2, 5), 4, 2, 32, F32, position_dtype=F32, seed=27))
+    parts[2] = parts[2][0]
+    plain = list(parts)
+    parts[table] = parts[table].clone().requires_grad_()
+
+    def function(*given):
+        return call(given, implementation=implementation)
+
+    refused = "positions and inverse_frequencies have no gradient"
+    for fullgraph in (False, True):
+        torch._dynamo.reset()
+        with pytest.raises(RuntimeError, match=refused):
+            torch.compile(function, backend="aot_eager", fullgraph=fullgraph)(*parts)
+    with pytest.raises(RuntimeError, match=refused):
+        make_fx(function)(*parts)
+    operator = torch.ops.gfx1010_kernels.rotary_forward
+    with pytest.raises(RuntimeError, match=refused):
+        operator(*parts[:4], [], False, False, *parts[4:], EPS)
+    with warnings.catch_warnings(), torch.no_grad():
+        warnings.simplefilter("ignore")
+        traced = torch.jit.trace(function, plain)
+        expected = call(parts)
+        for found in (operator(*parts[:4], [], False, False, *parts[4:], EPS), traced(*parts)):
+            assert all(same_bits(a, b) for a, b in zip(found, expected))
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        with pytest.raises(RuntimeError, match=refused):
+            torch.jit.trace(function, parts, check_trace=False)
+    with pytest.raises(RuntimeError, match=refused):
+        traced(*parts)
+
+
+@pytest.mark.parametrize("table", [2, 3])
+def test_compiled_auto_calls_differentiate_the_tables(table):
+    """A gradient is a sum of upstream (a cosine) * turned value * the other table over heads and
+    tokens or pairs, S = |n1| + |n2| bounding the turned values. A term carries 28 u of the norm and
+    the turn, as much times S through the cosine, and 8 u of its own products; the sum adds its
+    number of terms. Both runs are that near to the formula's value."""
+    parts = to_gpu(reference.make((2, 5), 4, 2, 32, F32, position_dtype=F32, seed=27))
+    parts[2] = parts[2][0] % 7
+
+    def function(*given):
+        q, k = call(given, implementation="auto")
+        return q.sin().sum() + k.sin().sum()
+
+    grads = []
+    for run in (function, torch.compile(function, backend="aot_eager", fullgraph=True)):
+        torch._dynamo.reset()
+        given = list(parts)
+        given[table] = given[table].clone().requires_grad_()
+        with warnings.catch_warnings():
+            warnings.simplefilter("ignore")  # the PyTorch path says that it is taken
+            grads.append(torch.autograd.grad(run(*given), given[table])[0].double())
+    size = torch.cat([reference.pair_size(
+        heads.double() * reference.rstd_of(heads.double(), EPS) * weight.double(), 16, False)
+        for heads, weight in ((parts[0], parts[4]), (parts[1], parts[5]))], 2)
+    other = parts[3].double() if table == 2 else parts[2].double()[..., None]
+    over = (2, 3) if table == 2 else (0, 1, 2)  # both values of a pair among the terms
+    sums = (size * (other.repeat(2) if table == 2 else other[..., None]).abs()).sum(over)
+    sums = sums if table == 2 else sums[:16] + sums[16:]
+    bound = 2 * (36 + 28 * size.max() + size.numel()) * 2.0 ** -24 * sums
+    assert grads[0].any()
+    assert ((grads[0] - grads[1]).abs() <= bound).all()

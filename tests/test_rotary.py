@@ -331,3 +331,50 @@ def test_fake_shapes():
             grads = ops.rotary_backward(q, given, q, None, *rest, 7)
             assert grads[0].shape == q.shape and grads[2].shape == weight.shape
             assert grads[1].shape == k_out.shape and grads[3].shape == (0,)
+
+
+def fake_inputs(of_positions, of_frequencies):
+    """Fake HIP tensors; either table may require a gradient."""
+    q = torch.empty(2, 3, 4, 16, device="cuda").requires_grad_()
+    positions = torch.empty(2, 3, device="cuda").requires_grad_(of_positions)
+    return q, None, positions, torch.empty(8, device="cuda").requires_grad_(of_frequencies)
+
+
+@pytest.mark.parametrize("of_positions,of_frequencies", [(True, False), (False, True)])
+@pytest.mark.parametrize("heads_require", [True, False])
+def test_the_registered_operator_drops_no_gradient(of_positions, of_frequencies, heads_require):
+    """Its kernel runs without grad mode: what cannot be differentiated is refused above it."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    forward = torch.ops.gfx1010_kernels.rotary_forward
+    rest = ([], False, False, None, None, EPS)
+    with FakeTensorMode():
+        given = fake_inputs(of_positions, of_frequencies)
+        given[0].requires_grad_(heads_require)
+        with pytest.raises(RuntimeError, match="positions and inverse_frequencies have no gradient"):
+            forward(*given, *rest)
+        with torch.no_grad():
+            assert not forward(*given, *rest)[0].requires_grad
+        assert forward(given[0].requires_grad_(), None, *(t.detach() for t in given[2:]),
+                       *rest)[0].requires_grad
+
+
+@pytest.mark.parametrize("of_positions,of_frequencies", [(True, False), (False, True)])
+@pytest.mark.parametrize("implementation", ["gfx950", "gfx1010"])
+@pytest.mark.parametrize("recorder", ["compile", "trace"])
+def test_strict_modes_refuse_gradients_of_tables_in_graphs(of_positions, of_frequencies,
+                                                           implementation, recorder, monkeypatch):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    if recorder == "compile":
+        monkeypatch.setattr(torch.compiler, "is_compiling", lambda: True)
+    else:
+        monkeypatch.setattr(rotary, "graph_recorded", lambda: True)
+    # What is reached behind the refusal: nothing of these calls.
+    monkeypatch.setattr(rotary, "rms_norm_rotary_op", lambda *given: given)
+    with FakeTensorMode():
+        given = fake_inputs(of_positions, of_frequencies)
+        with pytest.raises(RuntimeError, match="unavailable: positions and inverse_frequencies"):
+            rms_norm_rotary(*given, implementation=implementation)
+        with torch.no_grad():
+            assert rms_norm_rotary(*given, implementation=implementation)[0] is given[0]
