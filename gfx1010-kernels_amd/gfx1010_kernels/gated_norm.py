@@ -104,7 +104,8 @@ def _input_reason(x, branch, weight, branch_weight, gate, eps, branch_eps, resid
         return "gate and weight must match the hidden size"
     if not (eps >= 0.0 and branch_eps >= 0.0):
         return "eps must not be negative"
-    if not (math.isfinite(residual_scale) and math.isfinite(branch_scale)):
+    # By comparisons, which a graph of torch.compile with symbolic numbers can hold.
+    if not all(-math.inf < scale < math.inf for scale in (residual_scale, branch_scale)):
         return "residual_scale and branch_scale must be finite"
     return None
 

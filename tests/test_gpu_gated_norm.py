@@ -747,3 +747,38 @@ def test_without_gate_and_weight_it_is_the_residual_norm():
         for a, b in zip(call([x, branch, weight, None, None]),
                         residual_rms_norm(x, branch, weight, EPS, implementation="gfx950")):
             assert same_bits(a, b)
+
+
+@pytest.mark.parametrize("dynamic", [None, True])
+def test_compiled_calls_of_several_scales(dynamic):
+    """A number that changes from call to call becomes a symbol of the compiled graph."""
+    parts = to_gpu(reference.make((2, 3, 64), [F32] * 5, seed=31))
+    upstream = [torch.randn_like(parts[0]) for _ in range(2)]
+
+    def function(*given, residual_scale, branch_scale, eps):
+        x, branch, weight, post, gate = given
+        return gated_residual_rms_norm(
+            x, branch, weight, eps, branch_weight=post, gate=gate, branch_eps=2 * eps,
+            residual_scale=residual_scale, branch_scale=branch_scale)
+
+    torch._dynamo.reset()
+    compiled = torch.compile(function, backend="aot_eager", fullgraph=True, dynamic=dynamic)
+    for number in (1.0, 0.5, 0.22, 3.0):
+        options = dict(residual_scale=number, branch_scale=1.0 - number / 4, eps=number * 1e-6)
+        found = []
+        for run in (function, compiled):
+            leaves = [t.clone().requires_grad_() for t in parts]
+            outputs = run(*leaves, **options)
+            found.append([*outputs, *torch.autograd.grad(outputs, leaves, upstream)])
+        for a, b in zip(*found):
+            assert same_bits(a, b), number
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("which", ["residual_scale", "branch_scale"])
+def test_scales_that_are_not_finite_take_the_torch_path(bad, which):
+    parts = to_gpu(reference.make((2, 3, 64), [F32] * 5, seed=31))
+    with pytest.warns(RuntimeWarning, match="must be finite"):
+        gated_residual_rms_norm(*parts[:3], **{which: bad})
+    with pytest.raises(RuntimeError, match="must be finite"):
+        gated_residual_rms_norm(*parts[:3], **{which: bad}, implementation="gfx950")
