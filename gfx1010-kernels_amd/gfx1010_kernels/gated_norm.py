@@ -118,6 +118,14 @@ def _traced_reason(*args):
     return _input_reason(*args)
 
 
+def check_scales(residual_scale, branch_scale):
+    """Scales are numbers; a tensor's gradient would be lost with its conversion."""
+    for name, scale in (("residual_scale", residual_scale), ("branch_scale", branch_scale)):
+        if isinstance(scale, torch.Tensor) and scale.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} is a number and has no gradient: pass a learned scale of "
+                             "the branch as its gate")
+
+
 def _check_shapes(x, branch, weight, branch_weight, gate):
     """What no implementation takes: tensors that do not fit one another."""
     if x.ndim < 1 or branch.shape != x.shape:
@@ -151,10 +159,10 @@ def gated_residual_rms_norm(
     norm of it; returns ``(updated, normalized)``.
 
     ``branch`` has ``x``'s shape ``[..., hidden]``. With ``branch_weight`` (``[hidden]``) it is
-    normed first, with ``branch_eps`` (None: ``eps``). ``gate`` is None, ``[hidden]``, or has
-    ``x``'s leading dimensions from the first one on and 1 in the rest (``[batch, 1,
-    hidden]`` for one a sample, ``x``'s shape for one a token); ``weight``, of the last
-    norm, may have the same shapes. ``updated`` is computed in fp32 and rounded to
+    normed first, with ``branch_eps`` (None: ``eps``). The scales are numbers; one that is
+    learned is a gate. ``gate`` is None, ``[hidden]``, or has ``x``'s leading dimensions from
+    the first one on and 1 in the rest (``[batch, 1, hidden]`` for one a sample, ``x``'s shape
+    for one a token); ``weight``, of the last norm, may have the same shapes. ``updated`` is computed in fp32 and rounded to
     ``x``'s type, ``normalized`` is the norm of the rounded stream in ``x``'s type or
     ``normalized_dtype``. Every tensor uses fp32, fp16 or bf16, each its own; tensors
     whose rows are evenly spaced are read in place. The kernels take 1 to 16384 columns
@@ -169,6 +177,8 @@ def gated_residual_rms_norm(
     reproducible). The graph keeps ``updated``, ``branch`` and the factors, and four or
     eight bytes per row.
     """
+    if type(residual_scale) is not float or type(branch_scale) is not float:
+        check_scales(residual_scale, branch_scale)
     if (implementation == "auto" and x.is_cuda and x.get_device() in _READY_DEVICES
             and normalized_dtype in _DTYPES_OR_NONE and not torch.compiler.is_compiling()):
         result = _extension()[0].gated_residual_rms_norm_if_supported(

@@ -33,7 +33,7 @@ import torch
 from torch import nn
 from torch.nn import functional as F
 
-from .gated_norm import gated_residual_rms_norm
+from .gated_norm import check_scales, gated_residual_rms_norm
 from .normalization import residual_layer_norm
 from .rms_norm import residual_rms_norm
 
@@ -112,6 +112,8 @@ def residual_norm(x, branch, norm: Union[nn.LayerNorm, nn.RMSNorm], dropout_p: f
     branch_norm(dropout(branch))`` and its norm.
     """
     _check_norm(norm, x.shape[-1])
+    if type(residual_scale) is not float or type(branch_scale) is not float:
+        check_scales(residual_scale, branch_scale)  # a learned one may be 1 at the start
     if (branch_norm is not None or gate is not None or residual_scale != 1.0
             or branch_scale != 1.0):
         return _gated_norm(x, branch, norm, branch_norm, gate, residual_scale, branch_scale,

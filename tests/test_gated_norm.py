@@ -361,3 +361,27 @@ def test_without_gate_and_weight_it_is_the_residual_norm():
     for a, b in zip(gated_residual_rms_norm(x, branch, weight, EPS, **options),
                     residual_rms_norm(x, branch, weight, EPS, **options)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("value", [1.0, 0.5])
+@pytest.mark.parametrize("which", ["residual_scale", "branch_scale"])
+def test_scales_lose_no_gradient(which, value):
+    """A scale is a number; a tensor that requires a gradient is refused, whatever it holds."""
+    import numpy as np
+
+    x, branch, weight, _, _ = reference.make((2, 3, 8), [torch.float32] * 5)
+    scale = {which: torch.nn.Parameter(torch.tensor(value))}
+    norm = torch.nn.RMSNorm(8, eps=1e-6)
+    for implementation in ("auto", "torch", "gfx950"):
+        with pytest.raises(ValueError, match=f"{which} is a number"):
+            gated_residual_rms_norm(x, branch, weight, **scale, implementation=implementation)
+        with pytest.raises(ValueError, match=f"{which} is a number"):
+            residual_norm(x, branch, norm, **scale, implementation=implementation)
+    number = {which: value}
+    for given in (scale, {which: torch.tensor(value)}, {which: np.float32(value)}):
+        with torch.no_grad():
+            for a, b in zip(gated_residual_rms_norm(x, branch, weight, **given,
+                                                    implementation="torch"),
+                            gated_residual_rms_norm(x, branch, weight, **number,
+                                                    implementation="torch")):
+                assert torch.equal(a, b)
