@@ -114,6 +114,18 @@ def _broadcasts(sizes, over):
     return missing >= 0 and all(size in (1, whole) for size, whole in zip(sizes, over[missing:]))
 
 
+def _whole_sections(sections):
+    """``sections`` as a tuple of ints; any sequence of whole numbers."""
+    if sections is None:
+        return None
+    whole = tuple(int(section) for section in sections)
+    if not whole:
+        raise ValueError("sections must hold at least one number of pairs")
+    if any(own != section for own, section in zip(whole, sections)):
+        raise ValueError("sections must be whole numbers of pairs")
+    return whole
+
+
 def _check_shapes(q, k, positions, frequencies, sections, arrangement, q_weight, k_weight):
     """What no implementation takes: tensors that do not fit one another."""
     if arrangement not in ARRANGEMENTS:
@@ -218,16 +230,18 @@ def rms_norm_rotary(
     ready = q.is_cuda and q.get_device() in _READY_DEVICES
     if (implementation == "auto" and ready and arrangement in ARRANGEMENTS
             and (sections is None or len(sections) > 0) and not torch.compiler.is_compiling()):
-        result = _extension()[0].rms_norm_rotary_if_supported(
-            q, k, positions, inverse_frequencies, () if sections is None else sections,
-            arrangement == "cyclic", interleaved, q_weight, k_weight, float(eps))
+        try:
+            result = _extension()[0].rms_norm_rotary_if_supported(
+                q, k, positions, inverse_frequencies, () if sections is None else sections,
+                arrangement == "cyclic", interleaved, q_weight, k_weight, float(eps))
+        except TypeError:  # sections of another kind than the extension takes, among others
+            if sections is None:
+                raise
+            result = None
         if result is not None:
             return result
     _check_implementation(implementation, _WHAT)
-    if sections is not None:
-        sections = tuple(int(section) for section in sections)
-        if not sections:
-            raise ValueError("sections must hold at least one number of pairs")
+    sections = _whole_sections(sections)
     args = (q, k, positions, inverse_frequencies)
     _check_shapes(*args, sections, arrangement, q_weight, k_weight)
     eps = float(eps)
@@ -266,6 +280,7 @@ def can_use_rms_norm_rotary(q, k, positions, inverse_frequencies, *, sections=No
                             eps=1e-6):
     """True when ``implementation="auto"`` runs natively."""
     try:
+        sections = _whole_sections(sections)
         _check_shapes(q, k, positions, inverse_frequencies, sections, arrangement, q_weight,
                       k_weight)
     except ValueError:

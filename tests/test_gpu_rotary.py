@@ -905,3 +905,22 @@ def test_compiled_auto_calls_differentiate_the_tables(table):
     bound = 2 * (36 + 28 * size.max() + size.numel()) * 2.0 ** -24 * sums
     assert grads[0].any()
     assert ((grads[0] - grads[1]).abs() <= bound).all()
+
+
+def test_sections_are_any_sequence_of_whole_numbers():
+    """In every mode, on the first call and on later ones."""
+    from test_rotary import sections_of_every_kind
+
+    parts = to_gpu(reference.make((2, 5), 4, 2, 32, F32, axes=2, seed=28))
+    keywords = dict(q_weight=parts[4], k_weight=parts[5])
+    expected = call(parts, sections=(9, 7))
+    for implementation in ("auto", "gfx950", "gfx1010"):
+        for sections in sections_of_every_kind((9, 7)):
+            found = call(parts, sections=sections, implementation=implementation)
+            assert all(same_bits(a, b) for a, b in zip(found, expected)), type(sections)
+            assert can_use_rms_norm_rotary(*parts[:4], sections=sections, **keywords)
+    for sections in ((9.5, 6.5), torch.tensor([9.5, 6.5])):
+        for implementation in ("auto", "gfx950", "torch"):
+            with pytest.raises(ValueError, match="whole numbers"):
+                call(parts, sections=sections, implementation=implementation)
+        assert not can_use_rms_norm_rotary(*parts[:4], sections=sections, **keywords)

@@ -378,3 +378,23 @@ def test_strict_modes_refuse_gradients_of_tables_in_graphs(of_positions, of_freq
             rms_norm_rotary(*given, implementation=implementation)
         with torch.no_grad():
             assert rms_norm_rotary(*given, implementation=implementation)[0] is given[0]
+
+
+def sections_of_every_kind(numbers):
+    import numpy as np
+
+    return [tuple(numbers), list(numbers), torch.Size(numbers), np.array(numbers),
+            torch.tensor(numbers), [np.int32(number) for number in numbers],
+            tuple(float(number) for number in numbers)]
+
+
+def test_sections_are_any_sequence_of_whole_numbers():
+    given = dict(inputs(), implementation="torch")
+    given["positions"] = torch.stack([given["positions"], given["positions"] + 3])
+    expected = rms_norm_rotary(**given, sections=(5, 3))
+    for sections in sections_of_every_kind((5, 3)):
+        for a, b in zip(rms_norm_rotary(**given, sections=sections), expected):
+            assert torch.equal(a, b), type(sections)
+    for sections in ((5.5, 2.5), torch.tensor([5.5, 2.5]), (8.5, -0.5)):
+        with pytest.raises(ValueError, match="whole numbers"):
+            rms_norm_rotary(**given, sections=sections)
