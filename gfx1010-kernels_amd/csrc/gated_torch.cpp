@@ -168,8 +168,7 @@ std::tuple<at::Tensor, at::Tensor> forward_impl(
     int64_t branch_stride = 0;
     const auto x = as_rows(in.x, &x_stride);
     const auto branch = as_rows(in.branch, &branch_stride);
-    const auto branch_weight =
-        in.branch_weight.defined() ? in.branch_weight.contiguous() : at::Tensor();
+    const auto branch_weight = dense(in.branch_weight);
     at::Tensor gate_kept;
     at::Tensor weight_kept;
     const rln_factor_t gate = factor_of(in.gate, in.x, &gate_kept);
@@ -232,9 +231,6 @@ std::vector<at::Tensor> backward_impl(
     if (rows == 0) {
         return {grad_x, grad_branch, grad_weight, grad_branch_weight, grad_gate};
     }
-    const auto dense = [](const at::Tensor& tensor) {
-        return tensor.defined() ? tensor.contiguous() : tensor;
-    };
     const auto updated = dense(updated_in);
     const auto grad_updated = dense(grad_updated_in);
     const auto grad_normalized = dense(grad_normalized_in);

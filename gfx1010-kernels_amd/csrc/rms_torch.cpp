@@ -116,7 +116,7 @@ std::tuple<at::Tensor, at::Tensor> forward_impl(
     }
     int64_t branch_stride = 0;
     const auto branch_rows = branch.defined() ? as_rows(branch, &branch_stride) : branch;
-    const auto weight_row = weight.contiguous();
+    const auto weight_row = dense(weight);
     const bool codes = kept != nullptr && checkpoint;
     check_status(rln_rms_forward(
         x_rows.data_ptr(), dtype_of(x.scalar_type()), x_stride,
@@ -180,10 +180,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> backward_impl(
         updated_rows = as_rows(updated, &updated_stride);
     }
     c10::hip::HIPGuardMasqueradingAsCUDA guard(device);
-    const auto grad_normalized = grad_normalized_in.contiguous();
-    const auto grad_updated =
-        grad_updated_in.defined() ? grad_updated_in.contiguous() : grad_updated_in;
-    const auto weight_row = weight.contiguous();
+    const auto grad_normalized = dense(grad_normalized_in);
+    const auto grad_updated = dense(grad_updated_in);
+    const auto weight_row = dense(weight);
     auto grad_x = empty_device(grad_normalized.sizes(), x_type, device);
     auto grad_branch = branch_type && *branch_type != x_type
         ? empty_device(grad_normalized.sizes(), *branch_type, device) : at::Tensor();
@@ -561,7 +560,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> residual_rms_norm_quantized(
     const auto x_rows = as_rows(x, &x_stride);
     int64_t branch_stride = 0;
     const auto branch_rows = branch.defined() ? as_rows(branch, &branch_stride) : branch;
-    const auto weight_row = weight.contiguous();
+    const auto weight_row = dense(weight);
     check_status(rln_rms_quantize(
         x_rows.data_ptr(), dtype_of(x.scalar_type()), x_stride,
         branch.defined() ? branch_rows.data_ptr() : nullptr,
@@ -605,8 +604,8 @@ at::Tensor dequantize(const at::Tensor& quantized, const at::Tensor& scale, int6
     TORCH_CHECK(scale.sizes() == at::IntArrayRef(scale_sizes(quantized.sizes(), group)),
                 "scale must have one value for each group of columns");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(quantized.device());
-    const auto codes = quantized.contiguous();
-    const auto scales = scale.contiguous();
+    const auto codes = dense(quantized);
+    const auto scales = dense(scale);
     auto values = empty_device_like(codes, dtype);
     if (values.numel() == 0) {
         return values;

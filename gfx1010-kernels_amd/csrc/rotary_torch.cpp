@@ -158,7 +158,7 @@ void check_inputs(const Inputs& in) {
 // Heads as [outer, inner, heads, size] with consecutive elements: views where the
 // strides allow it, copies elsewhere.
 at::Tensor as_heads(const at::Tensor& heads) {
-    at::Tensor out = heads;
+    at::Tensor out = stored(heads);
     if (out.size(-1) != 1 && out.stride(-1) != 1) {
         out = out.contiguous();
     }
@@ -187,7 +187,10 @@ void fill_rotary(const Inputs& in, at::IntArrayRef lead, Rotary* out) {
     const int64_t axes = in.sections.empty() ? 1 : static_cast<int64_t>(in.sections.size());
     std::vector<int64_t> sizes{axes};
     sizes.insert(sizes.end(), lead.begin(), lead.end());
-    at::Tensor positions = in.sections.empty() ? in.positions.unsqueeze(0) : in.positions;
+    at::Tensor positions = stored(in.positions);
+    if (in.sections.empty()) {
+        positions = positions.unsqueeze(0);
+    }
     // The axes stay in front of tokens that broadcast.
     while (positions.dim() < static_cast<int64_t>(sizes.size())) {
         positions = positions.unsqueeze(1);
@@ -200,7 +203,7 @@ void fill_rotary(const Inputs& in, at::IntArrayRef lead, Rotary* out) {
         positions = positions.flatten(1, -2);
     }
     out->positions = positions;
-    out->frequencies = in.frequencies.contiguous();
+    out->frequencies = dense(in.frequencies);
     out->outer = positions.size(1);
     out->inner = positions.size(2);
     const int64_t pairs = in.frequencies.size(0);
@@ -288,7 +291,7 @@ std::tuple<at::Tensor, at::Tensor> forward_impl(const Inputs& in) {
             continue;
         }
         kept[i] = as_heads(*heads[i]);
-        weights[i] = given[i]->defined() ? given[i]->contiguous() : at::Tensor();
+        weights[i] = dense(*given[i]);
         sides[i].heads = heads_of(kept[i]);
         sides[i].count = kept[i].size(2);
         sides[i].weight = data_or_null(weights[i]);
@@ -363,7 +366,7 @@ std::vector<at::Tensor> backward_impl(
         sides[i].output = results[i].data_ptr();
         if (normed) {
             kept[i][1] = as_heads(*heads[i]);
-            weights[i] = given[i]->contiguous();
+            weights[i] = dense(*given[i]);
             sides[i].heads = heads_of(kept[i][1]);
             sides[i].weight = weights[i].data_ptr();
             sides[i].weight_dtype = dtype_of(weights[i].scalar_type());

@@ -36,9 +36,21 @@ inline std::optional<int64_t> row_stride(const at::Tensor& tensor) {
     return stride;
 }
 
+// `tensor` with its values in memory: the imaginary part of a conjugate is a view
+// whose elements are negated as they are read.
+inline at::Tensor stored(const at::Tensor& tensor) {
+    return tensor.is_neg() ? tensor.resolve_neg() : tensor;
+}
+
+// `tensor` as one dense run of values; undefined where it is.
+inline at::Tensor dense(const at::Tensor& tensor) {
+    return tensor.defined() ? stored(tensor.contiguous()) : tensor;
+}
+
 // `tensor` with rows of consecutive elements one stride apart, copied only
 // where it has none.
-inline at::Tensor as_rows(const at::Tensor& tensor, int64_t* stride) {
+inline at::Tensor as_rows(const at::Tensor& given, int64_t* stride) {
+    const auto tensor = stored(given);
     const auto found = row_stride(tensor);
     *stride = found.value_or(tensor.size(-1));
     return found ? tensor : tensor.contiguous();
