@@ -129,7 +129,6 @@ struct SumArgs {
     void* grad_weight;
     int64_t groups;
     int64_t group_units;
-    int64_t rows;
     int concurrent;
     int hidden;
     int branch_weight_dtype;
@@ -458,7 +457,6 @@ int rln_gated_backward(
     sum.grad_weight = grad_weight;
     sum.groups = units.groups;
     sum.group_units = units.group_units;
-    sum.rows = rows;
     sum.concurrent = 1;
     while (sum.concurrent < units.groups && sum.concurrent < kSumSlots) {
         sum.concurrent *= 2;

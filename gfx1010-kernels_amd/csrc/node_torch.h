@@ -25,10 +25,6 @@ struct Held {
     std::vector<int64_t> integers;
     std::vector<double> numbers;
     int64_t needed = 0;  // bit i: the gradient of input i is asked for
-
-    bool needs(int input) const {
-        return needed >> input & 1;
-    }
 };
 
 // Operator: `name` (static const char*), `gradients(grads, held)` (static).

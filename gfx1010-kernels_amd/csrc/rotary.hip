@@ -568,7 +568,7 @@ __global__ __launch_bounds__(kThreads, waves_of(kPass, N)) void heads_kernel(Arg
             for (int half = 0; half < 2; ++half) {
                 store_vector<kWhole, T, N>(to, place, half, values[half]);
             }
-            }
+        }
         __syncthreads();  // the tile's angles are read before the next one's are written
     }
     if constexpr (kSums) {
