@@ -586,8 +586,8 @@ typedef struct rln_rotary_side_t {
 
 /*
  * Forward, of outer * inner tokens (no counterpart in the reference): q->output and
- * k->output from q->heads and k->heads. size is 1 to 256, and outer * inner and the
- * number of heads fit 31 bits. No output may overlap an input.
+ * k->output from q->heads and k->heads. size is at most 256, outer * inner at most
+ * 2^30 - 1, and each side has at most 65536 heads. No output may overlap an input.
  */
 int rln_rotary_forward(
     const rln_rotary_side_t* q,

@@ -398,3 +398,20 @@ def test_sections_are_any_sequence_of_whole_numbers():
     for sections in ((5.5, 2.5), torch.tensor([5.5, 2.5]), (8.5, -0.5)):
         with pytest.raises(ValueError, match="whole numbers"):
             rms_norm_rotary(**given, sections=sections)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_limits_are_those_of_the_header(backward):
+    """At each limit a later check answers, past it the limit's own."""
+    last = side(output=None)
+    for outer, inner in ((1, (1 << 30) - 1), ((1 << 30) - 1, 1), (3, (1 << 30) // 3)):
+        assert "output must not" in run(backward, q=last, outer=outer, inner=inner)
+    for outer, inner in ((1, 1 << 30), (1 << 30, 1), (1 << 15, 1 << 15), (3, (1 << 30) // 3 + 1)):
+        assert "number of tokens" in run(backward, q=last, outer=outer, inner=inner)
+    assert "output must not" in run(backward, q=side(output=None, count=1 << 16))
+    assert "output must not" in run(backward, k=side(output=None, count=1 << 16))
+    assert "number of heads" in run(backward, q=side(output=None, count=(1 << 16) + 1))
+    assert "number of heads" in run(backward, k=side(output=None, count=(1 << 16) + 1))
+    assert "output must not" in run(backward, q=last, size=256)
+    assert "output must not" in run(backward, q=last, size=2, rotary=table(pairs=1))
+    assert "pairs must be" in run(backward, q=last, size=1, rotary=table(pairs=1))
