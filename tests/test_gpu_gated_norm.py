@@ -782,3 +782,37 @@ def test_scales_that_are_not_finite_take_the_torch_path(bad, which):
         gated_residual_rms_norm(*parts[:3], **{which: bad})
     with pytest.raises(RuntimeError, match="must be finite"):
         gated_residual_rms_norm(*parts[:3], **{which: bad}, implementation="gfx950")
+
+
+def test_what_transforms_and_fake_tensors_are_refused_for():
+    """The kernels ask for addresses, which a transform's tensor does not have and a fake output's
+    are null."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    parts = to_gpu(reference.make((2, 3, 64), [F32] * 5, gate="shared"))
+    call(parts, implementation="auto")
+    for implementation in ("auto", "gfx950"):
+        options = dict(implementation=implementation)
+        for place in range(5):
+            with pytest.raises(RuntimeError, match="data pointer"):
+                torch.func.grad(lambda t: call([*parts[:place], t, *parts[place + 1:]],
+                                               **options)[1].sum())(parts[place])
+        with pytest.raises(RuntimeError, match="data pointer"):
+            torch.func.vmap(lambda t, b: call([t, b, *parts[2:]], **options)[1])(*parts[:2])
+        with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(
+                RuntimeError, match="must not be null|data is not allocated"):
+            call(parts, **options)
+        assert call(parts, **options)[1].isfinite().all()
+
+
+@pytest.mark.parametrize("gate", ["none", "shared", "token"])
+@pytest.mark.parametrize("shape,x_dtype", [((1, 1, 96), F32), ((3, 5, 1027), BF16),
+                                           ((3, 1237, 264), BF16), ((2, 1500, 40), F16),
+                                           ((2, 301, 4096), BF16), ((2, 150, 8200), F32)])
+def test_a_weight_for_each_token(gate, shape, x_dtype):
+    """Every row is then a group of its own, whatever the gate, up to more groups than the launch
+    has blocks at once and than the sums take in one turn."""
+    for post in (True, False):
+        parts = reference.make(shape, [x_dtype, BF16, x_dtype, F32, x_dtype], post=post, gate=gate,
+                               weight="token", seed=33)
+        check(parts, upstream_of(parts, x_dtype), (gate, shape, post), branch_scale=0.3)

@@ -924,3 +924,73 @@ def test_sections_are_any_sequence_of_whole_numbers():
             with pytest.raises(ValueError, match="whole numbers"):
                 call(parts, sections=sections, implementation=implementation)
         assert not can_use_rms_norm_rotary(*parts[:4], sections=sections, **keywords)
+
+
+def test_what_transforms_and_fake_tensors_are_refused_for():
+    """The kernels ask for addresses, which a transform's tensor does not have and a fake output's
+    are null."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    parts = to_gpu(reference.make((2, 5), 4, 2, 32, F32, seed=25))
+    parts[2] = parts[2][0]
+    call(parts, implementation="auto")
+    for implementation in ("auto", "gfx950"):
+        options = dict(implementation=implementation)
+        with pytest.raises(RuntimeError, match="data pointer"):
+            torch.func.grad(lambda t: call([t, *parts[1:]], **options)[0].sum())(parts[0])
+        with pytest.raises(RuntimeError, match="data pointer"):
+            torch.func.vmap(lambda q, k, p: call([q, k, p, *parts[3:]], **options)[0])(*parts[:3])
+        with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(
+                RuntimeError, match="must not be null|data is not allocated"):
+            call(parts, **options)
+        assert call(parts, **options)[0].isfinite().all()
+
+
+# Tokens that are no single run: positions shared by the samples, heads before tokens.
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("dtype,size,interleaved", [(BF16, 128, False), (F16, 72, True),
+                                                    (F32, 37, False)])
+@pytest.mark.parametrize("tokens", [(3, 1), (3, 37), (1, 401), (2, 1283), (2, 3, 130)])
+def test_shared_positions_are_those_of_each_sample(norm, dtype, size, interleaved, tokens):
+    """A step with positions that repeat over the samples against one with positions of their own,
+    bit for bit but for the weights' sums, whose order may differ: those against the reference. The
+    longest fill several tiles and more than one per block."""
+    parts = reference.make(tokens, 3, 2, size, dtype, norm=norm, axes=2, seed=29)
+    options = dict(sections=(size // 2 - 4, 4), interleaved=interleaved)
+    shared = parts[2].reshape(2, -1, tokens[-1])[:, 0]
+    whole = shared.reshape(2, *[1] * (len(tokens) - 1), -1).expand(2, *tokens).contiguous()
+    upstream = upstream_of(parts, 29)
+    found, expected = (
+        step(to_gpu([*parts[:2], positions, *parts[3:]]), [t.cuda() for t in upstream], **options)
+        for positions in (shared, whole))
+    for a, b in zip([*found[0], *found[1][:2]], [*expected[0], *expected[1][:2]]):
+        assert same_bits(a, b)
+    angles = reference.angles_of(shared, parts[3], options["sections"], "blocks", tokens)
+    for i in range(2):
+        reference.check_gradients(None, found[1][2 + i], parts[i], parts[4 + i], upstream[i],
+                                  angles, interleaved, EPS, i)
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("dtype,size", [(BF16, 128), (F16, 64), (F32, 80)])
+@pytest.mark.parametrize("tokens", [(1, 1), (4, 1), (3, 37), (2, 1283)])
+def test_heads_before_tokens(norm, dtype, size, tokens):
+    """[batch, heads, length, size] seen as [batch, length, heads, size], both ways, with positions
+    of each sample and shared ones."""
+    parts = to_gpu(reference.make(tokens, 3, 2, size, dtype, norm=norm, seed=30))
+    upstream = [t.cuda() for t in upstream_of(parts, 30)]
+
+    def turned(heads):
+        return heads.transpose(1, 2).contiguous().transpose(1, 2)
+
+    for positions in (parts[2][0], parts[2][0, 0], parts[2][0, :1]):
+        given = [*parts[:2], positions, *parts[3:]]
+        expected = step(given, upstream)
+        found = step([*map(turned, given[:2]), *given[2:]], [turned(t) for t in upstream])
+        for a, b in zip([*found[0], *found[1][:2]], [*expected[0], *expected[1][:2]]):
+            assert same_bits(a, b)
+        angles = reference.angles_of(positions, parts[3], None, "blocks", tokens)
+        for i in range(2):
+            reference.check_gradients(None, found[1][2 + i], parts[i], parts[4 + i], upstream[i],
+                                      angles, False, EPS, i)
