@@ -764,22 +764,26 @@ __global__ __launch_bounds__(kMaxParts * kWave) void backward_kernel(BackwardArg
 //    against 192 us with two: the next row's words no longer fit the registers), two
 //    from 5 vectors on of a 32-bit one ([4096, 4096] fp32 64 against 74 us, [8192, 1024]
 //    37.4 and 37.9).
-//  * One block of about 8 waves for each CU, of 12 to 16 where a row has 5 waves or more
-//    ([16384, 4096] bf16 148 against 162 us, [8192, 2048] 46.7 and 47.8): each block
+//  * One block of about 8 waves for each CU, of 9 to 16 where a 16-bit row has 5 waves
+//    or more ([16384, 4096] bf16 148 against 162 us, [8192, 2048] 46.7 and 47.8): each block
 //    leaves two rows of partial sums, and more blocks cost more in those than they gain
 //    ([8192, 4096] fp32 111 against 114 us with two blocks). Two where a block has fewer
 //    than 8 waves, and of token gates up to 10, whose next row is not read ahead
 //    ([8192, 2048] bf16 62 against 73 us).
 //  * Rows of more columns than 16 waves of 8 hold keep their sums in LDS ([2048, 16384]
-//    bf16 113 us, 154 with sums that left the registers for memory).
+//    bf16 111-113 us, 154 with sums that left the registers for memory).
+//  * A unit's rows are of one group, so groups of fewer rows than a block has teams leave
+//    teams idle and nothing to read ahead, and each leaves two rows of partial sums ([8192,
+//    4096] bf16 with a weight for each token 733 us, 83 with one for all rows).
 
 inline Split split_of(const Shape& shape) {
     const uint32_t parts = static_cast<uint32_t>(shape.parts);
     return Split{shape.parts, teams_of(shape), ((1u << 16) + parts - 1) / parts};
 }
 
-// How a factor's row is found from the stream's: rows / `factor.rows` by a product
-// with ceil(2^(32 + s) / rows) - 2^32, s = ceil(log2(rows)), for 32-bit row numbers.
+// How a factor's row is found from the stream's: rows / `factor.rows` by the round-up
+// method of Granlund and Montgomery (1994), a product with ceil(2^(32 + s) / rows) - 2^32,
+// s = ceil(log2(rows)), for 32-bit row numbers.
 inline void set_repeat(Factor* factor, int64_t rows) {
     factor->kind = factor->rows >= rows ? kShared
         : factor->rows == 1 ? kToken : rows <= INT32_MAX ? kSample : kWideSample;

@@ -16,7 +16,9 @@
 // polynomials, about 45 operations, and all heads of a token share them. So a
 // block first makes the cosines and sines of a tile of tokens in LDS, and its lanes then
 // walk the heads of those tokens, those of q or those of k: one side's weight and sums
-// fit the registers beside a head that is read ahead.
+// fit the registers beside a head that is read ahead. Turns without a norm have neither
+// and take the same blocks, which make their angles for each side ([6001, 28 + 4 heads
+// of 128] bf16 24 us; a simpler kernel with blocks of both sides took 22).
 //
 // A head belongs to the fewest lanes, a power of two, that hold it: a lane takes two
 // vectors of 16 bytes, eight pairs of a 16-bit type (four of fp32): from each half of
@@ -26,9 +28,11 @@
 // a lane's columns, hence its weights, are the same for every head it walks.
 //
 // Measured: [16384, 32 + 8 heads of 128] bf16 with norms, forward 67 us, backward 100,
-// both 5.0 TB/s, what a large copy reaches; [8192, 12 + 12 of 64] fp16 15.5 and 25.4
-// (3.0-3.2 TB/s: the halves of such a head fill half a line each); [8858, 16 + 16 of 72]
-// fp16 24-28 (9 lanes of 16 hold a head); 16 tokens of 32 + 8 of 128 3.8.
+// both 5.0 TB/s, what a large copy reaches (in graphs 70 and 115 where 4 samples share
+// positions, 72 and 119 with heads before tokens, 69 and 113 as one run); [8192, 12 + 12
+// of 64] fp16 15.5 and 25.4 (3.0-3.2 TB/s: the halves of such a head fill half a line
+// each); [8858, 16 + 16 of 72] fp16 24-28 (9 lanes of 16 hold a head); 16 tokens of 32 +
+// 8 of 128 3.8.
 
 #include "rms_device.h"
 

@@ -158,24 +158,25 @@ def gated_residual_rms_norm(
     """Fused ``residual_scale * x + branch_scale * gate * RMS norm(branch)`` and the RMS
     norm of it; returns ``(updated, normalized)``.
 
-    ``branch`` has ``x``'s shape ``[..., hidden]``. With ``branch_weight`` (``[hidden]``) it is
-    normed first, with ``branch_eps`` (None: ``eps``). The scales are numbers; one that is
-    learned is a gate. ``gate`` is None, ``[hidden]``, or has ``x``'s leading dimensions from
-    the first one on and 1 in the rest (``[batch, 1, hidden]`` for one a sample, ``x``'s shape
-    for one a token); ``weight``, of the last norm, may have the same shapes. ``updated`` is computed in fp32 and rounded to
-    ``x``'s type, ``normalized`` is the norm of the rounded stream in ``x``'s type or
-    ``normalized_dtype``. Every tensor uses fp32, fp16 or bf16, each its own; tensors
-    whose rows are evenly spaced are read in place. The kernels take 1 to 16384 columns
-    and a gate and a weight that, where both differ between samples, differ between
-    the same ones; ``implementation="auto"`` computes other shapes that broadcast over
-    ``x`` in PyTorch, with a ``RuntimeWarning``.
+    ``branch`` has ``x``'s shape ``[..., hidden]``. With ``branch_weight`` (``[hidden]``) it
+    is normed first, with ``branch_eps`` (None: ``eps``). The scales are numbers; one that
+    is learned is a gate. ``gate`` is None, ``[hidden]``, or has ``x``'s leading dimensions
+    from the first one on and 1 in the rest (``[batch, 1, hidden]`` for one a sample,
+    ``x``'s shape for one a token); ``weight``, of the last norm, may have the same shapes.
+    ``updated`` is computed in fp32 and rounded to ``x``'s type, ``normalized`` is the norm
+    of the rounded stream in ``x``'s type or ``normalized_dtype``. Every tensor uses fp32,
+    fp16 or bf16, each its own; tensors whose rows are evenly spaced are read in place. The
+    kernels take 1 to 16384 columns and a gate and a weight that, where both differ between
+    samples, differ between the same ones; ``implementation="auto"`` computes other shapes
+    that broadcast over ``x`` in PyTorch, with a ``RuntimeWarning``.
 
     Supports first-order autograd, HIP graph capture, ``torch.compile``,
     ``torch.jit.trace`` and ``make_fx``, as :func:`residual_rms_norm` does; inputs with a
     forward-mode tangent take the PyTorch path. The gradients of ``weight``,
     ``branch_weight`` and ``gate`` are summed in fp32 in a fixed order (bitwise
-    reproducible). The graph keeps ``updated``, ``branch`` and the factors, and four or
-    eight bytes per row.
+    reproducible); a weight whose rows serve few tokens each costs several times its bytes
+    there. The graph keeps ``updated``, ``branch`` and the factors, and four or eight bytes
+    per row.
     """
     if type(residual_scale) is not float or type(branch_scale) is not float:
         check_scales(residual_scale, branch_scale)
